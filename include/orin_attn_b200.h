@@ -291,6 +291,64 @@ int oattn_prefill(const float* q, const float* k_new, const float* v_new, uint16
  * the output is not valid.  SYNCHRONOUS (a blocking device-to-host copy): for tests and diagnostics. */
 int oattn_prefill_status(const void* workspace, int n_head, int head_dim, int batch, int* status);
 
+/* ---- KV cache held in 4 bits (no counterpart in the reference) ---------------------------------------------------
+ * The same path over a cache of 4.5 bits a value instead of 16: 72 bytes a K or V row of 128 instead of 256, so a decode
+ * step reads 3.6 times less and a context takes 3.6 times less memory.
+ *
+ * Format.  One layer is oattn_kv_q4_bytes() bytes, [n_kv][ceil(n_ctx/16)][18 * head_dim]: blocks of 16 consecutive
+ * positions of one kv head, K and V together.  Layers of one cache follow each other without a gap.  A head row is cut
+ * into groups of 64 dims; a group keeps an fp16 offset m and an fp16 step d, a value is m + d * code, code 0..15:
+ *     m = fp16(min x)    d = fp16(max(0, (max x - m) / 15))    code = clamp(round((x - m) / d), 0, 15), 0 where d = 0,
+ * each evaluated exactly and rounded once, ties to even: the bytes depend on the row alone, not on the call that wrote
+ * it.  A group that holds a NaN, an infinity or a minimum beyond the fp16 range reads back as NaN.  Bytes of a block,
+ * with hd = head_dim and NG = hd/64 (little endian):
+ *     [0, 8 hd)       K codes: row s at 32-bit word s * hd/8; word t * hd/32 + i of a row (t < 4) holds dims
+ *                     32 i + 8 t + e, dim e in bits 4e..4e+3
+ *     [8 hd, 16 hd)   V codes: one byte per row and pair of dims 2p, 2p+1 (the even one in the low half); with p = 8 j + r and
+ *                     row 8 h + 2 t + u the byte is at (j/4) * 512 + (4 r + t) * 16 + (j%4) * 4 + 2 u + h
+ *     then            K steps and offsets, fp16 [16 rows][NG][d, m], and the same for V
+ * A byte belongs to one row: writing a row leaves the bytes of every other row as they are.  Rows that were never
+ * written may hold anything; no call lets them into a result.
+ *
+ * `cache` must be 16-byte aligned; k, v, q, k_new, v_new and out likewise.  head_dim 64 or 128. */
+size_t oattn_kv_q4_bytes(int n_kv, int head_dim, int n_ctx);
+
+/* oattn_kv_store into the 4-bit cache: rows k, v [batch][heads][head_dim] fp32 at positions pos_base + b, or with d_pos
+ * one row at *d_pos (batch 1, pos_base ignored; a position outside [0, n_ctx) writes nothing). */
+int oattn_kv_store_q4(void* cache, const float* k, const float* v, int heads, int head_dim, int n_ctx, int pos_base, int batch,
+                      const int* d_pos, void* stream);
+
+/* Reads rows [row_base, row_base + rows) back as fp16, m + d * code rounded to nearest: into kc, vc [heads][dst_ctx][head_dim]
+ * from row dst_base on -- an fp16 cache, or a plain [heads][rows][head_dim] block with dst_ctx = rows, dst_base = 0.
+ * kc and vc must be 16-byte aligned. */
+int oattn_kv_load_q4(const void* cache, uint16_t* kc, uint16_t* vc, int heads, int head_dim, int n_ctx, int row_base, int rows,
+                     int dst_ctx, int dst_base, void* stream);
+
+/* oattn_kv_shift on the 4-bit cache of all layers: rows [n_keep, n_keep + shift) are dropped, the rest slides left, the last
+ * `shift` rows read back as zero.  The codes move as they are: nothing is quantised again.  In place, no scratch. */
+int oattn_kv_shift_q4(void* cache, int n_layer, int n_kv, int head_dim, int n_ctx, int n_keep, int shift, void* stream);
+
+/* oattn_decode_ex on the 4-bit cache (ext may be NULL): q attends over rows 0..*d_pos; with OATTN_FUSE_KV_APPEND the new row is
+ * [biased, normed, rotated,] quantised and stored at row *d_pos in the same launch.  k_new is rotated in double and rounded
+ * to fp32 before it is quantised (q in fp32, as in oattn_decode).  The result has fp32 accuracy: the codes are exact, q and the
+ * softmax weights enter the products as two fp16 halves.  ONE launch; oattn_set_decode_overlap applies.  The workspace rules
+ * are those of oattn_decode_workspace_bytes: calls that may run at the same time, graph replays among them, need
+ * workspaces of their own. */
+size_t oattn_decode_q4_workspace_bytes(int n_head, int n_kv, int head_dim);
+int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, int n_head, int n_kv,
+                    int head_dim, int n_ctx, const int* d_pos, float scale, int fuse, const oattn_rope_params* rope,
+                    const oattn_ext* ext, void* workspace, size_t workspace_bytes, void* stream);
+
+/* oattn_prefill_ex on the 4-bit cache (ext may be NULL): the chunk's rows are quantised into the cache, and every query sees the
+ * rows as the cache holds them, its own chunk's among them.  The output is fp32 (`out`) or fp16 (`out_f16`, [batch][n_head]
+ * [head_dim]): pass one of them; with ext->out_mmq both may be NULL.  The attention itself runs on fp16 copies of the
+ * rows, which the first of the two launches makes in the workspace; the workspace is sized for `max_rows` = the largest n_past + batch and serves
+ * all layers.  oattn_prefill_status reads its status word (same n_head, head_dim, batch). */
+size_t oattn_prefill_q4_workspace_bytes(int n_head, int n_kv, int head_dim, int max_batch, int max_rows);
+int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, uint16_t* out_f16, int n_head,
+                     int n_kv, int head_dim, int n_ctx, int n_past, int batch, float scale, int fuse,
+                     const oattn_rope_params* rope, const oattn_ext* ext, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Which prefill kernel oattn_prefill launches: 0 = tcgen05/TMEM kernel (default),
  * 1 = the warp-level mma.sync kernel kept as an in-library cross-check.  Process-wide. */
 int oattn_set_prefill_impl(int impl);

@@ -27,6 +27,8 @@ EXPORTS = [
     "oattn_prefill_status",
     "oattn_set_prefill_impl", "oattn_set_decode_min_tiles", "oattn_set_decode_overlap", "oattn_set_wait_limit_cycles", "oattn_profile_enable", "oattn_profile_collect",
     "oattn_launch_count",
+    "oattn_kv_q4_bytes", "oattn_kv_store_q4", "oattn_kv_load_q4", "oattn_kv_shift_q4", "oattn_decode_q4_workspace_bytes",
+    "oattn_decode_q4", "oattn_prefill_q4_workspace_bytes", "oattn_prefill_q4",
 ]
 
 
@@ -111,6 +113,17 @@ def lib():
     L.oattn_set_wait_limit_cycles.argtypes = [ctypes.c_longlong]
     L.oattn_profile_enable.argtypes = [i]
     L.oattn_profile_collect.argtypes = [ctypes.POINTER(ctypes.c_float), i, ctypes.POINTER(ctypes.c_int)]
+    L.oattn_kv_q4_bytes.restype = sz
+    L.oattn_kv_q4_bytes.argtypes = [i, i, i]
+    L.oattn_kv_store_q4.argtypes = [vp, vp, vp, i, i, i, i, i, vp, vp]
+    L.oattn_kv_load_q4.argtypes = [vp, vp, vp, i, i, i, i, i, i, i, vp]
+    L.oattn_kv_shift_q4.argtypes = [vp, i, i, i, i, i, i, vp]
+    L.oattn_decode_q4_workspace_bytes.restype = sz
+    L.oattn_decode_q4_workspace_bytes.argtypes = [i, i, i]
+    L.oattn_decode_q4.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp, f, i, rp, ep, vp, sz, vp]
+    L.oattn_prefill_q4_workspace_bytes.restype = sz
+    L.oattn_prefill_q4_workspace_bytes.argtypes = [i, i, i, i, i]
+    L.oattn_prefill_q4.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, f, i, rp, ep, vp, sz, vp]
     L.oattn_launch_count.restype = ctypes.c_ulonglong
     L.oattn_launch_count.argtypes = []
     _lib = L

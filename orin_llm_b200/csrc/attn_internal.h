@@ -139,6 +139,7 @@ struct PrefillArgs {
     RopeArgs rope;
     PreArgs pre;           // optional bias / per-head RMSNorm in front of RoPE (k and v parts only with the append)
     uint8_t* out_mmq = nullptr;   // optional: the output as block_q8_1_mmq blocks [head][batch], 144 bytes each
+    __half* out16 = nullptr;      // optional: the output as fp16 [batch][n_head][hd], instead of `out`
     int mmq_ds4 = 0;              // scales as fp16 (d, sum) pairs instead of fp32 d
 };
 

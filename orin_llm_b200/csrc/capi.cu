@@ -4,6 +4,7 @@
 
 #include "../../include/orin_attn_b200.h"
 #include "attn_internal.h"
+#include "kv_q4.cuh"
 
 using namespace oattn;
 
@@ -101,6 +102,7 @@ int oattn_init(int device) {
         if ((e = decode_set_attributes()) != cudaSuccess) return cuda_fail(e, "decode attributes");
         if ((e = prefill_mma_set_attributes()) != cudaSuccess) return cuda_fail(e, "prefill (mma) attributes");
         if ((e = prefill_tc_set_attributes()) != cudaSuccess) return cuda_fail(e, "prefill (tcgen05) attributes");
+        if ((e = decode_q4_set_attributes()) != cudaSuccess) return cuda_fail(e, "decode (4-bit cache) attributes");
         void* scratch = nullptr;      // look the built-in scratch block up now, so that oattn_decode_noalloc never has to
         if ((e = decode_static_scratch(&scratch)) != cudaSuccess) return cuda_fail(e, "cudaGetSymbolAddress(built-in scratch)");
         unsigned* tickets = nullptr;  // ... and the arrival counters of the decode launches
@@ -486,6 +488,173 @@ int oattn_prefill_ex(const float* q, const float* k_new, const float* v_new, uin
         if (e != cudaErrorNotSupported) return cuda_fail(e, "prefill (tcgen05) launch");
     }
     if (mmq_only) return OATTN_ERR_UNSUPPORTED;       // the block form is written by the tcgen05 kernel only
+    e = launch_prefill_mma(a, s, &g_launches);
+    return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "prefill (mma) launch");
+}
+
+// ---- 4-bit KV cache ------------------------------------------------------------------------------------------
+// Shape of a call on the cache alone: any number of heads, head_dim 64 or 128.
+static int check_q4(const void* cache, int heads, int head_dim, int n_ctx) {
+    if (!cache || heads <= 0 || n_ctx <= 0) return OATTN_ERR_ARG;
+    if (head_dim != 64 && head_dim != 128) return OATTN_ERR_UNSUPPORTED;
+    if ((uintptr_t)cache & 15) return OATTN_ERR_ARG;                   // blocks are moved in 16-byte pieces
+    if (n_ctx > (1 << 30)) return OATTN_ERR_UNSUPPORTED;               // position + 16 stays an int
+    return OATTN_OK;
+}
+
+size_t oattn_kv_q4_bytes(int n_kv, int head_dim, int n_ctx) {
+    if (n_kv <= 0 || (head_dim != 64 && head_dim != 128) || n_ctx <= 0 || n_ctx > (1 << 30)) return 0;
+    return (size_t)n_kv * q4_blocks(n_ctx) * q4_block_bytes(head_dim);
+}
+
+int oattn_kv_store_q4(void* cache, const float* k, const float* v, int heads, int head_dim, int n_ctx, int pos_base, int batch,
+                      const int* d_pos, void* stream) {
+    if (!device_ready()) return OATTN_ERR_DEVICE;
+    const int rc = check_q4(cache, heads, head_dim, n_ctx);
+    if (rc != OATTN_OK) return rc;
+    if (!k || !v || batch <= 0) return OATTN_ERR_ARG;
+    if (((uintptr_t)k | (uintptr_t)v) & 15) return OATTN_ERR_ARG;      // read as float4
+    if (d_pos && batch != 1) return OATTN_ERR_ARG;
+    if (!d_pos && (pos_base < 0 || pos_base > n_ctx - batch)) return OATTN_ERR_ARG;
+    cudaError_t e = launch_kv_store_q4(reinterpret_cast<uint8_t*>(cache), k, v, heads, head_dim, n_ctx, pos_base, batch, d_pos,
+                                       (cudaStream_t)stream, &g_launches);
+    return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "kv_store_q4 launch");
+}
+
+int oattn_kv_load_q4(const void* cache, uint16_t* kc, uint16_t* vc, int heads, int head_dim, int n_ctx, int row_base, int rows,
+                     int dst_ctx, int dst_base, void* stream) {
+    if (!device_ready()) return OATTN_ERR_DEVICE;
+    const int rc = check_q4(cache, heads, head_dim, n_ctx);
+    if (rc != OATTN_OK) return rc;
+    if (!kc || !vc || rows <= 0 || row_base < 0 || row_base > n_ctx - rows) return OATTN_ERR_ARG;
+    if (dst_ctx <= 0 || dst_base < 0 || dst_base > dst_ctx - rows) return OATTN_ERR_ARG;
+    if (((uintptr_t)kc | (uintptr_t)vc) & 15) return OATTN_ERR_ARG;    // written in 16-byte pieces
+    cudaError_t e = launch_kv_load_q4(reinterpret_cast<const uint8_t*>(cache), kc, vc, heads, head_dim, n_ctx, row_base, rows,
+                                      dst_ctx, dst_base, (cudaStream_t)stream, &g_launches);
+    return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "kv_load_q4 launch");
+}
+
+int oattn_kv_shift_q4(void* cache, int n_layer, int n_kv, int head_dim, int n_ctx, int n_keep, int shift, void* stream) {
+    if (!device_ready()) return OATTN_ERR_DEVICE;
+    const int rc = check_q4(cache, n_kv, head_dim, n_ctx);
+    if (rc != OATTN_OK) return rc;
+    if (n_layer <= 0 || n_keep < 0 || shift <= 0 || n_keep > n_ctx - shift) return OATTN_ERR_ARG;
+    if ((long long)n_layer * n_kv > 0x7fffffffLL) return OATTN_ERR_UNSUPPORTED;
+    cudaError_t e = launch_kv_shift_q4(reinterpret_cast<uint8_t*>(cache), n_layer, n_kv, head_dim, n_ctx, n_keep, shift,
+                                       (cudaStream_t)stream, &g_launches);
+    return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "kv_shift_q4 launch");
+}
+
+// Heads of one CTA and CTAs per slice: a CTA takes at most eight heads of a kv head.
+static void q4_head_split(int n_head, int n_kv, int& per_cta, int& blocks) {
+    const int G = n_head / n_kv;
+    blocks = G > 8 ? 2 : 1;
+    per_cta = (G + blocks - 1) / blocks;
+}
+static DecodeWsLayout decode_q4_ws(int n_head, int n_kv, int head_dim, int sm_count) {
+    int per_cta, blocks;
+    q4_head_split(n_head, n_kv, per_cta, blocks);
+    return decode_ws_layout(n_kv * blocks * per_cta, n_kv * blocks, head_dim, decode_q4_num_splits(n_kv, sm_count));
+}
+
+size_t oattn_decode_q4_workspace_bytes(int n_head, int n_kv, int head_dim) {
+    const DeviceState* d = cur_dev();
+    if (!d || check_shape(n_head, n_kv, head_dim) != OATTN_OK) return 0;
+    return decode_q4_ws(n_head, n_kv, head_dim, d->sm_count).total;
+}
+
+int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, int n_head, int n_kv,
+                    int head_dim, int n_ctx, const int* d_pos, float scale, int fuse, const oattn_rope_params* rope,
+                    const oattn_ext* ext, void* workspace, size_t workspace_bytes, void* stream) {
+    const DeviceState* dev = cur_dev();
+    if (!dev) return OATTN_ERR_DEVICE;
+    int rc = check_shape(n_head, n_kv, head_dim);
+    if (rc != OATTN_OK) return rc;
+    if ((rc = check_q4(cache, n_kv, head_dim, n_ctx)) != OATTN_OK) return rc;
+    const bool q8_only = ext && ext->out_qs;
+    if (!q || (!out && !q8_only) || !d_pos || !(scale > 0.0f)) return OATTN_ERR_ARG;
+    if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new) & 15) return OATTN_ERR_ARG;
+    if (ext && (((uintptr_t)ext->bias_q | (uintptr_t)ext->bias_k | (uintptr_t)ext->bias_v) & 15)) return OATTN_ERR_ARG;
+    if (fuse & ~OATTN_FUSE_ALL) return OATTN_ERR_ARG;
+    if ((fuse & OATTN_FUSE_ROPE_K) && !(fuse & OATTN_FUSE_KV_APPEND)) return OATTN_ERR_ARG;
+    if ((fuse & OATTN_FUSE_KV_APPEND) && (!k_new || !v_new)) return OATTN_ERR_ARG;
+    DecodeQ4Args a;
+    if ((rc = check_rope(fuse, rope, head_dim, a.rope)) != OATTN_OK) return rc;
+    if ((rc = apply_ext(ext, fuse, true, n_head, n_kv, a.pre, &a.out_qs, &a.out_scales)) != OATTN_OK) return rc;
+    q4_head_split(n_head, n_kv, a.heads_per_cta, a.head_blocks);
+    const DecodeWsLayout w = decode_q4_ws(n_head, n_kv, head_dim, dev->sm_count);
+    if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < w.total) return OATTN_ERR_WORKSPACE;
+    if ((size_t)n_kv * a.head_blocks * (w.n_groups + 1) > (size_t)kTicketWords) return OATTN_ERR_UNSUPPORTED;
+    a.q = q; a.k_new = k_new; a.v_new = v_new; a.cache = reinterpret_cast<uint8_t*>(cache); a.out = out;
+    uint8_t* wsb = reinterpret_cast<uint8_t*>(workspace);
+    a.ws_o = reinterpret_cast<float*>(wsb + w.part_o);
+    a.ws_ml = reinterpret_cast<float*>(wsb + w.part_ml);
+    a.grp_o = reinterpret_cast<float*>(wsb + w.grp_o);
+    a.grp_ml = reinterpret_cast<float*>(wsb + w.grp_ml);
+    cudaError_t e = decode_ticket_slot(workspace, &a.tickets);
+    if (e != cudaSuccess) return cuda_fail(e, "arrival counters");
+    a.d_pos = d_pos;
+    a.n_head = n_head; a.n_kv = n_kv; a.n_ctx = n_ctx;
+    a.n_splits = w.n_splits; a.group = w.group; a.n_groups = w.n_groups;
+    a.scale = scale; a.fuse = fuse; a.overlap = g_decode_overlap;
+    e = launch_decode_q4(a, head_dim, (cudaStream_t)stream, &g_launches);
+    return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "decode (4-bit cache) launch");
+}
+
+// [fp16 queries][status word, 256 bytes][fp16 K rows][fp16 V rows]: the first two as in oattn_prefill
+size_t oattn_prefill_q4_workspace_bytes(int n_head, int n_kv, int head_dim, int max_batch, int max_rows) {
+    const size_t head = oattn_prefill_workspace_bytes(n_head, n_kv, head_dim, max_batch);
+    if (!head || max_rows < max_batch) return 0;
+    return head + 2 * align256((size_t)n_kv * max_rows * head_dim * sizeof(__half));
+}
+
+int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, uint16_t* out_f16, int n_head,
+                     int n_kv, int head_dim, int n_ctx, int n_past, int batch, float scale, int fuse, const oattn_rope_params* rope,
+                     const oattn_ext* ext, void* workspace, size_t workspace_bytes, void* stream) {
+    const DeviceState* dev = cur_dev();
+    if (!dev) return OATTN_ERR_DEVICE;
+    int rc = check_shape(n_head, n_kv, head_dim);
+    if (rc != OATTN_OK) return rc;
+    if ((rc = check_q4(cache, n_kv, head_dim, n_ctx)) != OATTN_OK) return rc;
+    const bool mmq = ext && ext->out_mmq;
+    if (!q || (!out && !out_f16 && !mmq) || (out && out_f16) || !(scale > 0.0f)) return OATTN_ERR_ARG;
+    if (mmq && (head_dim != 128 || g_prefill_impl != 0 || ((uintptr_t)ext->out_mmq & 15))) return OATTN_ERR_UNSUPPORTED;
+    if (batch <= 0 || n_past < 0 || n_past > n_ctx - batch) return OATTN_ERR_ARG;
+    if (((uintptr_t)out | (uintptr_t)out_f16) & 15) return OATTN_ERR_ARG;
+    if (fuse & ~OATTN_FUSE_ALL) return OATTN_ERR_ARG;
+    if ((fuse & OATTN_FUSE_ROPE_K) && !(fuse & OATTN_FUSE_KV_APPEND)) return OATTN_ERR_ARG;
+    if ((fuse & OATTN_FUSE_KV_APPEND) && (!k_new || !v_new)) return OATTN_ERR_ARG;
+    KvQ4PrologueArgs p;
+    PrefillArgs& a = p.a;
+    if ((rc = check_rope(fuse, rope, head_dim, a.rope)) != OATTN_OK) return rc;
+    if ((rc = apply_ext(ext, fuse, false, n_head, n_kv, a.pre, nullptr, nullptr)) != OATTN_OK) return rc;
+    const int rows = n_past + batch;
+    const size_t need = oattn_prefill_q4_workspace_bytes(n_head, n_kv, head_dim, batch, rows);
+    const size_t head = oattn_prefill_workspace_bytes(n_head, n_kv, head_dim, batch);
+    if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need) return OATTN_ERR_WORKSPACE;
+    uint8_t* wsb = reinterpret_cast<uint8_t*>(workspace);
+    a.q = q; a.k_new = k_new; a.v_new = v_new; a.out = out;
+    a.out16 = reinterpret_cast<__half*>(out_f16);
+    a.q16 = reinterpret_cast<__half*>(wsb);
+    a.status = reinterpret_cast<int*>(wsb + head - 256);
+    p.k16 = reinterpret_cast<__half*>(wsb + head);
+    p.v16 = reinterpret_cast<__half*>(wsb + head + align256((size_t)n_kv * rows * head_dim * sizeof(__half)));
+    a.kc = reinterpret_cast<uint16_t*>(p.k16);
+    a.vc = reinterpret_cast<uint16_t*>(p.v16);
+    a.n_head = n_head; a.n_kv = n_kv; a.head_dim = head_dim; a.n_ctx = rows; a.n_past = n_past; a.batch = batch;
+    a.scale = scale; a.fuse = fuse;
+    if (mmq) { a.out_mmq = reinterpret_cast<uint8_t*>(ext->out_mmq); a.mmq_ds4 = ext->out_mmq_ds4; }
+    p.cache = reinterpret_cast<uint8_t*>(cache);
+    p.cache_ctx = n_ctx;
+    cudaStream_t s = (cudaStream_t)stream;
+    cudaError_t e = launch_prefill_q4_prologue(p, s, &g_launches);
+    if (e != cudaSuccess) return cuda_fail(e, "prefill (4-bit cache) prologue launch");
+    if (g_prefill_impl == 0) {
+        e = launch_prefill_tc(a, dev->sm_count, s, &g_launches);
+        if (e == cudaSuccess) return OATTN_OK;
+        if (e != cudaErrorNotSupported) return cuda_fail(e, "prefill (tcgen05) launch");
+    }
+    if (mmq) return OATTN_ERR_UNSUPPORTED;
     e = launch_prefill_mma(a, s, &g_launches);
     return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "prefill (mma) launch");
 }

@@ -193,6 +193,13 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_mma_kernel(const PrefillA
         const int tok = R / G, hg = R % G;
         if (tok < ntok) {
             const float inv = 1.f / l;
+            if (p.out16) {
+                __half* dst16 = p.out16 + ((size_t)(t0 + tok) * p.n_head + kvh * G + hg) * HD;
+#pragma unroll
+                for (int j = 0; j < HD / 8; ++j)
+                    *reinterpret_cast<uint32_t*>(dst16 + 8 * j + 2 * t) = pack_half2(o[j][2 * hh] * inv, o[j][2 * hh + 1] * inv);
+                continue;
+            }
             float* dst = p.out + ((size_t)(t0 + tok) * p.n_head + kvh * G + hg) * HD;
 #pragma unroll
             for (int j = 0; j < HD / 8; ++j)

@@ -98,11 +98,12 @@ __device__ long long g_trace[3][8][128];
 
 struct TcArgs {
     float* out;
+    __half* out16;         // optional fp16 form of the output, instead of `out`
     uint8_t* out_mmq;      // optional block_q8_1_mmq form of the output (src/kernels.cu:147-155), [head][batch] blocks
     int mmq_ds4;
     int* status;
     int n_head, n_kv, n_past, batch, G, TQ;   // TQ = floor(128 / G) tokens per tile
-    int out_tma;           // the fp32 output leaves through shared memory and bulk tensor stores (tmO is valid)
+    int out_tma;           // the output leaves through shared memory and bulk tensor stores (tmO is valid): 1 fp32, 2 fp16
 };
 
 // ---- PTX wrappers ---------------------------------------------------------------------------------
@@ -619,7 +620,15 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 tmem_ld32(to + 64 * team + 32 * c, a);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) a[i] *= inv;
-                if (p.out_tma) {
+                if (p.out_tma == 2) {
+                    // fp16: two slabs of 64 columns, one per team, the same way
+                    uint8_t* rowp = smem + OFF_K + team * (BM * 128) + row * 128;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<uint4*>(rowp + (((4 * c + i) ^ (row & 7)) << 4)) =
+                            make_uint4(pack_half2(a[8 * i], a[8 * i + 1]), pack_half2(a[8 * i + 2], a[8 * i + 3]),
+                                       pack_half2(a[8 * i + 4], a[8 * i + 5]), pack_half2(a[8 * i + 6], a[8 * i + 7]));
+                } else if (p.out_tma) {
                     // Straight from here a warp's store would touch 32 rows, 512 bytes apart, with 16 bytes each.  The
                     // tile goes through shared memory instead (the K ring is idle now): four slabs of 32 columns, a row's
                     // 128 bytes of a slab swizzled like a tensor-map tile, and leaves as four bulk tensor stores.
@@ -664,8 +673,13 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             asm volatile("bar.sync 1, 256;\n" ::: "memory");
             if (tid == 32 * kFirstSoftmaxWarp && !*s_abort) {
                 // rows past the batch (a ragged last tile) lie outside the tensor map and are not written
+                if (p.out_tma == 2) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tma_store_3d(&tmO, 32 * c, kvh * p.G, t0, sbase + OFF_K + c * (BM * 128));
+                    for (int c = 0; c < 2; ++c) tma_store_3d(&tmO, 64 * c, kvh * p.G, t0, sbase + OFF_K + c * (BM * 128));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tma_store_3d(&tmO, 32 * c, kvh * p.G, t0, sbase + OFF_K + c * (BM * 128));
+                }
                 asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
                 asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");  // shared memory stays valid until it has been read
             }
@@ -744,9 +758,12 @@ cudaError_t launch_prefill_tc(const PrefillArgs& a, int sm_count, cudaStream_t s
     CUtensorMap tmO = tmQ;
     const uint64_t orow = HD * sizeof(float);
     const bool out_tma = a.out && !((uintptr_t)a.out & 15) && make_out_map(&tmO, a.out, a.n_head, a.batch, orow, orow * a.n_head, G, TQ);
+    // ... or the fp16 one, which has no other way out (the C entry checked its alignment)
+    if (a.out16 && !make_map(&tmO, a.out16, a.n_head, a.batch, rowb, rowb * a.n_head, G, TQ)) return cudaErrorInvalidValue;
     TcArgs t;
-    t.out_tma = out_tma ? 1 : 0;
+    t.out_tma = a.out16 ? 2 : (out_tma ? 1 : 0);
     t.out = a.out;
+    t.out16 = a.out16;
     t.out_mmq = a.out_mmq;
     t.mmq_ds4 = a.mmq_ds4;
     t.status = a.status;

@@ -14,7 +14,7 @@ from . import capi
 from .capi import (FUSE_ALL, FUSE_KV_APPEND, FUSE_NONE, FUSE_ROPE_K, FUSE_ROPE_Q, PART_PAD, ROPE_NEOX,  # noqa: F401
                    ROPE_NORMAL)
 
-_state = {"device": None, "stream": None, "decode_ws": {}, "prefill_ws": {}}
+_state = {"device": None, "stream": None, "decode_ws": {}, "prefill_ws": {}, "decode_q4_ws": {}, "prefill_q4_ws": {}}
 
 
 def _ptr(t):
@@ -311,6 +311,157 @@ class KVCache:
         if shift <= 0 or shift > self.n_ctx:
             return
         kv_shift(self.k, self.v, self.n_layer, self.n_kv, self.head_dim, self.n_ctx, n_keep, shift)
+
+
+# ---- KV cache held in 4 bits ------------------------------------------------------------------------------------------
+# The counterparts of kv_store_*, kv_shift, attn_decode and attn_prefill over a cache of 4.5 bits a value (format in
+# include/orin_attn_b200.h), and its read-back.  No counterpart in the reference.
+
+def _q4_tensor(name, t, dtype, numel, optional=False):
+    """The checks the C entry cannot make: a contiguous tensor of that type and size on the current CUDA device."""
+    if t is None and optional:
+        return
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s: a tensor is needed, got %s" % (name, type(t).__name__))
+    if t.dtype != dtype or not t.is_contiguous() or t.numel() < numel:
+        raise ValueError("%s: a contiguous %s tensor of at least %d elements is needed, got %s %s%s" % (
+            name, dtype, numel, t.dtype, list(t.shape), "" if t.is_contiguous() else ", not contiguous"))
+    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+        raise ValueError("%s: on %s, the current device is cuda:%d" % (name, t.device, torch.cuda.current_device()))
+
+
+def _q4_cache(cache, layers, n_kv, head_dim, n_ctx):
+    nbytes = kv_q4_bytes(n_kv, head_dim, n_ctx)
+    if nbytes == 0:
+        raise capi.AttnError(capi.ERR_UNSUPPORTED, "4-bit cache: head_dim 64 or 128, at least one head and one position")
+    _q4_tensor("cache", cache, torch.uint8, layers * nbytes)
+
+
+def kv_q4_bytes(n_kv, head_dim, n_ctx):
+    """Bytes of one layer of a 4-bit cache."""
+    return int(capi.lib().oattn_kv_q4_bytes(n_kv, head_dim, n_ctx))
+
+
+def kv_store_q4_batch(cache, k, v, heads, head_dim, n_ctx, pos_base, batch):
+    """kv_store_batch into a 4-bit cache: k, v [batch][heads][head_dim] fp32 at positions pos_base + b."""
+    _q4_cache(cache, 1, heads, head_dim, n_ctx)
+    for name, t in (("k", k), ("v", v)):
+        _q4_tensor(name, t, torch.float32, batch * heads * head_dim)
+    capi.check(capi.lib().oattn_kv_store_q4(_ptr(cache), _ptr(k), _ptr(v), heads, head_dim, n_ctx, pos_base, batch, None, _stream()))
+
+
+def kv_store_q4_ind(cache, k, v, heads, head_dim, n_ctx, d_pos):
+    """kv_store_ind into a 4-bit cache: one row at *d_pos."""
+    _q4_cache(cache, 1, heads, head_dim, n_ctx)
+    for name, t in (("k", k), ("v", v)):
+        _q4_tensor(name, t, torch.float32, heads * head_dim)
+    _q4_tensor("d_pos", d_pos, torch.int32, 1)
+    capi.check(capi.lib().oattn_kv_store_q4(_ptr(cache), _ptr(k), _ptr(v), heads, head_dim, n_ctx, 0, 1, _ptr(d_pos), _stream()))
+
+
+def kv_load_q4(cache, kc, vc, heads, head_dim, n_ctx, row_base, rows, dst_ctx=None, dst_base=0):
+    """Rows [row_base, row_base + rows) of a 4-bit cache as fp16, into kc, vc [heads][dst_ctx][head_dim] from row dst_base
+    on (default: a block of exactly these rows)."""
+    dst_ctx = rows if dst_ctx is None else dst_ctx
+    _q4_cache(cache, 1, heads, head_dim, n_ctx)
+    for name, t in (("kc", kc), ("vc", vc)):
+        _q4_tensor(name, t, torch.float16, heads * dst_ctx * head_dim)
+    capi.check(capi.lib().oattn_kv_load_q4(_ptr(cache), _ptr(kc), _ptr(vc), heads, head_dim, n_ctx, row_base, rows, dst_ctx, dst_base,
+                                           _stream()))
+
+
+def kv_shift_q4(cache, n_layer, n_kv, head_dim, n_ctx, n_keep, shift):
+    """kv_shift on the 4-bit cache of n_layer layers, in place."""
+    _q4_cache(cache, n_layer, n_kv, head_dim, n_ctx)
+    capi.check(capi.lib().oattn_kv_shift_q4(_ptr(cache), n_layer, n_kv, head_dim, n_ctx, n_keep, shift, _stream()))
+
+
+def decode_q4_workspace(n_head, n_kv, head_dim):
+    """Scratch for attn_decode_q4, allocated once per shape and device."""
+    key = (n_head, n_kv, head_dim, torch.cuda.current_device())
+    ws = _state["decode_q4_ws"].get(key)
+    if ws is None:
+        nbytes = capi.lib().oattn_decode_q4_workspace_bytes(n_head, n_kv, head_dim)
+        if nbytes == 0:
+            raise capi.AttnError(capi.ERR_UNSUPPORTED, "decode shape not supported or init() not called")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        _state["decode_q4_ws"][key] = ws
+    return ws
+
+
+def prefill_q4_workspace(n_head, n_kv, head_dim, batch, rows):
+    """Scratch for attn_prefill_q4 calls with n_past + batch <= rows; it serves every layer.  A block that became too small is
+    kept: work on a stream torch does not know of, or a captured graph, may still be using it."""
+    key = (n_head, n_kv, head_dim, torch.cuda.current_device())
+    blocks = _state["prefill_q4_ws"].setdefault(key, [])
+    nbytes = capi.lib().oattn_prefill_q4_workspace_bytes(n_head, n_kv, head_dim, batch, rows)
+    if nbytes == 0:
+        raise capi.AttnError(capi.ERR_UNSUPPORTED, "prefill shape not supported")
+    if not blocks or blocks[-1].numel() < nbytes:
+        grown = max(nbytes, 2 * blocks[-1].numel()) if blocks else nbytes
+        blocks.append(torch.empty(grown, dtype=torch.uint8, device="cuda"))
+    return blocks[-1]
+
+
+def attn_decode_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, d_pos, scale, fuse=FUSE_ALL, rope=None,
+                   workspace=None, ext=None):
+    """attn_decode over one layer of a 4-bit cache, the new row quantised and appended in the same launch."""
+    _q4_cache(cache, 1, n_kv, head_dim, n_ctx)
+    append = bool(fuse & FUSE_KV_APPEND)
+    _q4_tensor("q", q, torch.float32, n_head * head_dim)
+    _q4_tensor("k_new", k_new, torch.float32, n_kv * head_dim if append else 0, not append)
+    _q4_tensor("v_new", v_new, torch.float32, n_kv * head_dim if append else 0, not append)
+    _q4_tensor("out", out, torch.float32, n_head * head_dim, bool(ext) and ext.get("out_qs") is not None)
+    _q4_tensor("d_pos", d_pos, torch.int32, 1)
+    ws = workspace if workspace is not None else decode_q4_workspace(n_head, n_kv, head_dim)
+    _q4_tensor("workspace", ws, torch.uint8, 0)
+    ref, keep = _rope_params(rope)
+    eref, ekeep = _ext_params(ext)
+    capi.check(capi.lib().oattn_decode_q4(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(cache), _ptr(out), n_head, n_kv, head_dim, n_ctx,
+                                          _ptr(d_pos), scale, fuse, ref, eref, _ptr(ws), ws.numel(), _stream()))
+    del keep, ekeep
+
+
+def attn_prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse=FUSE_ALL, rope=None,
+                    workspace=None, ext=None):
+    """attn_prefill over one layer of a 4-bit cache, the chunk's rows quantised and appended first.  out: fp32 or fp16
+    [batch][n_head][head_dim] (the attention runs on fp16 operands either way)."""
+    _q4_cache(cache, 1, n_kv, head_dim, n_ctx)
+    append = bool(fuse & FUSE_KV_APPEND)
+    _q4_tensor("q", q, torch.float32, batch * n_head * head_dim)
+    _q4_tensor("k_new", k_new, torch.float32, batch * n_kv * head_dim if append else 0, not append)
+    _q4_tensor("v_new", v_new, torch.float32, batch * n_kv * head_dim if append else 0, not append)
+    half = isinstance(out, torch.Tensor) and out.dtype == torch.float16
+    _q4_tensor("out", out, torch.float16 if half else torch.float32, batch * n_head * head_dim,
+               bool(ext) and ext.get("out_mmq") is not None)
+    ws = workspace if workspace is not None else prefill_q4_workspace(n_head, n_kv, head_dim, batch, max(n_ctx, batch))
+    _q4_tensor("workspace", ws, torch.uint8, 0)
+    ref, keep = _rope_params(rope)
+    eref, ekeep = _ext_params(ext)
+    capi.check(capi.lib().oattn_prefill_q4(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(cache), _ptr(None if half else out),
+                                           _ptr(out if half else None), n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse,
+                                           ref, eref, _ptr(ws), ws.numel(), _stream()))
+    del keep, ekeep
+
+
+class KVCacheQ4:
+    """The 4-bit counterpart of KVCache: one allocation, uint8 [n_layer][n_kv][blocks of 16 positions][18 * head_dim],
+    zero-filled once (every row then reads back as zero)."""
+
+    def __init__(self, n_layer, n_kv, n_ctx, head_dim, device="cuda"):
+        self.n_layer, self.n_kv, self.n_ctx, self.head_dim = n_layer, n_kv, n_ctx, head_dim
+        if kv_q4_bytes(n_kv, head_dim, n_ctx) == 0:
+            raise capi.AttnError(capi.ERR_UNSUPPORTED, "4-bit cache: head_dim 64 or 128, at least one head and one position")
+        self.buf = torch.zeros(n_layer, n_kv, (n_ctx + 15) // 16, 18 * head_dim, dtype=torch.uint8, device=device)
+
+    def layer(self, l):
+        return self.buf[l]
+
+    def shift(self, n_keep, shift):
+        """Drop rows [n_keep, n_keep + shift) of every layer (KVCache.shift)."""
+        if shift <= 0 or shift > self.n_ctx:
+            return
+        kv_shift_q4(self.buf, self.n_layer, self.n_kv, self.head_dim, self.n_ctx, n_keep, shift)
 
 
 def default_scale(head_dim):
