@@ -581,6 +581,7 @@ int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void
     DecodeQ4Args a;
     if ((rc = check_rope(fuse, rope, head_dim, a.rope)) != OATTN_OK) return rc;
     if ((rc = apply_ext(ext, fuse, true, n_head, n_kv, a.pre, &a.out_qs, &a.out_scales)) != OATTN_OK) return rc;
+    rope_freq_table(a.rope, a.freq);
     q4_head_split(n_head, n_kv, a.heads_per_cta, a.head_blocks);
     const DecodeWsLayout w = decode_q4_ws(n_head, n_kv, head_dim, dev->sm_count);
     if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < w.total) return OATTN_ERR_WORKSPACE;
@@ -646,6 +647,7 @@ int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, voi
     if (mmq) { a.out_mmq = reinterpret_cast<uint8_t*>(ext->out_mmq); a.mmq_ds4 = ext->out_mmq_ds4; }
     p.cache = reinterpret_cast<uint8_t*>(cache);
     p.cache_ctx = n_ctx;
+    rope_freq_table(a.rope, p.freq);
     cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e = launch_prefill_q4_prologue(p, s, &g_launches);
     if (e != cudaSuccess) return cuda_fail(e, "prefill (4-bit cache) prologue launch");

@@ -8,19 +8,19 @@ namespace oattn {
 
 namespace {
 
-constexpr int kMergeThreads = 128;     // threads of a CTA that hold pieces of the block (the first 128 of a larger CTA)
+constexpr int kMergeThreads = 128;     // threads of a CTA that hold pieces of the block, unless said otherwise
 
 // ---- how the threads of a CTA share one kv head's [G][HD] block of fp32 values ------------------------------------
-// The block is cut into float4 pieces; thread `tid` owns pieces tid, tid + 128, ... (piece -> row = head in the group,
+// The block is cut into float4 pieces; thread `tid` < THREADS owns pieces tid, tid + THREADS, ... (piece -> row = head in the group,
 // col4 = which four dims).  With HD = 128 a warp owns whole rows (rows warp, warp + 4, ...), a lane four dims.
-template <int HD, bool WIDE>
+template <int HD, bool WIDE, int THREADS = kMergeThreads>
 struct Slots {
     static constexpr int F4_PER_ROW = HD / 4;
     static constexpr int ROWS = WIDE ? 16 : 8;
-    static constexpr int N = ROWS * F4_PER_ROW / kMergeThreads;
+    static constexpr int N = ROWS * F4_PER_ROW / THREADS;
     static_assert(N >= 1, "at least one piece per thread");
-    __device__ static __forceinline__ int row(int tid, int k) { return (tid + k * kMergeThreads) / F4_PER_ROW; }
-    __device__ static __forceinline__ int col4(int tid, int k) { return (tid + k * kMergeThreads) % F4_PER_ROW; }
+    __device__ static __forceinline__ int row(int tid, int k) { return (tid + k * THREADS) / F4_PER_ROW; }
+    __device__ static __forceinline__ int col4(int tid, int k) { return (tid + k * THREADS) % F4_PER_ROW; }
 };
 
 // Running log-sum-exp merge of one piece: acc = sum_i e^(m_i - M) O_i, L = sum_i e^(m_i - M) l_i, M = max m_i.
@@ -58,11 +58,11 @@ __device__ __forceinline__ void run_add(RunState& s, const float (&m)[8], const 
 // other SMs a moment ago: read them from L2 (ld.cg), never through this SM's L1.  This runs on the critical path of the
 // launch as a chain of L2 round trips, so a pass issues every load it needs before it uses any of them: the lanes that
 // share a row (HD/4 of them) each fetch the (m, l) of one part and exchange the weights by shuffle, and every lane keeps
-// its O pieces of up to 16 parts in flight.  Called by all threads of the CTA.
-template <int HD, bool WIDE>
+// its O pieces of up to 16 parts in flight.  Called by all THREADS threads.
+template <int HD, bool WIDE, int THREADS = kMergeThreads>
 __device__ __forceinline__ void merge_parts(const float* o_base, const float* ml_base, int n, int G, float c,
-                                            RunState (&st)[Slots<HD, WIDE>::N]) {
-    using S = Slots<HD, WIDE>;
+                                            RunState (&st)[Slots<HD, WIDE, THREADS>::N]) {
+    using S = Slots<HD, WIDE, THREADS>;
     constexpr int LPR = S::F4_PER_ROW;            // lanes per row: 32 or 16
     constexpr int PASS = 16;                      // parts per pass
     constexpr int KB = S::N < 2 ? S::N : 2;       // pieces per thread handled together
@@ -117,9 +117,9 @@ __device__ __forceinline__ void merge_parts(const float* o_base, const float* ml
     }
 }
 
-template <int HD, bool WIDE>
-__device__ __forceinline__ void store_part(float* o_base, float* ml_base, int G, const RunState (&st)[Slots<HD, WIDE>::N]) {
-    using S = Slots<HD, WIDE>;
+template <int HD, bool WIDE, int THREADS = kMergeThreads>
+__device__ __forceinline__ void store_part(float* o_base, float* ml_base, int G, const RunState (&st)[Slots<HD, WIDE, THREADS>::N]) {
+    using S = Slots<HD, WIDE, THREADS>;
     const int tid = threadIdx.x;
 #pragma unroll
     for (int k = 0; k < S::N; ++k) {
@@ -171,11 +171,11 @@ __device__ __forceinline__ float4 normalised(const RunState& s) {
     return make_float4(s.acc.x / s.L, s.acc.y / s.L, s.acc.z / s.L, s.acc.w / s.L);
 }
 
-// What the CTA that holds the merged (M, L, O) of the G heads from head0 on does with it.  Called by all merge threads of
-// that CTA.
-template <int HD, bool WIDE, typename Args>
-__device__ __forceinline__ void emit_final(const Args& p, int head0, int G, const RunState (&st)[Slots<HD, WIDE>::N]) {
-    using S = Slots<HD, WIDE>;
+// What the CTA that holds the merged (M, L, O) of the G heads from head0 on does with it.  Called by all THREADS
+// threads.
+template <int HD, bool WIDE, int THREADS = kMergeThreads, typename Args>
+__device__ __forceinline__ void emit_final(const Args& p, int head0, int G, const RunState (&st)[Slots<HD, WIDE, THREADS>::N]) {
+    using S = Slots<HD, WIDE, THREADS>;
     const int tid = threadIdx.x;
     if (!p.emit_partial) {
 #pragma unroll

@@ -13,6 +13,8 @@
 // first eight to fp16 left over (x = hi + lo, 22 bits together): the result keeps fp32 accuracy and the instruction count is
 // the same.  q is scaled by a power of two per head, P d by a power of two that is lowered when a step of 2 or more is met,
 // so that neither half leaves the fp16 range.
+#include <type_traits>
+
 #include "decode_merge.cuh"
 #include "kv_q4.cuh"
 
@@ -22,12 +24,12 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 4;                 // blocks in flight per warp
+constexpr int kTurns = 2;                  // pairs of blocks in the ring of a warp
 
 template <int HD>
 struct Q4Smem {
     static constexpr int BLOCK = Q4<HD>::BLOCK;
-    static constexpr int RING = kWarps * kStages * BLOCK;
+    static constexpr int RING = kWarps * kTurns * 2 * BLOCK;
     static constexpr int QF_OFF = RING;                                // q fragments [HD/16 steps][32 lanes][4 words]
     static constexpr int QF_BYTES = HD / 16 * 512;
     static constexpr int IN_OFF = QF_OFF + QF_BYTES;                   // fp32 rows: q [8], k_new, v_new
@@ -43,32 +45,72 @@ struct Q4Smem {
 };
 
 struct Q4Plan {
-    int blocks, per_split, active;       // 16-row blocks in all, of one slice, slices that have any
+    int blocks, per_split, active, step; // 16-row blocks in all, of one slice, slices that have any; blocks a warp takes at a time
 };
+// A warp works on pairs of blocks (half the softmax bookkeeping); while there are no more blocks than warps it takes one.
 __device__ __forceinline__ Q4Plan q4_plan(int npos, int n_splits) {
     Q4Plan s;
     s.blocks = (npos + 15) >> 4;
-    const int units = (s.blocks + kWarps - 1) / kWarps;                // a unit: one block for each warp
-    const int per = max(1, (units + n_splits - 1) / n_splits);
-    s.per_split = per * kWarps;
-    s.active = (units + per - 1) / per;
+    s.step = s.blocks <= n_splits * kWarps ? 1 : 2;
+    s.per_split = s.step == 1 ? kWarps : 2 * (((s.blocks + 1) / 2 + n_splits - 1) / n_splits);
+    s.active = (s.blocks + s.per_split - 1) / s.per_split;
     return s;
 }
 
-__device__ __forceinline__ float2 half2_word(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+// Pairs of fp32 in one 64-bit register: two-wide add, multiply and fma, each half rounded as the scalar instruction would.
+struct F2 {
+    unsigned long long v;
+    __device__ __forceinline__ F2() {}
+    __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(x), "f"(y)); }
+    __device__ __forceinline__ float x() const { float a, b; asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); return a; }
+    __device__ __forceinline__ float y() const { float a, b; asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); return b; }
+};
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+
+__device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)w)); }
+__device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)(w >> 16))); }
 
 // hi = fp16(x), lo = fp16(x - hi), for a pair
-__device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    hi = pack_half2(x0, x1);
-    const float2 h = half2_word(hi);
-    lo = pack_half2(x0 - h.x, x1 - h.y);
+__device__ __forceinline__ void split_half2(F2 x, uint32_t& hi, uint32_t& lo) {
+    hi = pack_half2(x.x(), x.y());
+    const F2 rest = fma2(F2(half_lo(hi), half_hi(hi)), F2(-1.f, -1.f), x);
+    lo = pack_half2(rest.x(), rest.y());
 }
 
+// Scale words (d, m) of two neighbouring rows, [row][group], in one load.
+template <int NG>
+__device__ __forceinline__ void load_scales(const uint8_t* at, uint32_t (&w)[2][NG]) {
+    if constexpr (NG == 2) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at);
+        w[0][0] = v.x; w[0][1] = v.y; w[1][0] = v.z; w[1][1] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(at);
+        w[0][0] = v.x; w[1][0] = v.y;
+    }
+}
+
+// Nibbles i and i + 4 of a code word as a pair of fp16 subnormals, code * 2^-20 (bits 4..7 of each half).  Two of the four
+// pairs would need no shift at all as code * 2^-24, but the matrix unit aligns products by the operands' exponent fields: the
+// more leading zeros a subnormal has, the more low bits of every partial sum are cut off (measured: the error of a step over
+// 1K rows is 4e-6 of the output with codes at bits 0..3, against FIXME with these).
+struct Nibbles {
+    uint32_t x[4];
+    __device__ __forceinline__ explicit Nibbles(uint32_t w) {
+        x[0] = (w << 4) & 0x00F000F0u;
+        x[1] = w & 0x00F000F0u;
+        x[2] = (w >> 4) & 0x00F000F0u;
+        x[3] = (w >> 8) & 0x00F000F0u;
+    }
+};
+
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const DecodeQ4Args p) {
+__global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const __grid_constant__ DecodeQ4Args p) {
     using F = Q4<HD>;
     using L = Q4Smem<HD>;
-    using S = Slots<HD, false>;
+    constexpr int MT = HD == 128 ? 256 : 128;    // threads that hold pieces of the merged block
+    using S = Slots<HD, false, MT>;
     constexpr int NG = F::NG, NW = HD / 32;      // groups of a row, code words of a lane per K row
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -78,8 +120,37 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const DecodeQ4Ar
     const int head0 = kvh * GA + hb * p.heads_per_cta;
     const int G = min(p.heads_per_cta, GA - hb * p.heads_per_cta);
 
+    // Inputs of the step, one or two float4 pieces per thread (8 q rows of 128; k_new and v_new by the first threads), all issued
+    // together and, where the order against preceding kernels allows it, along with the position word.
+    constexpr int C4 = HD / 4;
+    const bool append = (p.fuse & 4) != 0;
+    float4 in_q = make_float4(0.f, 0.f, 0.f, 0.f), in_kv = in_q;
+    auto load_inputs = [&]() {
+        if (tid < G * C4) {
+            const size_t at = (size_t)head0 * HD + tid * 4;
+            in_q = *reinterpret_cast<const float4*>(p.q + at);
+            if (p.pre.bias_q) {
+                const float4 b = *reinterpret_cast<const float4*>(p.pre.bias_q + at);
+                in_q.x += b.x; in_q.y += b.y; in_q.z += b.z; in_q.w += b.w;
+            }
+        }
+        if (append && tid < 2 * C4) {
+            const size_t at = (size_t)kvh * HD + (tid % C4) * 4;
+            in_kv = *reinterpret_cast<const float4*>((tid < C4 ? p.k_new : p.v_new) + at);
+            const float* bias = tid < C4 ? p.pre.bias_k : p.pre.bias_v;
+            if (bias) {
+                const float4 b = *reinterpret_cast<const float4*>(bias + at);
+                in_kv.x += b.x; in_kv.y += b.y; in_kv.z += b.z; in_kv.w += b.w;
+            }
+        }
+    };
+    static_assert(8 * C4 <= kThreads, "one piece of q per thread");
+
     pdl_trigger();
-    if (p.overlap != 2) pdl_wait();
+    if (p.overlap != 2) {
+        pdl_wait();
+        load_inputs();
+    }
     const int npos = max(0, min(*p.d_pos + 1, p.n_ctx));
     const Q4Plan plan = q4_plan(npos, p.n_splits);
     if (split >= max(plan.active, 1)) return;
@@ -87,36 +158,41 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const DecodeQ4Ar
     const int GP = p.heads_per_cta;                          // rows kept there per slice
     if (plan.active == 0) {
         if (p.overlap == 2) pdl_wait();
-        if (tid < kMergeThreads) {
+        if (tid < MT) {
             RunState st[S::N];
 #pragma unroll
             for (int k = 0; k < S::N; ++k) st[k] = run_empty();
-            emit_final<HD, false>(p, head0, G, st);
+            emit_final<HD, false, MT>(p, head0, G, st);
         }
         return;
     }
     const int blk0 = split * plan.per_split, blk1 = min(blk0 + plan.per_split, plan.blocks);
-    const bool append = (p.fuse & 4) != 0;
-    const bool last_slice = split == plan.active - 1;
-    const bool owner = append && last_slice;
+    const bool owner = append && split == plan.active - 1;
     const int new_pos = npos - 1;
     uint8_t* cache = p.cache + (size_t)kvh * q4_blocks(p.n_ctx) * F::BLOCK;
-    uint8_t* ring = smem + warp * kStages * F::BLOCK;
+    uint8_t* ring = smem + warp * kTurns * 2 * F::BLOCK;
 
-    // block `b` of the sequence -> stage; 16-byte pieces, consecutive lanes
-    auto load_block = [&](int b, int stage) {
-        const uint8_t* src = cache + (size_t)b * F::BLOCK;
-        const uint32_t dst = smem_u32(ring + stage * F::BLOCK);
+    // This warp's it-th turn: blocks b, b + 1 (one with step 1, or at the end), b = first(it); ring slots 2 (it % kTurns), + 1.
+    auto first = [&](int it) { return blk0 + plan.step * (warp + kWarps * it); };
+    const int turns = first(0) < blk1 ? (blk1 - first(0) + plan.step * kWarps - 1) / (plan.step * kWarps) : 0;
+    auto load_turn = [&](int it) {
+        const int b = first(it);
+        const uint8_t* src = cache + (size_t)b * F::BLOCK + 16 * lane;
+        const uint32_t dst = smem_u32(ring + (it % kTurns) * 2 * F::BLOCK + 16 * lane);
+        const int n16 = (plan.step == 2 && b + 1 < blk1 ? 2 : 1) * (F::BLOCK / 16) - lane;
+        constexpr int ALL = (2 * F::BLOCK / 16 + 31) / 32;
+        if (2 * F::BLOCK % 512 == 0 && n16 > F::BLOCK / 16) {
 #pragma unroll
-        for (int i = 0; i < (F::BLOCK / 16 + 31) / 32; ++i) {
-            const int c = lane + 32 * i;
-            if (c < F::BLOCK / 16) cp_async_16(dst + 16 * c, src + 16 * c, 16);
+            for (int i = 0; i < ALL; ++i) cp_async_16(dst + 512 * i, src + 512 * i, 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < ALL; ++i)
+                if (32 * i < n16) cp_async_16(dst + 512 * i, src + 512 * i, 16);
         }
     };
-    const int nb = blk1 - blk0 > warp ? (blk1 - blk0 - warp + kWarps - 1) / kWarps : 0;      // blocks of this warp
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) {
-        if (s < nb) load_block(blk0 + warp + s * kWarps, s);
+    for (int s = 0; s < kTurns; ++s) {
+        if (s < turns) load_turn(s);
         cp_async_commit();
     }
 
@@ -126,35 +202,25 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const DecodeQ4Ar
     double* s_cd = reinterpret_cast<double*>(smem + L::CD_OFF);
     double* s_sd = s_cd + HD / 2;
     const bool rope_q = (p.fuse & 1) != 0, rope_k = (p.fuse & 2) != 0;
-    if (rope_q || (rope_k && owner)) {
-        const int half = p.rope.n_rot / 2;
-        for (int i = tid; i < 2 * HD / 2; i += kThreads) {
-            const int pair = i & (HD / 2 - 1);
-            if (pair >= half) continue;
-            const float f = rope_freq(pair, p.rope.n_rot, p.rope.theta, p.rope.freq_factors);
-            if (i < HD / 2) rope_cs(new_pos, f, s_cos[pair], s_sin[pair]);
-            else if (rope_k && owner) sincos((double)__fmul_rn((float)new_pos, f), &s_sd[pair], &s_cd[pair]);
+    if (tid < HD) {
+        const int pair = tid & (HD / 2 - 1);
+        if (pair < p.rope.n_rot / 2 && (tid < HD / 2 ? rope_q : rope_k && owner)) {
+            float f = p.freq[pair];
+            if (p.rope.freq_factors) f = __fdiv_rn(f, p.rope.freq_factors[pair]);
+            if (tid < HD / 2) rope_cs(new_pos, f, s_cos[pair], s_sin[pair]);
+            else sincos((double)__fmul_rn((float)new_pos, f), &s_sd[pair], &s_cd[pair]);
         }
     }
-    if (p.overlap == 2) pdl_wait();
+    if (p.overlap == 2) {
+        pdl_wait();
+        load_inputs();
+    }
     float* s_in = reinterpret_cast<float*>(smem + L::IN_OFF);
     float* s_qsum = reinterpret_cast<float*>(smem + L::QS_OFF);
     float* s_unit = s_qsum + 16;
     uint32_t* s_new = reinterpret_cast<uint32_t*>(smem + L::NEW_OFF);
-    const int in_rows = G + (owner ? 2 : 0);
-    for (int idx = tid; idx < in_rows * (HD / 4); idx += kThreads) {
-        const int row = idx / (HD / 4), c4 = idx % (HD / 4);
-        const float* src = row < G ? p.q + (size_t)(head0 + row) * HD : (row == G ? p.k_new : p.v_new) + (size_t)kvh * HD;
-        const float* bias = row < G ? (p.pre.bias_q ? p.pre.bias_q + (size_t)(head0 + row) * HD : nullptr)
-                                    : (row == G ? p.pre.bias_k : p.pre.bias_v);
-        if (row >= G && bias) bias += (size_t)kvh * HD;
-        float4 v = *reinterpret_cast<const float4*>(src + c4 * 4);
-        if (bias) {
-            const float4 bv = *reinterpret_cast<const float4*>(bias + c4 * 4);
-            v.x += bv.x; v.y += bv.y; v.z += bv.z; v.w += bv.w;
-        }
-        *reinterpret_cast<float4*>(s_in + (row < G ? row : 8 + row - G) * HD + c4 * 4) = v;
-    }
+    if (tid < G * C4) *reinterpret_cast<float4*>(s_in + tid * 4) = in_q;
+    if (owner && tid < 2 * C4) *reinterpret_cast<float4*>(s_in + 8 * HD + tid * 4) = in_kv;
     __syncthreads();
     // Warp h: head h.  Norm, rotation, then the power of two that brings the largest |q| to [2^13, 2^14), and the group sums.
     if (warp < G) {
@@ -193,9 +259,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const DecodeQ4Ar
         for (int g = 0; g < NG; ++g) {
 #pragma unroll
             for (int off = 16; off; off >>= 1) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], off);
-            if (lane == 0) s_qsum[warp * 2 + g] = sum[g] * 5.9604644775390625e-8f;           // 2^-24
+            if (lane == 0) s_qsum[warp * 2 + g] = sum[g] * 9.5367431640625e-7f;              // 2^-20
         }
-        if (lane == 0) s_unit[warp] = __uint_as_float((uint32_t)(127 + 24 - k) << 23);         // back to q . k
+        if (lane == 0) s_unit[warp] = __uint_as_float((uint32_t)(127 + 20 - k) << 23);         // back to q . k
     } else {
         for (int e = lane; e < HD; e += 32) s_in[warp * HD + e] = 0.f;
         if (lane < 2) s_qsum[warp * 2 + lane] = 0.f;
@@ -234,15 +300,14 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const DecodeQ4Ar
         }
     }
     __syncthreads();
-    // q fragments: step 2i + o of word i takes the nibbles 0, 4 | 2, 6 (o = 0) or 1, 5 | 3, 7 (o = 1, whose codes read 16 times as
-    // large); words: row r hi, row r lo (as row r + 8), and the same for k + 8
+    // q fragments: step 2i + o of word i takes the nibbles 0, 4 | 2, 6 (o = 0) or 1, 5 | 3, 7 (o = 1); words: row r hi, row r lo
+    // (as row r + 8), and the same for k + 8
     for (int idx = tid; idx < HD / 16 * 32; idx += kThreads) {
         const int step = idx >> 5, ln = idx & 31, o = step & 1;
         const float* row = s_in + (ln >> 2) * HD + 32 * (step >> 1) + 8 * (ln & 3) + o;
-        const float f = o ? 0.0625f : 1.f;
         uint4 w;
-        split_half2(row[0] * f, row[4] * f, w.x, w.y);
-        split_half2(row[2] * f, row[6] * f, w.z, w.w);
+        split_half2(F2(row[0], row[4]), w.x, w.y);
+        split_half2(F2(row[2], row[6]), w.z, w.w);
         *reinterpret_cast<uint4*>(smem + L::QF_OFF + idx * 16) = w;
     }
     __syncthreads();
@@ -254,173 +319,199 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const DecodeQ4Ar
     const float c = p.scale * LOG2E * unit;
     const uint4* qf = reinterpret_cast<const uint4*>(smem + L::QF_OFF) + lane;
 
-    float o[HD / 8][4];
-#pragma unroll
-    for (int j = 0; j < HD / 8; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f; }
-    float om[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) om[g] = 0.f;
-    float m_run = -CUDART_INF_F, l_run = 0.f;
-    float pscale = 8192.f;                                   // P d is carried times this; 2^-2 once a step of 2 or more was met
+    // O of head r, dims 16 j + 4 t + {0, 2} (o[2j]) and {1, 3} (o[2j+1]), in the scale of the codes
+    F2 o[HD / 8], om[NG];
+    float m_run, l_run;
+    float pscale = 8192.f;                                   // P d is carried times this
 
-    for (int it = 0; it < nb; ++it) {
-        cp_async_wait<kStages - 1>();
-        __syncwarp();
-        const int b = blk0 + warp + it * kWarps;
-        uint8_t* blk = ring + (it % kStages) * F::BLOCK;
-        const int nrow = npos - b * 16;                      // valid rows, where fewer than 16
-        if (b == plan.blocks - 1) {
-            if (owner) {
-                // the new row, which is not (or not safely) in what was copied
+    // One turn over NB blocks that lie next to each other in the ring.
+    auto turn = [&](auto nb_c, const uint8_t* blk, int nrow) {
+        constexpr int NB = decltype(nb_c)::value, NT = 2 * NB;         // tiles of eight rows
+        // ---- S = q . K ------------------------------------------------------------------------------------------
+        F2 s[NT];                                            // rows 8j + 2t, + 1
+        {
+            uint32_t w[NT][NW], ks[NT][2][NG];
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const uint32_t codes = s_new[w * 32 + lane];
-                    if (w == 0) {
-                        if (F::EPL == 4) *reinterpret_cast<uint16_t*>(blk + q4_k_byte<HD>(new_pos & 15, F::EPL * lane)) = (uint16_t)codes;
-                        else             blk[q4_k_byte<HD>(new_pos & 15, F::EPL * lane)] = (uint8_t)codes;
-                    } else {
+            for (int j = 0; j < NT; ++j) {
+                const uint8_t* row = blk + (j >> 1) * F::BLOCK + (8 * (j & 1) + r) * F::ROWB + t * (F::ROWB / 4);
+                if constexpr (NW == 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(row);
+                    w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2*>(row);
+                    w[j][0] = v.x; w[j][1] = v.y;
+                }
+                load_scales<NG>(blk + (j >> 1) * F::BLOCK + F::KS_OFF + (8 * (j & 1) + 2 * t) * F::SROWB, ks[j]);
+            }
 #pragma unroll
-                        for (int e = 0; e < F::EPL; e += 2) blk[q4_v_byte<HD>(new_pos & 15, F::EPL * lane + e)] = (uint8_t)(codes >> (4 * e));
+            for (int g = 0; g < NG; ++g) {
+                float acc[NT][4];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll
+                for (int i = 2 * g; i < 2 * g + 2; ++i) {
+                    const uint4 a0 = qf[(2 * i) * 32], a1 = qf[(2 * i + 1) * 32];
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const Nibbles n(w[j][i]);
+                        mma_16816(acc[j], a0.x, a0.y, a0.z, a0.w, n.x[0], n.x[2]);
+                        mma_16816(acc[j], a1.x, a1.y, a1.z, a1.w, n.x[1], n.x[3]);
                     }
                 }
+                const F2 qs(qsum[g], qsum[g]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const F2 m(half_hi(ks[j][0][g]), half_hi(ks[j][1][g])), d(half_lo(ks[j][0][g]), half_lo(ks[j][1][g]));
+                    const F2 mq = g == 0 ? m * qs : fma2(m, qs, s[j]);
+                    s[j] = fma2(d, F2(acc[j][0], acc[j][1]) + F2(acc[j][2], acc[j][3]), mq);
+                }
+            }
+        }
+        if (nrow < 16 * NB) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                s[j] = F2(8 * j + 2 * t >= nrow ? -CUDART_INF_F : s[j].x(), 8 * j + 2 * t + 1 >= nrow ? -CUDART_INF_F : s[j].y());
+        }
+
+        // ---- online softmax -------------------------------------------------------------------------------------
+        float mx = m_run;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mx = fmaxf(mx, fmaxf(s[j].x(), s[j].y()));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_safe = mx == -CUDART_INF_F ? 0.f : mx;
+        const float alpha = fast_exp2((m_run - m_safe) * c);
+        const F2 alpha2(alpha, alpha);
+        m_run = mx;
+        F2 sum(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const F2 x = (s[j] + F2(-m_safe, -m_safe)) * F2(c, c);
+            s[j] = F2(fast_exp2(x.x()), fast_exp2(x.y()));
+            sum = j == 0 ? s[j] : sum + s[j];
+        }
+        l_run = fmaf(l_run, alpha, sum.x() + sum.y());
+
+        // ---- O = alpha O + (P d) codes, and P m -----------------------------------------------------------------
+        uint32_t vs[NT][2][NG];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) load_scales<NG>(blk + (j >> 1) * F::BLOCK + F::VS_OFF + (8 * (j & 1) + 2 * t) * F::SROWB, vs[j]);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            uint32_t a[NB][4];
+            om[g] = om[g] * alpha2;
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int j = 2 * h + e;
+                    om[g] = fma2(s[j], F2(half_hi(vs[j][0][g]), half_hi(vs[j][1][g])), om[g]);
+                    const F2 d(half_lo(vs[j][0][g]), half_lo(vs[j][1][g]));
+                    split_half2(s[j] * F2(pscale, pscale) * d, a[h][2 * e], a[h][2 * e + 1]);
+                }
+            }
+            uint32_t w[NB][4];
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
+                const uint4 v = *reinterpret_cast<const uint4*>(blk + h * F::BLOCK + F::V_OFF + g * 512 + lane * 16);
+                w[h][0] = v.x; w[h][1] = v.y; w[h][2] = v.z; w[h][3] = v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < NB; ++h) {
+                    const Nibbles n(w[h][i]);
+                    mma_16816(x, a[h][0], a[h][1], a[h][2], a[h][3], n.x[0], n.x[2]);
+                    mma_16816(y, a[h][0], a[h][1], a[h][2], a[h][3], n.x[1], n.x[3]);
+                }
+                F2& ox = o[2 * (4 * g + i)];
+                F2& oy = o[2 * (4 * g + i) + 1];
+                ox = fma2(ox, alpha2, F2(x[0], x[1]) + F2(x[2], x[3]));
+                oy = fma2(oy, alpha2, F2(y[0], y[1]) + F2(y[2], y[3]));
+            }
+        }
+    };
+
+    // Twice at most: P d is carried times 2^13, which overflows fp16 where a step is 8 or more (values of V spread over
+    // more than 120).  Infinities cannot leave the sums again, so one look at the end finds them, and the warp starts over with
+    // 2^-2, which holds for every fp16 step, and still has 23 bits below the largest.
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) o[j] = F2(0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) om[g] = F2(0.f, 0.f);
+    m_run = -CUDART_INF_F;
+    l_run = 0.f;
+    if (pass) {
+#pragma unroll
+        for (int k = 0; k < kTurns; ++k) {
+            if (k < turns) load_turn(k);
+            cp_async_commit();
+        }
+    }
+    for (int it = 0; it < turns; ++it) {
+        cp_async_wait<kTurns - 1>();
+        __syncwarp();
+        const int b = first(it);
+        const bool two = plan.step == 2 && b + 1 < blk1;
+        uint8_t* blk = ring + (it % kTurns) * 2 * F::BLOCK;
+        const int nrow = npos - b * 16;                      // valid rows from the first block on
+        if (b + (two ? 1 : 0) == plan.blocks - 1) {
+            // the block of the newest row
+            uint8_t* last = blk + (two ? F::BLOCK : 0);
+            if (owner) {
+                // ... which is not (or not safely) in what was copied
+                const int slot = new_pos & 15, D = F::EPL * lane;
+                const uint32_t kcode = s_new[lane], vcode = s_new[32 + lane];
+                if (F::EPL == 4) *reinterpret_cast<uint16_t*>(last + q4_k_byte<HD>(slot, D)) = (uint16_t)kcode;
+                else             last[q4_k_byte<HD>(slot, D)] = (uint8_t)kcode;
+#pragma unroll
+                for (int e = 0; e < F::EPL; e += 2) last[q4_v_byte<HD>(slot, D + e)] = (uint8_t)(vcode >> (4 * e));
                 if (lane < 2 * NG) {
                     const int w = lane / NG, g = lane % NG;
-                    *reinterpret_cast<uint32_t*>(blk + (w ? F::VS_OFF : F::KS_OFF) + (new_pos & 15) * F::SROWB + 4 * g) = s_new[64 + w * 2 + g];
+                    *reinterpret_cast<uint32_t*>(last + (w ? F::VS_OFF : F::KS_OFF) + slot * F::SROWB + 4 * g) = s_new[64 + w * 2 + g];
                 }
             } else if (!append && p.overlap == 2) {
                 // copied ahead of the dependency wait: the newest row may have been written since
-                const uint4* src = reinterpret_cast<const uint4*>(cache + (size_t)b * F::BLOCK);
-                for (int i = lane; i < F::BLOCK / 16; i += 32) reinterpret_cast<uint4*>(blk)[i] = __ldcg(src + i);
+                const uint4* src = reinterpret_cast<const uint4*>(cache + (size_t)(plan.blocks - 1) * F::BLOCK);
+                for (int i = lane; i < F::BLOCK / 16; i += 32) reinterpret_cast<uint4*>(last)[i] = __ldcg(src + i);
             }
             __syncwarp();
             // rows past the end: whatever the memory held, their steps and offsets count as zero
             for (int i = lane; i < 2 * 16 * NG; i += 32) {
                 const int row = (i % (16 * NG)) / NG;
-                if (row >= nrow) reinterpret_cast<uint32_t*>(blk + F::KS_OFF)[i] = 0u;
+                if (row > (new_pos & 15)) reinterpret_cast<uint32_t*>(last + F::KS_OFF)[i] = 0u;
             }
             __syncwarp();
         }
-
-        // ---- S = q . K for two tiles of eight rows --------------------------------------------------------------
-        float s[2][2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            uint32_t w[NW];
-            if constexpr (NW == 4) {
-                const uint4 v = *reinterpret_cast<const uint4*>(blk + (8 * j + r) * F::ROWB + t * 16);
-                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-            } else {
-                const uint2 v = *reinterpret_cast<const uint2*>(blk + (8 * j + r) * F::ROWB + t * 8);
-                w[0] = v.x; w[1] = v.y;
-            }
-            s[j][0] = s[j][1] = 0.f;
-            const uint32_t* sc = reinterpret_cast<const uint32_t*>(blk + F::KS_OFF + (8 * j + 2 * t) * F::SROWB);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 2 * g; i < 2 * g + 2; ++i) {
-                    const uint32_t w8 = w[i] >> 8;
-                    const uint4 a0 = qf[(2 * i) * 32], a1 = qf[(2 * i + 1) * 32];
-                    mma_16816(acc, a0.x, a0.y, a0.z, a0.w, w[i] & 0x000F000Fu, w8 & 0x000F000Fu);
-                    mma_16816(acc, a1.x, a1.y, a1.z, a1.w, w[i] & 0x00F000F0u, w8 & 0x00F000F0u);
-                }
-                const float2 s0 = half2_word(sc[g]), s1 = half2_word(sc[NG + g]);
-                s[j][0] = fmaf(s0.x, acc[0] + acc[2], fmaf(s0.y, qsum[g], s[j][0]));
-                s[j][1] = fmaf(s1.x, acc[1] + acc[3], fmaf(s1.y, qsum[g], s[j][1]));
-            }
-        }
-        if (nrow < 16) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (8 * j + 2 * t + e >= nrow) s[j][e] = -CUDART_INF_F;
-        }
-
-        // ---- online softmax -------------------------------------------------------------------------------------
-        float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m_run, mx);
-        const float m_safe = m_new == -CUDART_INF_F ? 0.f : m_new;
-        const float alpha = fast_exp2((m_run - m_safe) * c);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) s[j][e] = fast_exp2((s[j][e] - m_safe) * c);
-        l_run = fmaf(l_run, alpha, (s[0][0] + s[0][1]) + (s[1][0] + s[1][1]));
-        m_run = m_new;
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-            for (int j = 0; j < HD / 8; ++j) { o[j][0] *= alpha; o[j][1] *= alpha; o[j][2] *= alpha; o[j][3] *= alpha; }
-#pragma unroll
-            for (int g = 0; g < NG; ++g) om[g] *= alpha;
-        }
-
-        // ---- O += (P d) codes, and P m --------------------------------------------------------------------------
-        uint32_t vs[2][2][NG];                               // scales of rows 8j + 2t + e
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t* sc = reinterpret_cast<const uint32_t*>(blk + F::VS_OFF + (8 * j + 2 * t) * F::SROWB);
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int g = 0; g < NG; ++g) vs[j][e][g] = sc[e * NG + g];
-        }
-        uint32_t big = 0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) big |= vs[j][0][g] | vs[j][1][g];
-        if (pscale > 1.f && __any_sync(0xffffffffu, (big & 0x4000u) != 0)) {     // a step of 2 or more
-            pscale = 0.25f;
-#pragma unroll
-            for (int j = 0; j < HD / 8; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] *= 3.0517578125e-5f;         // 2^-15
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            float pd[2][2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float2 dm = half2_word(vs[j][e][g]);
-                    om[g] = fmaf(s[j][e], dm.y, om[g]);
-                    pd[j][e] = s[j][e] * pscale * dm.x;
-                }
-            uint32_t a0, a1, a2, a3;
-            split_half2(pd[0][0], pd[0][1], a0, a1);
-            split_half2(pd[1][0], pd[1][1], a2, a3);
-            const uint4 v = *reinterpret_cast<const uint4*>(blk + F::V_OFF + g * 512 + lane * 16);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = 4 * g + i;
-                const uint32_t w8 = w[i] >> 8;
-                mma_16816(o[2 * j], a0, a1, a2, a3, w[i] & 0x000F000Fu, w8 & 0x000F000Fu);
-                mma_16816(o[2 * j + 1], a0, a1, a2, a3, w[i] & 0x00F000F0u, w8 & 0x00F000F0u);
-            }
-        }
-        __syncwarp();                                        // every lane has read the stage
-        const int nxt = it + kStages;
-        if (nxt < nb) load_block(blk0 + warp + nxt * kWarps, it % kStages);
+        if (two) turn(std::integral_constant<int, 2>{}, blk, nrow);
+        else     turn(std::integral_constant<int, 1>{}, blk, nrow);
+        __syncwarp();                                        // every lane has read the ring slots
+        if (it + kTurns < turns) load_turn(it + kTurns);
         cp_async_commit();
+    }
+    cp_async_wait<0>();
+    F2 any = o[0];
+#pragma unroll
+    for (int j = 1; j < HD / 8; ++j) any = any + o[j];
+    // (an infinity or a NaN in any of them leaves no finite sum)
+    if (!__any_sync(0xffffffffu, !(fabsf(any.x()) + fabsf(any.y()) <= 3.402823466e38f))) break;
+    pscale = 0.25f;
     }
 
     // ---- merge the warps: O of a warp scaled by e^(m_w - M), sums in warp order ----------------------------------
-    cp_async_wait<0>();
     __syncthreads();
     float* mO = reinterpret_cast<float*>(smem);
     float* mML = reinterpret_cast<float*>(smem + L::ML_OFF);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+    float oms[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        om[g] += __shfl_xor_sync(0xffffffffu, om[g], 1);
-        om[g] += __shfl_xor_sync(0xffffffffu, om[g], 2);
+        float v = om[g].x() + om[g].y();
+        v += __shfl_xor_sync(0xffffffffu, v, 1);
+        oms[g] = v + __shfl_xor_sync(0xffffffffu, v, 2);
     }
     const float m_raw = m_run * unit;                        // q . k, the unit the CTAs share
     if (t == 0) *reinterpret_cast<float2*>(&mML[(warp * 8 + r) * 2]) = make_float2(m_raw, l_run);
@@ -431,20 +522,18 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const DecodeQ4Ar
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mML[(w * 8 + r) * 2]);
         const float wgt = m_raw == -CUDART_INF_F ? 0.f : fast_exp2((m_raw - M) * c_raw);
-        const float lo = 16777216.f / pscale * wgt, hi = 1048576.f / pscale * wgt;     // 2^24, 2^20: the scale of the codes
+        const float f = 1048576.f / pscale * wgt;            // 2^20: the scale of the codes
         float* dst = mO + (size_t)(warp * 8 + r) * L::MSTRIDE + 4 * t;
 #pragma unroll
         for (int j = 0; j < HD / 16; ++j) {
-            const float a = om[j / 4] * wgt;
-            const float* e = o[2 * j];
-            const float* f = o[2 * j + 1];
-            *reinterpret_cast<float4*>(dst + 16 * j) = make_float4(fmaf(e[0] + e[2], lo, a), fmaf(f[0] + f[2], hi, a),
-                                                                   fmaf(e[1] + e[3], lo, a), fmaf(f[1] + f[3], hi, a));
+            const float a = oms[j / 4] * wgt;
+            *reinterpret_cast<float4*>(dst + 16 * j) = make_float4(fmaf(o[2 * j].x(), f, a), fmaf(o[2 * j + 1].x(), f, a),
+                                                                   fmaf(o[2 * j].y(), f, a), fmaf(o[2 * j + 1].y(), f, a));
         }
     }
     __syncthreads();
     RunState st[S::N];
-    if (tid < kMergeThreads) {
+    if (tid < MT) {
 #pragma unroll
         for (int k = 0; k < S::N; ++k) {
             const int row = S::row(tid, k), c4 = S::col4(tid, k);
@@ -467,37 +556,37 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const DecodeQ4Ar
     // ---- merge across the CTAs of these heads (one or two levels, see decode.cu) -----------------------------------
     if (plan.active > 1) {
         const size_t blk = (size_t)GP * HD;
-        if (tid < kMergeThreads) {
+        if (tid < MT) {
             const size_t part = (size_t)vh * p.n_splits + split;
-            store_part<HD, false>(p.ws_o + part * blk, p.ws_ml + part * GP * 2, G, st);
+            store_part<HD, false, MT>(p.ws_o + part * blk, p.ws_ml + part * GP * 2, G, st);
         }
         const int group = plan.active <= 16 ? plan.active : p.group;
         const int grp = split / group;
         const int grp_n = min(group, plan.active - grp * group);
         if (!arrive_last(p.tickets + vh * p.n_groups + grp, grp_n)) return;
-        if (tid < kMergeThreads) {
+        if (tid < MT) {
             const size_t part0 = (size_t)vh * p.n_splits + (size_t)grp * group;
-            merge_parts<HD, false>(p.ws_o + part0 * blk, p.ws_ml + part0 * GP * 2, grp_n, GP, c_raw, st);
+            merge_parts<HD, false, MT>(p.ws_o + part0 * blk, p.ws_ml + part0 * GP * 2, grp_n, GP, c_raw, st);
         }
         const int n_grp = (plan.active + group - 1) / group;
         if (n_grp > 1) {
-            if (tid < kMergeThreads) {
+            if (tid < MT) {
                 const size_t gpart = (size_t)vh * p.n_groups + grp;
-                store_part<HD, false>(p.grp_o + gpart * blk, p.grp_ml + gpart * GP * 2, G, st);
+                store_part<HD, false, MT>(p.grp_o + gpart * blk, p.grp_ml + gpart * GP * 2, G, st);
             }
             if (!arrive_last(p.tickets + p.n_kv * p.head_blocks * p.n_groups + vh, n_grp)) return;
-            if (tid < kMergeThreads) {
+            if (tid < MT) {
                 const size_t g0 = (size_t)vh * p.n_groups;
-                merge_parts<HD, false>(p.grp_o + g0 * blk, p.grp_ml + g0 * GP * 2, n_grp, GP, c_raw, st);
+                merge_parts<HD, false, MT>(p.grp_o + g0 * blk, p.grp_ml + g0 * GP * 2, n_grp, GP, c_raw, st);
             }
         }
     }
-    if (tid < kMergeThreads) {
+    if (tid < MT) {
         // a NaN among the scores or values shows in the output
 #pragma unroll
         for (int k = 0; k < S::N; ++k)
             if (st[k].L != st[k].L) { st[k].acc = make_float4(st[k].L, st[k].L, st[k].L, st[k].L); st[k].L = 1.f; }
-        emit_final<HD, false>(p, head0, G, st);
+        emit_final<HD, false, MT>(p, head0, G, st);
     }
 }
 

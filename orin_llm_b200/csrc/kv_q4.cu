@@ -1,4 +1,8 @@
 // Writing, reading back and rolling the 4-bit KV cache, and the prologue of the prefill call that uses it.
+#include <math.h>
+
+#include <mutex>
+
 #include "kv_q4.cuh"
 
 namespace oattn {
@@ -116,7 +120,7 @@ __global__ void __launch_bounds__(kShiftThreads) kv_shift_q4_kernel(uint8_t* cac
 constexpr int kPrologueThreads = 256;
 
 template <int HD>
-__global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(const KvQ4PrologueArgs p) {
+__global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(const __grid_constant__ KvQ4PrologueArgs p) {
     using F = Q4<HD>;
     const PrefillArgs& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -141,7 +145,8 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
     const int b = blockIdx.x, pos = a.n_past + b;
     if (rope_q || rope_k) {
         for (int i = tid; i < a.rope.n_rot / 2; i += kPrologueThreads) {
-            const float f = rope_freq(i, a.rope.n_rot, a.rope.theta, a.rope.freq_factors);
+            float f = p.freq[i];
+            if (a.rope.freq_factors) f = __fdiv_rn(f, a.rope.freq_factors[i]);
             sincos((double)__fmul_rn((float)pos, f), &s_sin[i], &s_cos[i]);
         }
     }
@@ -196,6 +201,29 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
 }
 
 } // namespace
+
+void rope_freq_table(const RopeArgs& r, float (&freq)[64]) {
+    // a model has one (theta, n_rot); the last few are kept
+    struct Entry { int n_rot = 0; float theta = 0.f; float freq[64]; };
+    static Entry kept[4];
+    static int next = 0;
+    static std::mutex mutex;
+    std::lock_guard<std::mutex> lock(mutex);
+    Entry* e = nullptr;
+    for (Entry& k : kept)
+        if (k.n_rot == r.n_rot && k.theta == r.theta) e = &k;
+    if (!e) {
+        e = &kept[next];
+        next = (next + 1) % 4;
+        e->n_rot = r.n_rot;
+        e->theta = r.theta;
+        for (int i = 0; i < 64; ++i) {
+            const float x = r.n_rot > 0 ? (-2.0f * (float)i) / (float)r.n_rot : 0.f;
+            e->freq[i] = (float)exp2((double)x * log2((double)r.theta));
+        }
+    }
+    for (int i = 0; i < 64; ++i) freq[i] = e->freq[i];
+}
 
 cudaError_t launch_kv_store_q4(uint8_t* cache, const float* k, const float* v, int heads, int head_dim, int n_ctx, int pos_base,
                                int batch, const int* d_pos, cudaStream_t stream, unsigned long long* launches) {

@@ -127,12 +127,17 @@ __device__ __forceinline__ void q4_store_row(uint8_t* blk, int s, uint32_t codes
 // fp16 value of a code: m + d * code, exact in fp32 but for far apart m and d, rounded to fp16 once.
 __device__ __forceinline__ float q4_value(uint32_t code, float d, float m) { return fmaf((float)code, d, m); }
 
+// The frequencies rope_freq() computes, before the factors, once on the host: in the kernels every CTA would spend two double
+// transcendentals per pair on them, on the path in front of its first product.
+void rope_freq_table(const RopeArgs& r, float (&freq)[64]);
+
 struct KvQ4PrologueArgs {
     PrefillArgs a;             // kc, vc, out are those of the attention launch behind it and not used here
     uint8_t* cache;
     __half* k16;               // fp16 copies of the cache rows [n_kv][n_past + batch][hd]
     __half* v16;
     int cache_ctx;             // positions of the 4-bit cache
+    float freq[64];            // see rope_freq_table
 };
 
 cudaError_t launch_kv_store_q4(uint8_t* cache, const float* k, const float* v, int heads, int head_dim, int n_ctx, int pos_base,
@@ -162,6 +167,7 @@ struct DecodeQ4Args {
     int fuse, overlap;
     RopeArgs rope;
     PreArgs pre;
+    float freq[64];                     // RoPE frequencies before the optional factors, theta^(-2i/n_rot) rounded to fp32
     int emit_partial = 0;
     int8_t* out_qs = nullptr;
     float* out_scales = nullptr;

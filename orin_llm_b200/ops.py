@@ -317,63 +317,74 @@ class KVCache:
 # The counterparts of kv_store_*, kv_shift, attn_decode and attn_prefill over a cache of 4.5 bits a value (format in
 # include/orin_attn_b200.h), and its read-back.  No counterpart in the reference.
 
-def _q4_tensor(name, t, dtype, numel, optional=False):
-    """The checks the C entry cannot make: a contiguous tensor of that type and size on the current CUDA device."""
-    if t is None and optional:
-        return
+def _q4_check(dev, name, t, dtype, numel):
+    """The checks the C entry cannot make: a contiguous tensor of that type and size on CUDA device `dev`; -> its address."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s: a tensor is needed, got %s" % (name, type(t).__name__))
-    if t.dtype != dtype or not t.is_contiguous() or t.numel() < numel:
+    if t.dtype is not dtype or t.numel() < numel or not t.is_contiguous():
         raise ValueError("%s: a contiguous %s tensor of at least %d elements is needed, got %s %s%s" % (
             name, dtype, numel, t.dtype, list(t.shape), "" if t.is_contiguous() else ", not contiguous"))
-    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
-        raise ValueError("%s: on %s, the current device is cuda:%d" % (name, t.device, torch.cuda.current_device()))
+    if t.get_device() != dev:
+        raise ValueError("%s: on %s, the cache on device %d" % (name, t.device, dev))
+    return t.data_ptr()
 
 
 def _q4_cache(cache, layers, n_kv, head_dim, n_ctx):
+    """Checks a cache of `layers` layers; -> its device, which has to be the current one, and its address."""
     nbytes = kv_q4_bytes(n_kv, head_dim, n_ctx)
-    if nbytes == 0:
+    if nbytes == 0 or layers <= 0:
         raise capi.AttnError(capi.ERR_UNSUPPORTED, "4-bit cache: head_dim 64 or 128, at least one head and one position")
-    _q4_tensor("cache", cache, torch.uint8, layers * nbytes)
+    dev = cache.get_device() if isinstance(cache, torch.Tensor) else -1
+    ptr = _q4_check(dev, "cache", cache, torch.uint8, layers * nbytes)
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise ValueError("cache: on %s, not on the current CUDA device" % cache.device)
+    return dev, ptr
+
+
+def _q4_stream(dev):
+    s = _state["stream"]
+    return torch._C._cuda_getCurrentRawStream(dev) if s is None else s
 
 
 def kv_q4_bytes(n_kv, head_dim, n_ctx):
-    """Bytes of one layer of a 4-bit cache."""
-    return int(capi.lib().oattn_kv_q4_bytes(n_kv, head_dim, n_ctx))
+    """Bytes of one layer of a 4-bit cache (oattn_kv_q4_bytes); 0 for a shape that has none."""
+    if n_kv <= 0 or n_ctx <= 0 or n_ctx > 1 << 30 or head_dim not in (64, 128):
+        return 0
+    return n_kv * ((n_ctx + 15) // 16) * 18 * head_dim
 
 
 def kv_store_q4_batch(cache, k, v, heads, head_dim, n_ctx, pos_base, batch):
     """kv_store_batch into a 4-bit cache: k, v [batch][heads][head_dim] fp32 at positions pos_base + b."""
-    _q4_cache(cache, 1, heads, head_dim, n_ctx)
-    for name, t in (("k", k), ("v", v)):
-        _q4_tensor(name, t, torch.float32, batch * heads * head_dim)
-    capi.check(capi.lib().oattn_kv_store_q4(_ptr(cache), _ptr(k), _ptr(v), heads, head_dim, n_ctx, pos_base, batch, None, _stream()))
+    dev, cp = _q4_cache(cache, 1, heads, head_dim, n_ctx)
+    n = batch * heads * head_dim
+    kp, vp = _q4_check(dev, "k", k, torch.float32, n), _q4_check(dev, "v", v, torch.float32, n)
+    capi.check(capi.lib().oattn_kv_store_q4(cp, kp, vp, heads, head_dim, n_ctx, pos_base, batch, None, _q4_stream(dev)))
 
 
 def kv_store_q4_ind(cache, k, v, heads, head_dim, n_ctx, d_pos):
     """kv_store_ind into a 4-bit cache: one row at *d_pos."""
-    _q4_cache(cache, 1, heads, head_dim, n_ctx)
-    for name, t in (("k", k), ("v", v)):
-        _q4_tensor(name, t, torch.float32, heads * head_dim)
-    _q4_tensor("d_pos", d_pos, torch.int32, 1)
-    capi.check(capi.lib().oattn_kv_store_q4(_ptr(cache), _ptr(k), _ptr(v), heads, head_dim, n_ctx, 0, 1, _ptr(d_pos), _stream()))
+    dev, cp = _q4_cache(cache, 1, heads, head_dim, n_ctx)
+    n = heads * head_dim
+    kp, vp = _q4_check(dev, "k", k, torch.float32, n), _q4_check(dev, "v", v, torch.float32, n)
+    pp = _q4_check(dev, "d_pos", d_pos, torch.int32, 1)
+    capi.check(capi.lib().oattn_kv_store_q4(cp, kp, vp, heads, head_dim, n_ctx, 0, 1, pp, _q4_stream(dev)))
 
 
 def kv_load_q4(cache, kc, vc, heads, head_dim, n_ctx, row_base, rows, dst_ctx=None, dst_base=0):
     """Rows [row_base, row_base + rows) of a 4-bit cache as fp16, into kc, vc [heads][dst_ctx][head_dim] from row dst_base
     on (default: a block of exactly these rows)."""
-    dst_ctx = rows if dst_ctx is None else dst_ctx
-    _q4_cache(cache, 1, heads, head_dim, n_ctx)
-    for name, t in (("kc", kc), ("vc", vc)):
-        _q4_tensor(name, t, torch.float16, heads * dst_ctx * head_dim)
-    capi.check(capi.lib().oattn_kv_load_q4(_ptr(cache), _ptr(kc), _ptr(vc), heads, head_dim, n_ctx, row_base, rows, dst_ctx, dst_base,
-                                           _stream()))
+    if dst_ctx is None:
+        dst_ctx = rows
+    dev, cp = _q4_cache(cache, 1, heads, head_dim, n_ctx)
+    n = heads * dst_ctx * head_dim
+    kp, vp = _q4_check(dev, "kc", kc, torch.float16, n), _q4_check(dev, "vc", vc, torch.float16, n)
+    capi.check(capi.lib().oattn_kv_load_q4(cp, kp, vp, heads, head_dim, n_ctx, row_base, rows, dst_ctx, dst_base, _q4_stream(dev)))
 
 
 def kv_shift_q4(cache, n_layer, n_kv, head_dim, n_ctx, n_keep, shift):
     """kv_shift on the 4-bit cache of n_layer layers, in place."""
-    _q4_cache(cache, n_layer, n_kv, head_dim, n_ctx)
-    capi.check(capi.lib().oattn_kv_shift_q4(_ptr(cache), n_layer, n_kv, head_dim, n_ctx, n_keep, shift, _stream()))
+    dev, cp = _q4_cache(cache, n_layer, n_kv, head_dim, n_ctx)
+    capi.check(capi.lib().oattn_kv_shift_q4(cp, n_layer, n_kv, head_dim, n_ctx, n_keep, shift, _q4_stream(dev)))
 
 
 def decode_q4_workspace(n_head, n_kv, head_dim):
@@ -406,19 +417,21 @@ def prefill_q4_workspace(n_head, n_kv, head_dim, batch, rows):
 def attn_decode_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, d_pos, scale, fuse=FUSE_ALL, rope=None,
                    workspace=None, ext=None):
     """attn_decode over one layer of a 4-bit cache, the new row quantised and appended in the same launch."""
-    _q4_cache(cache, 1, n_kv, head_dim, n_ctx)
-    append = bool(fuse & FUSE_KV_APPEND)
-    _q4_tensor("q", q, torch.float32, n_head * head_dim)
-    _q4_tensor("k_new", k_new, torch.float32, n_kv * head_dim if append else 0, not append)
-    _q4_tensor("v_new", v_new, torch.float32, n_kv * head_dim if append else 0, not append)
-    _q4_tensor("out", out, torch.float32, n_head * head_dim, bool(ext) and ext.get("out_qs") is not None)
-    _q4_tensor("d_pos", d_pos, torch.int32, 1)
+    dev, cp = _q4_cache(cache, 1, n_kv, head_dim, n_ctx)
+    qp = _q4_check(dev, "q", q, torch.float32, n_head * head_dim)
+    kp = vp = op = None
+    if fuse & FUSE_KV_APPEND:
+        kp = _q4_check(dev, "k_new", k_new, torch.float32, n_kv * head_dim)
+        vp = _q4_check(dev, "v_new", v_new, torch.float32, n_kv * head_dim)
+    if out is not None or not ext or ext.get("out_qs") is None:
+        op = _q4_check(dev, "out", out, torch.float32, n_head * head_dim)
+    pp = _q4_check(dev, "d_pos", d_pos, torch.int32, 1)
     ws = workspace if workspace is not None else decode_q4_workspace(n_head, n_kv, head_dim)
-    _q4_tensor("workspace", ws, torch.uint8, 0)
+    wp = _q4_check(dev, "workspace", ws, torch.uint8, 0)
     ref, keep = _rope_params(rope)
     eref, ekeep = _ext_params(ext)
-    capi.check(capi.lib().oattn_decode_q4(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(cache), _ptr(out), n_head, n_kv, head_dim, n_ctx,
-                                          _ptr(d_pos), scale, fuse, ref, eref, _ptr(ws), ws.numel(), _stream()))
+    capi.check(capi.lib().oattn_decode_q4(qp, kp, vp, cp, op, n_head, n_kv, head_dim, n_ctx, pp, scale, fuse, ref, eref, wp,
+                                          ws.numel(), _q4_stream(dev)))
     del keep, ekeep
 
 
@@ -426,21 +439,22 @@ def attn_prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, 
                     workspace=None, ext=None):
     """attn_prefill over one layer of a 4-bit cache, the chunk's rows quantised and appended first.  out: fp32 or fp16
     [batch][n_head][head_dim] (the attention runs on fp16 operands either way)."""
-    _q4_cache(cache, 1, n_kv, head_dim, n_ctx)
-    append = bool(fuse & FUSE_KV_APPEND)
-    _q4_tensor("q", q, torch.float32, batch * n_head * head_dim)
-    _q4_tensor("k_new", k_new, torch.float32, batch * n_kv * head_dim if append else 0, not append)
-    _q4_tensor("v_new", v_new, torch.float32, batch * n_kv * head_dim if append else 0, not append)
-    half = isinstance(out, torch.Tensor) and out.dtype == torch.float16
-    _q4_tensor("out", out, torch.float16 if half else torch.float32, batch * n_head * head_dim,
-               bool(ext) and ext.get("out_mmq") is not None)
+    dev, cp = _q4_cache(cache, 1, n_kv, head_dim, n_ctx)
+    qp = _q4_check(dev, "q", q, torch.float32, batch * n_head * head_dim)
+    kp = vp = op = hp = None
+    if fuse & FUSE_KV_APPEND:
+        kp = _q4_check(dev, "k_new", k_new, torch.float32, batch * n_kv * head_dim)
+        vp = _q4_check(dev, "v_new", v_new, torch.float32, batch * n_kv * head_dim)
+    if isinstance(out, torch.Tensor) and out.dtype is torch.float16:
+        hp = _q4_check(dev, "out", out, torch.float16, batch * n_head * head_dim)
+    elif out is not None or not ext or ext.get("out_mmq") is None:
+        op = _q4_check(dev, "out", out, torch.float32, batch * n_head * head_dim)
     ws = workspace if workspace is not None else prefill_q4_workspace(n_head, n_kv, head_dim, batch, max(n_ctx, batch))
-    _q4_tensor("workspace", ws, torch.uint8, 0)
+    wp = _q4_check(dev, "workspace", ws, torch.uint8, 0)
     ref, keep = _rope_params(rope)
     eref, ekeep = _ext_params(ext)
-    capi.check(capi.lib().oattn_prefill_q4(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(cache), _ptr(None if half else out),
-                                           _ptr(out if half else None), n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse,
-                                           ref, eref, _ptr(ws), ws.numel(), _stream()))
+    capi.check(capi.lib().oattn_prefill_q4(qp, kp, vp, cp, op, hp, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse, ref,
+                                           eref, wp, ws.numel(), _q4_stream(dev)))
     del keep, ekeep
 
 
