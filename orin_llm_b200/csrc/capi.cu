@@ -103,6 +103,7 @@ int oattn_init(int device) {
         if ((e = prefill_mma_set_attributes()) != cudaSuccess) return cuda_fail(e, "prefill (mma) attributes");
         if ((e = prefill_tc_set_attributes()) != cudaSuccess) return cuda_fail(e, "prefill (tcgen05) attributes");
         if ((e = decode_q4_set_attributes()) != cudaSuccess) return cuda_fail(e, "decode (4-bit cache) attributes");
+        if ((e = kv_q4_set_attributes()) != cudaSuccess) return cuda_fail(e, "4-bit cache attributes");
         void* scratch = nullptr;      // look the built-in scratch block up now, so that oattn_decode_noalloc never has to
         if ((e = decode_static_scratch(&scratch)) != cudaSuccess) return cuda_fail(e, "cudaGetSymbolAddress(built-in scratch)");
         unsigned* tickets = nullptr;  // ... and the arrival counters of the decode launches
@@ -513,6 +514,7 @@ int oattn_kv_store_q4(void* cache, const float* k, const float* v, int heads, in
     const int rc = check_q4(cache, heads, head_dim, n_ctx);
     if (rc != OATTN_OK) return rc;
     if (!k || !v || batch <= 0) return OATTN_ERR_ARG;
+    if (heads > 65535) return OATTN_ERR_UNSUPPORTED;                   // one grid row per head
     if (((uintptr_t)k | (uintptr_t)v) & 15) return OATTN_ERR_ARG;      // read as float4
     if (d_pos && batch != 1) return OATTN_ERR_ARG;
     if (!d_pos && (pos_base < 0 || pos_base > n_ctx - batch)) return OATTN_ERR_ARG;
@@ -539,7 +541,7 @@ int oattn_kv_shift_q4(void* cache, int n_layer, int n_kv, int head_dim, int n_ct
     const int rc = check_q4(cache, n_kv, head_dim, n_ctx);
     if (rc != OATTN_OK) return rc;
     if (n_layer <= 0 || n_keep < 0 || shift <= 0 || n_keep > n_ctx - shift) return OATTN_ERR_ARG;
-    if ((long long)n_layer * n_kv > 0x7fffffffLL) return OATTN_ERR_UNSUPPORTED;
+    if ((long long)n_layer * n_kv > 65535) return OATTN_ERR_UNSUPPORTED;         // one grid row per (layer, head)
     cudaError_t e = launch_kv_shift_q4(reinterpret_cast<uint8_t*>(cache), n_layer, n_kv, head_dim, n_ctx, n_keep, shift,
                                        (cudaStream_t)stream, &g_launches);
     return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "kv_shift_q4 launch");

@@ -22,9 +22,15 @@ namespace oattn {
 
 namespace {
 
-constexpr int kWarps = 8;
+#ifndef KW
+#define KW 8
+#define KC 2
+#define KT 2
+#endif
+constexpr int kWarps = KW;
+constexpr int kCtas = KC;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTurns = 2;                  // pairs of blocks in the ring of a warp
+constexpr int kTurns = KT;                  // pairs of blocks in the ring of a warp
 
 template <int HD>
 struct Q4Smem {
@@ -106,10 +112,10 @@ struct Nibbles {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const __grid_constant__ DecodeQ4Args p) {
+__global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid_constant__ DecodeQ4Args p) {
     using F = Q4<HD>;
     using L = Q4Smem<HD>;
-    constexpr int MT = HD == 128 ? 256 : 128;    // threads that hold pieces of the merged block
+    constexpr int MT = HD == 128 && kThreads >= 256 ? 256 : 128;    // threads that hold pieces of the merged block
     using S = Slots<HD, false, MT>;
     constexpr int NG = F::NG, NW = HD / 32;      // groups of a row, code words of a lane per K row
     extern __shared__ __align__(128) uint8_t smem[];
@@ -124,14 +130,18 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const __grid_con
     // together and, where the order against preceding kernels allows it, along with the position word.
     constexpr int C4 = HD / 4;
     const bool append = (p.fuse & 4) != 0;
-    float4 in_q = make_float4(0.f, 0.f, 0.f, 0.f), in_kv = in_q;
+    constexpr int NQ = (8 * C4 + kThreads - 1) / kThreads;
+    float4 in_q[NQ], in_kv;
     auto load_inputs = [&]() {
-        if (tid < G * C4) {
-            const size_t at = (size_t)head0 * HD + tid * 4;
-            in_q = *reinterpret_cast<const float4*>(p.q + at);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int piece = tid + i * kThreads;
+            if (piece >= G * C4) continue;
+            const size_t at = (size_t)head0 * HD + piece * 4;
+            in_q[i] = *reinterpret_cast<const float4*>(p.q + at);
             if (p.pre.bias_q) {
                 const float4 b = *reinterpret_cast<const float4*>(p.pre.bias_q + at);
-                in_q.x += b.x; in_q.y += b.y; in_q.z += b.z; in_q.w += b.w;
+                in_q[i].x += b.x; in_q[i].y += b.y; in_q[i].z += b.z; in_q[i].w += b.w;
             }
         }
         if (append && tid < 2 * C4) {
@@ -144,7 +154,6 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const __grid_con
             }
         }
     };
-    static_assert(8 * C4 <= kThreads, "one piece of q per thread");
 
     pdl_trigger();
     if (p.overlap != 2) {
@@ -219,12 +228,20 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const __grid_con
     float* s_qsum = reinterpret_cast<float*>(smem + L::QS_OFF);
     float* s_unit = s_qsum + 16;
     uint32_t* s_new = reinterpret_cast<uint32_t*>(smem + L::NEW_OFF);
-    if (tid < G * C4) *reinterpret_cast<float4*>(s_in + tid * 4) = in_q;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+        if (tid + i * kThreads < G * C4) *reinterpret_cast<float4*>(s_in + (tid + i * kThreads) * 4) = in_q[i];
     if (owner && tid < 2 * C4) *reinterpret_cast<float4*>(s_in + 8 * HD + tid * 4) = in_kv;
     __syncthreads();
-    // Warp h: head h.  Norm, rotation, then the power of two that brings the largest |q| to [2^13, 2^14), and the group sums.
-    if (warp < G) {
-        float* row = s_in + warp * HD;
+    // One warp per head.  Norm, rotation, then the power of two that brings the largest |q| to [2^13, 2^14), and the group sums.
+    for (int h = warp; h < 8; h += kWarps) {
+        float* row = s_in + h * HD;
+        if (h >= G) {
+            for (int e = lane; e < HD; e += 32) row[e] = 0.f;
+            if (lane < 2) s_qsum[h * 2 + lane] = 0.f;
+            if (lane == 0) s_unit[h] = 1.f;
+            continue;
+        }
         if (p.pre.norm_q) {
             const float rn = warp_row_rnorm(row, nullptr, HD, p.pre.eps, lane);
             __syncwarp();
@@ -259,13 +276,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const __grid_con
         for (int g = 0; g < NG; ++g) {
 #pragma unroll
             for (int off = 16; off; off >>= 1) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], off);
-            if (lane == 0) s_qsum[warp * 2 + g] = sum[g] * 9.5367431640625e-7f;              // 2^-20
+            if (lane == 0) s_qsum[h * 2 + g] = sum[g] * 9.5367431640625e-7f;              // 2^-20
         }
-        if (lane == 0) s_unit[warp] = __uint_as_float((uint32_t)(127 + 20 - k) << 23);         // back to q . k
-    } else {
-        for (int e = lane; e < HD; e += 32) s_in[warp * HD + e] = 0.f;
-        if (lane < 2) s_qsum[warp * 2 + lane] = 0.f;
-        if (lane == 0) s_unit[warp] = 1.f;
+        if (lane == 0) s_unit[h] = __uint_as_float((uint32_t)(127 + 20 - k) << 23);         // back to q . k
     }
     // the new row of K (warp 0) and V (warp 1): codes, into the cache and into s_new for this CTA's copy of the block
     if (owner && warp < 2) {
@@ -592,7 +605,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_q4_kernel(const __grid_con
 
 } // namespace
 
-int decode_q4_num_splits(int n_kv, int sm_count) { return decode_num_splits(n_kv, sm_count); }
+int decode_q4_num_splits(int n_kv, int sm_count) {
+    return max(1, min(DECODE_MAX_SPLITS, kCtas * sm_count / n_kv));
+}
 
 cudaError_t decode_q4_set_attributes() {
     cudaError_t e = cudaFuncSetAttribute(decode_q4_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<128>::TOTAL);

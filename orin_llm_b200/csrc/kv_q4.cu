@@ -9,51 +9,189 @@ namespace oattn {
 
 namespace {
 
-template <int HD>
-__device__ __forceinline__ void load_row(const float* src, int lane, float (&x)[Q4<HD>::EPL]) {
-#pragma unroll
-    for (int e = 0; e < Q4<HD>::EPL; ++e) x[e] = src[Q4<HD>::EPL * lane + e];
-}
+__device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
-// ---- store: one warp per (token, head, K or V) row --------------------------------------------------------------
-constexpr int kStoreWarps = 8;
+// ---- store --------------------------------------------------------------------------------------------------------
+// One CTA per (block of 16 positions, kv head): warps 0..3 four rows of K each, warps 4..7 four rows of V.  Eight lanes (HD 128)
+// or four (HD 64) share a row, four lanes a 64-dim group, a lane 16 dims: the 8 of word t, i and the 8 of word t, i + 1, so that
+// it owns two neighbouring code words of K, and the minimum and maximum of a group cost two shuffles.  The block is put
+// together in shared memory and leaves in 16-byte pieces; of a block at either end of the range only the stored rows' bytes do.
+// Bound by the fp32 rows it reads; FIXME measured.
+constexpr int kStoreThreads = 256;
 
 template <int HD>
-__global__ void __launch_bounds__(32 * kStoreWarps) kv_store_q4_kernel(uint8_t* cache, const float* k, const float* v, int heads,
-                                                                       int n_ctx, int pos_base, int batch, const int* d_pos) {
-    const int lane = threadIdx.x & 31;
-    const long long job = (long long)blockIdx.x * kStoreWarps + (threadIdx.x >> 5);
-    const long long row = job >> 1;                       // token * heads + head
-    if (row >= (long long)batch * heads) return;
-    const int head = (int)(row % heads), b = (int)(row / heads);
-    const int pos = d_pos ? *d_pos : pos_base + b;
-    if (pos < 0 || pos >= n_ctx) return;
-    uint8_t* blk = cache + ((size_t)head * q4_blocks(n_ctx) + (pos >> 4)) * Q4<HD>::BLOCK;
-    float x[Q4<HD>::EPL];
-    load_row<HD>(((job & 1) ? v : k) + (size_t)row * HD, lane, x);
-    const Q4Scale s = q4_scale<HD>(x, lane);
-    const uint32_t codes = q4_codes<HD>(x, s);
-    if (job & 1) q4_store_row<HD, true>(blk, pos & 15, codes, s, lane);
-    else         q4_store_row<HD, false>(blk, pos & 15, codes, s, lane);
-}
-
-// ---- read back: a warp turns one row into fp16 ------------------------------------------------------------------
-// (row `pos` of `blk`; dst = K and V rows of HD fp16 values)
-template <int HD>
-__device__ __forceinline__ void q4_load_row(const uint8_t* blk, int s, uint16_t* dk, uint16_t* dv, int lane) {
+__global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(uint8_t* cache, const float* k, const float* v, int heads,
+                                                                    int n_ctx, int pos_base, int batch, const int* d_pos) {
     using F = Q4<HD>;
-    const int D = F::EPL * lane, g = D / 64;
+    constexpr int LPR = 4 * F::NG;                        // lanes of a row
+    __shared__ __align__(16) uint8_t s_blk[F::BLOCK];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int head = blockIdx.y;
+    int first = pos_base;
+    if (d_pos) {
+        first = *d_pos;
+        if (first < 0 || first >= n_ctx) return;
+    }
+    const int b = (first >> 4) + blockIdx.x;              // block of the sequence
+    const int row0 = max(first - 16 * b, 0), row1 = min(first + batch - 16 * b, 16);     // its rows that are stored
+    const bool is_v = warp >= 4;
+    const int s = (warp & 3) * 4 + lane / 8, t = lane & 3, g = (lane % 8) / 4;           // HD 64: lanes with g = 1 idle
+    const bool on = g < F::NG && s >= row0 && s < row1;
+    float x[16];
+    if (on) {
+        const float* src = (is_v ? v : k) + ((size_t)(16 * b + s - first) * heads + head) * HD + 64 * g + 8 * t;
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        const uint32_t sw = *reinterpret_cast<const uint32_t*>(blk + (which ? F::VS_OFF : F::KS_OFF) + s * F::SROWB + 4 * g);
-        const float d = __half2float(__ushort_as_half((uint16_t)sw)), m = __half2float(__ushort_as_half((uint16_t)(sw >> 16)));
-        uint16_t* dst = which ? dv : dk;
+        for (int i = 0; i < 4; ++i) {
+            const float4 q = *reinterpret_cast<const float4*>(src + 32 * (i >> 1) + 4 * (i & 1));
+            x[4 * i] = q.x; x[4 * i + 1] = q.y; x[4 * i + 2] = q.z; x[4 * i + 3] = q.w;
+        }
+    } else {
 #pragma unroll
-        for (int e = 0; e < F::EPL; e += 2) {
-            const uint32_t c = blk[which ? q4_v_byte<HD>(s, D + e) : q4_k_byte<HD>(s, D + e)];
-            *reinterpret_cast<uint32_t*>(dst + D + e) = pack_half2(q4_value(c & 15u, d, m), q4_value(c >> 4, d, m));
+        for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    }
+    float mn = x[0], mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) { mn = min_nan(mn, x[i]); mx = max_nan(mx, x[i]); }
+#pragma unroll
+    for (int off = 1; off <= 2; off <<= 1) {
+        mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, off));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    }
+    const Q4Scale sc = q4_scale_of(mn, mx);
+    const float m = __half2float(sc.m), d = __half2float(sc.d), inv = __frcp_rn(d);
+    uint32_t w[2] = {0u, 0u};
+    // code = round((x - m) / d): adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low bits.
+    // `far` is how close any of the 16 came to a border between two codes.
+    float far = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float y = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
+        const float r = y + 12582912.f;
+        far = fmaxf(far, fabsf(y - (r - 12582912.f)));
+        w[i >> 3] |= (__float_as_uint(r) & 15u) << (4 * (i & 7));
+    }
+    if (!(d > 0.f)) {
+        w[0] = w[1] = 0u;
+    } else if (far > 0.5f - 1e-5f) {
+        w[0] = w[1] = 0u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i >> 3] |= q4_code(x[i], m, d, inv) << (4 * (i & 7));
+    }
+    if (on) {
+        if (!is_v) {
+            *reinterpret_cast<uint2*>(s_blk + s * F::ROWB + (t * (HD / 32) + 2 * g) * 4) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                s_blk[q4_v_byte<HD>(s, 64 * g + 32 * (i >> 2) + 8 * t + 2 * (i & 3))] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+        }
+        if (t == 0) *reinterpret_cast<uint32_t*>(s_blk + (is_v ? F::VS_OFF : F::KS_OFF) + s * F::SROWB + 4 * g) = q4_scale_word(sc);
+    }
+    static_assert(LPR <= 8, "eight lanes per row");
+    __syncthreads();
+    uint8_t* blk = cache + ((size_t)head * q4_blocks(n_ctx) + b) * F::BLOCK;
+    if (row0 == 0 && row1 == 16) {
+        if (tid < F::BLOCK / 16) *reinterpret_cast<uint4*>(blk + 16 * tid) = *reinterpret_cast<const uint4*>(s_blk + 16 * tid);
+        return;
+    }
+    // some rows: K words and the scales word by word, V byte by byte
+    for (int i = tid; i < 4 * F::ROWB; i += kStoreThreads)
+        if (i / (F::ROWB / 4) >= row0 && i / (F::ROWB / 4) < row1) reinterpret_cast<uint32_t*>(blk)[i] = reinterpret_cast<const uint32_t*>(s_blk)[i];
+    for (int i = tid; i < 16 * F::ROWB; i += kStoreThreads) {
+        const int row = 8 * (i & 1) + 2 * ((i >> 4) & 3) + ((i >> 1) & 1);
+        if (row >= row0 && row < row1) blk[F::V_OFF + i] = s_blk[F::V_OFF + i];
+    }
+    if (tid < 2 * 16 * F::NG) {
+        const int row = tid % (16 * F::NG) / F::NG;
+        if (row >= row0 && row < row1) reinterpret_cast<uint32_t*>(blk + F::KS_OFF)[tid] = reinterpret_cast<const uint32_t*>(s_blk + F::KS_OFF)[tid];
+    }
+}
+
+// ---- read back ----------------------------------------------------------------------------------------------------
+// One warp turns rows [row0, row1) of a block into fp16; dk, dv: where row 0 of the block would go.  K: a lane takes the four
+// (two) code words of place t of a row, 16 bytes, and writes 16-byte pieces, four lanes 64 bytes.  V: a word holds a pair of
+// dims of four rows, so the block passes through shared memory (`s_v`, kVStride bytes a row: the lanes' 4-byte stores
+// then fall into 32 different banks).
+template <int HD>
+constexpr int kVStride = HD * 2 + 16;
+
+template <int HD>
+__device__ __forceinline__ uint4 q4_eight(uint32_t w, float d, float m) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = q4_value((w >> (4 * e)) & 15u, d, m);
+    return make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+}
+
+template <int HD>
+__device__ __forceinline__ void q4_load_block(const uint8_t* blk, __half* dk, __half* dv, int row0, int row1, uint8_t* s_v, int lane) {
+    using F = Q4<HD>;
+    constexpr int NW = HD / 32, NG = F::NG;
+    const int r = lane >> 2, t = lane & 3;
+    uint32_t kw[2][NW], vw[NG][4], ks[2][NG], vs[4][NG];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint8_t* at = blk + (8 * j + r) * F::ROWB + t * (F::ROWB / 4);
+        if constexpr (NW == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(at);
+            kw[j][0] = v.x; kw[j][1] = v.y; kw[j][2] = v.z; kw[j][3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(at);
+            kw[j][0] = v.x; kw[j][1] = v.y;
         }
     }
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+        const uint4 v = *reinterpret_cast<const uint4*>(blk + F::V_OFF + 512 * q + 16 * lane);
+        vw[q][0] = v.x; vw[q][1] = v.y; vw[q][2] = v.z; vw[q][3] = v.w;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) ks[j][g] = *reinterpret_cast<const uint32_t*>(blk + F::KS_OFF + (8 * j + r) * F::SROWB + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)      // byte i of a word: row 2t, 2t + 8, 2t + 1, 2t + 9
+            vs[i][g] = *reinterpret_cast<const uint32_t*>(blk + F::VS_OFF + (2 * t + 8 * (i & 1) + (i >> 1)) * F::SROWB + 4 * g);
+    }
+    auto dm = [](uint32_t w, float& d, float& m) {
+        d = __half2float(__ushort_as_half((uint16_t)w));
+        m = __half2float(__ushort_as_half((uint16_t)(w >> 16)));
+    };
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int row = 8 * j + r;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            float d, m;
+            dm(ks[j][i >> 1], d, m);
+            const uint4 v = q4_eight<HD>(kw[j][i], d, m);
+            if (row >= row0 && row < row1) *reinterpret_cast<uint4*>(dk + (size_t)row * HD + 32 * i + 8 * t) = v;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 2 * t + 8 * (i & 1) + (i >> 1);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            float d, m;
+            dm(vs[i][g], d, m);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t c = vw[g][j] >> (8 * i);
+                *reinterpret_cast<uint32_t*>(s_v + row * kVStride<HD> + 32 * (4 * g + j) + 4 * r) =
+                    pack_half2(q4_value(c & 15u, d, m), q4_value((c >> 4) & 15u, d, m));
+            }
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) {
+        const int c = lane + 32 * i, row = c / (HD / 8), col = c % (HD / 8);
+        const uint4 v = *reinterpret_cast<const uint4*>(s_v + row * kVStride<HD> + 16 * col);
+        if (row >= row0 && row < row1) *reinterpret_cast<uint4*>(dv + (size_t)row * HD + 8 * col) = v;
+    }
+    __syncwarp();
 }
 
 constexpr int kLoadWarps = 8;
@@ -61,55 +199,120 @@ constexpr int kLoadWarps = 8;
 template <int HD>
 __global__ void __launch_bounds__(32 * kLoadWarps) kv_load_q4_kernel(const uint8_t* cache, uint16_t* kc, uint16_t* vc, int heads,
                                                                      int n_ctx, int row_base, int rows, int dst_ctx, int dst_base) {
-    const long long job = (long long)blockIdx.x * kLoadWarps + (threadIdx.x >> 5);
-    if (job >= (long long)heads * rows) return;
-    const int head = (int)(job / rows), i = (int)(job % rows);
-    const int pos = row_base + i;
-    const uint8_t* blk = cache + ((size_t)head * q4_blocks(n_ctx) + (pos >> 4)) * Q4<HD>::BLOCK;
-    const size_t dst = ((size_t)head * dst_ctx + dst_base + i) * HD;
-    q4_load_row<HD>(blk, pos & 15, kc + dst, vc + dst, threadIdx.x & 31);
+    __shared__ __align__(16) uint8_t s_v[kLoadWarps][16 * kVStride<HD>];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b0 = row_base >> 4, nb = ((row_base + rows - 1) >> 4) - b0 + 1;
+    const long long job = (long long)blockIdx.x * kLoadWarps + warp;
+    if (job >= (long long)heads * nb) return;
+    const int head = (int)(job / nb), b = b0 + (int)(job % nb);
+    const uint8_t* blk = cache + ((size_t)head * q4_blocks(n_ctx) + b) * Q4<HD>::BLOCK;
+    // row 0 of the block; may lie in front of the destination, whose rows outside [row0, row1) are not touched
+    const long long at = ((long long)head * dst_ctx + dst_base + 16 * b - row_base) * HD;
+    q4_load_block<HD>(blk, reinterpret_cast<__half*>(kc) + at, reinterpret_cast<__half*>(vc) + at, max(row_base - 16 * b, 0),
+                      min(row_base + rows - 16 * b, 16), s_v[warp], lane);
 }
 
-// ---- roll: one CTA per (layer, kv head) -------------------------------------------------------------------------
-// Row r becomes row r + shift for n_keep <= r < n_ctx - shift, the last `shift` rows become zero.  A step composes
-// kShiftBlocks blocks in shared memory from the rows `shift` further on and then writes them; what later steps read lies
-// behind everything written so far, so one CTA can work in place.
-constexpr int kShiftThreads = 256;
-constexpr int kShiftBlocks = 8;
+// ---- roll -----------------------------------------------------------------------------------------------------------
+// Row r becomes row r + shift for n_keep <= r < n_ctx - shift, the last `shift` rows become zero.  One CTA per (layer, kv head)
+// and tensor: the codes and the scales of K or of V.  It walks the blocks in order; a step brings the blocks that hold
+// the source rows of kShiftBlocks blocks to shared memory and writes those blocks from there.  Sources lie at or behind the
+// place they go to, and those of later steps behind everything a step writes, so the copies of the next steps run
+// while this one writes.
+constexpr int kShiftThreads = 512;
+constexpr int kShiftBlocks = 16;
+constexpr int kShiftWindows = 4;           // steps in flight, this one among them
 
 template <int HD>
 __global__ void __launch_bounds__(kShiftThreads) kv_shift_q4_kernel(uint8_t* cache, int n_ctx, int n_keep, int shift) {
     using F = Q4<HD>;
-    extern __shared__ __align__(16) uint8_t smem[];       // kShiftBlocks composed blocks
+    constexpr int CODES = 16 * F::ROWB, SCALES = 16 * F::SROWB, PART = CODES + SCALES;
+    constexpr int WINDOW = (kShiftBlocks + 1) * PART;
+    extern __shared__ __align__(16) uint8_t smem[];       // kShiftWindows windows
+    const bool is_v = blockIdx.x != 0;
+    const int tid = threadIdx.x;
     const int nblk = q4_blocks(n_ctx);
-    uint8_t* base = cache + (size_t)blockIdx.x * nblk * F::BLOCK;
-    for (int b0 = n_keep >> 4; b0 < nblk; b0 += kShiftBlocks) {
-        const int nb = min(kShiftBlocks, nblk - b0);
-        // one warp per row
-        for (int i = threadIdx.x >> 5; i < nb * 16; i += kShiftThreads / 32) {
-            const int lane = threadIdx.x & 31;
-            const int row = b0 * 16 + i;
-            int src = row < n_keep || row >= n_ctx ? row : row + shift;
-            const bool zero = row < n_ctx && src >= n_ctx;
-            if (zero) src = row;
-            const uint8_t* sb = base + (size_t)(src >> 4) * F::BLOCK;
-            uint8_t* db = smem + (size_t)(i >> 4) * F::BLOCK;
-            const int ss = src & 15, ds = i & 15;
-            for (int D = 2 * lane; D < HD; D += 64) {
-                db[q4_k_byte<HD>(ds, D)] = zero ? (uint8_t)0 : sb[q4_k_byte<HD>(ss, D)];
-                db[q4_v_byte<HD>(ds, D)] = zero ? (uint8_t)0 : sb[q4_v_byte<HD>(ss, D)];
-            }
-            if (lane < 2 * F::NG) {
-                const int off = (lane >= F::NG ? F::VS_OFF : F::KS_OFF), g = lane % F::NG;
-                *reinterpret_cast<uint32_t*>(db + off + ds * F::SROWB + 4 * g) =
-                    zero ? 0u : *reinterpret_cast<const uint32_t*>(sb + off + ss * F::SROWB + 4 * g);
-            }
+    uint8_t* base = cache + (size_t)blockIdx.y * nblk * F::BLOCK;
+    const int c_off = is_v ? F::V_OFF : 0, s_off = is_v ? F::VS_OFF : F::KS_OFF;
+    const int first = n_keep >> 4;
+    const int last = n_ctx - shift;                       // first row that becomes zero
+
+    auto load = [&](int step) {
+        const int b0 = first + step * kShiftBlocks + (shift >> 4);
+        const uint32_t dst = smem_u32(smem + (step % kShiftWindows) * WINDOW);
+        for (int i = tid; i < (kShiftBlocks + 1) * (PART / 16); i += kShiftThreads) {
+            const int b = b0 + i / (PART / 16), c = i % (PART / 16);
+            if (b >= nblk) break;
+            const uint8_t* src = base + (size_t)b * F::BLOCK + (c < CODES / 16 ? c_off + 16 * c : s_off + 16 * c - CODES);
+            cp_async_16(dst + 16 * i, src, 16);
         }
-        __syncthreads();
-        uint4* dst = reinterpret_cast<uint4*>(base + (size_t)b0 * F::BLOCK);
-        const uint4* from = reinterpret_cast<const uint4*>(smem);
-        for (int i = threadIdx.x; i < nb * F::BLOCK / 16; i += kShiftThreads) dst[i] = from[i];
-        __syncthreads();
+        cp_async_commit();
+    };
+    const int steps = (nblk - first + kShiftBlocks - 1) / kShiftBlocks;
+#pragma unroll
+    for (int step = 0; step < kShiftWindows - 1; ++step) {
+        if (step < steps) load(step); else cp_async_commit();
+    }
+    for (int step = 0; step < steps; ++step) {
+        cp_async_wait<kShiftWindows - 2>();
+        __syncthreads();                                  // this step's window has landed, the one before is free
+        if (step + kShiftWindows - 1 < steps) load(step + kShiftWindows - 1); else cp_async_commit();
+        const int b0 = first + step * kShiftBlocks, nb = min(kShiftBlocks, nblk - b0);
+        const uint8_t* win = smem + (step % kShiftWindows) * WINDOW;
+        const int skip = shift & 15;                      // row i of the step lies at row i + skip of the window
+        auto src_byte = [&](int i) { return win + ((i + skip) >> 4) * PART; };
+        for (int idx = tid; idx < nb * (PART / 16); idx += kShiftThreads) {
+            const int bl = idx / (PART / 16), c = idx % (PART / 16);
+            const int row_b = (b0 + bl) * 16;             // first row of the block
+            uint32_t w[4];
+            bool whole = row_b >= n_keep && row_b + 16 <= n_ctx;
+            uint8_t* dst = base + (size_t)(b0 + bl) * F::BLOCK;
+            if (c >= CODES / 16) {
+                // scales: four words, one (row, group) each
+                dst += s_off + 16 * c - CODES;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int word = 4 * (c - CODES / 16) + k, i = 16 * bl + word / F::NG;
+                    w[k] = b0 * 16 + i < last ? *reinterpret_cast<const uint32_t*>(src_byte(i) + CODES + ((i + skip) & 15) * F::SROWB + 4 * (word % F::NG)) : 0u;
+                    if (!whole) {
+                        const int row = b0 * 16 + i;
+                        if (row >= n_keep && row < n_ctx) reinterpret_cast<uint32_t*>(dst)[k] = w[k];
+                    }
+                }
+            } else if (!is_v) {
+                // K codes: 16 bytes of one row
+                dst += c_off + 16 * c;
+                const int i = 16 * bl + 16 * c / F::ROWB, row = b0 * 16 + i;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (row < last) v = *reinterpret_cast<const uint4*>(src_byte(i) + ((i + skip) & 15) * F::ROWB + 16 * c % F::ROWB);
+                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+                if (!whole && row >= n_keep && row < n_ctx) *reinterpret_cast<uint4*>(dst) = v;
+            } else {
+                // V codes: four words of the rows 2t, 2t + 8, 2t + 1, 2t + 9
+                dst += c_off + 16 * c;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = 0u;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 16 * bl + 2 * (c & 3) + 8 * (e & 1) + (e >> 1), row = b0 * 16 + i;
+                    const int ss = (i + skip) & 15;
+                    // the same pair of dims of the source row: place t of the row, and its byte
+                    const uint8_t* from = src_byte(i) + (c >> 5) * 512 + (((c & 31) & ~3) + ((ss & 7) >> 1)) * 16;
+                    const uint32_t sel = 8 * (2 * (ss & 1) + (ss >> 3));
+                    if (row < last) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(from);
+                        w[0] |= ((v.x >> sel) & 255u) << (8 * e);
+                        w[1] |= ((v.y >> sel) & 255u) << (8 * e);
+                        w[2] |= ((v.z >> sel) & 255u) << (8 * e);
+                        w[3] |= ((v.w >> sel) & 255u) << (8 * e);
+                    }
+                    if (!whole && row >= n_keep && row < n_ctx) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) dst[4 * k + e] = (uint8_t)(w[k] >> (8 * e));
+                    }
+                }
+            }
+            if (whole) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
     }
 }
 
@@ -128,20 +331,19 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
     const int nblk = q4_blocks(p.cache_ctx);
     const bool rope_q = (a.fuse & 1) != 0, rope_k = (a.fuse & 2) != 0, append = (a.fuse & 4) != 0;
     pdl_trigger();
+    __shared__ __align__(16) uint8_t s_v[kPrologueThreads / 32][16 * kVStride<HD>];
     if ((int)blockIdx.x >= a.batch) {
         pdl_wait();
-        const int expand = append ? a.n_past : rows;
+        const int expand = append ? a.n_past : rows, nb = q4_blocks(expand);
         const long long job = (long long)(blockIdx.x - a.batch) * (kPrologueThreads / 32) + warp;
-        if (job >= (long long)a.n_kv * expand) return;
-        const int head = (int)(job / expand), pos = (int)(job % expand);
-        const uint8_t* blk = p.cache + ((size_t)head * nblk + (pos >> 4)) * F::BLOCK;
-        const size_t dst = ((size_t)head * rows + pos) * HD;
-        q4_load_row<HD>(blk, pos & 15, reinterpret_cast<uint16_t*>(p.k16) + dst, reinterpret_cast<uint16_t*>(p.v16) + dst, lane);
+        if (job >= (long long)a.n_kv * nb) return;
+        const int head = (int)(job / nb), b = (int)(job % nb);
+        const size_t dst = ((size_t)head * rows + 16 * b) * HD;
+        q4_load_block<HD>(p.cache + ((size_t)head * nblk + b) * F::BLOCK, p.k16 + dst, p.v16 + dst, 0, min(expand - 16 * b, 16), s_v[warp], lane);
         return;
     }
     // cos and sin in double: a key's code is a decision at a border, so the rotated key is rounded to fp32 once
     __shared__ double s_cos[HD / 2], s_sin[HD / 2];
-    __shared__ float s_row[kPrologueThreads / 32][HD];
     const int b = blockIdx.x, pos = a.n_past + b;
     if (rope_q || rope_k) {
         for (int i = tid; i < a.rope.n_rot / 2; i += kPrologueThreads) {
@@ -155,7 +357,7 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
     if (b == 0 && tid == 0 && a.status) *a.status = 0;
     const float qs = a.scale * LOG2E;
     const int jobs = a.n_head + (append ? 2 * a.n_kv : 0);
-    float* row = s_row[warp];
+    float* row = reinterpret_cast<float*>(s_v[warp]);
     for (int job = warp; job < jobs; job += kPrologueThreads / 32) {
         const int kind = job < a.n_head ? 0 : (job < a.n_head + a.n_kv ? 1 : 2);
         const int head = kind == 0 ? job : (kind == 1 ? job - a.n_head : job - a.n_head - a.n_kv);
@@ -200,6 +402,8 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
     }
 }
 
+constexpr int shift_smem(int head_dim) { return kShiftWindows * (kShiftBlocks + 1) * 9 * head_dim; }
+
 } // namespace
 
 void rope_freq_table(const RopeArgs& r, float (&freq)[64]) {
@@ -225,19 +429,24 @@ void rope_freq_table(const RopeArgs& r, float (&freq)[64]) {
     for (int i = 0; i < 64; ++i) freq[i] = e->freq[i];
 }
 
+cudaError_t kv_q4_set_attributes() {
+    cudaError_t e = cudaFuncSetAttribute(kv_shift_q4_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, shift_smem(128));
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(kv_shift_q4_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, shift_smem(64));
+}
+
 cudaError_t launch_kv_store_q4(uint8_t* cache, const float* k, const float* v, int heads, int head_dim, int n_ctx, int pos_base,
                                int batch, const int* d_pos, cudaStream_t stream, unsigned long long* launches) {
-    const long long jobs = 2LL * batch * heads;
-    const dim3 grid((unsigned)((jobs + kStoreWarps - 1) / kStoreWarps));
-    if (head_dim == 128) kv_store_q4_kernel<128><<<grid, 32 * kStoreWarps, 0, stream>>>(cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
-    else                 kv_store_q4_kernel<64><<<grid, 32 * kStoreWarps, 0, stream>>>(cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
+    const dim3 grid(d_pos ? 1 : ((pos_base + batch - 1) >> 4) - (pos_base >> 4) + 1, heads);
+    if (head_dim == 128) kv_store_q4_kernel<128><<<grid, kStoreThreads, 0, stream>>>(cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
+    else                 kv_store_q4_kernel<64><<<grid, kStoreThreads, 0, stream>>>(cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
     if (launches) *launches += 1;
     return cudaGetLastError();
 }
 
 cudaError_t launch_kv_load_q4(const uint8_t* cache, uint16_t* kc, uint16_t* vc, int heads, int head_dim, int n_ctx, int row_base,
                               int rows, int dst_ctx, int dst_base, cudaStream_t stream, unsigned long long* launches) {
-    const long long jobs = (long long)heads * rows;
+    const long long jobs = (long long)heads * (((row_base + rows - 1) >> 4) - (row_base >> 4) + 1);
     const dim3 grid((unsigned)((jobs + kLoadWarps - 1) / kLoadWarps));
     if (head_dim == 128) kv_load_q4_kernel<128><<<grid, 32 * kLoadWarps, 0, stream>>>(cache, kc, vc, heads, n_ctx, row_base, rows, dst_ctx, dst_base);
     else                 kv_load_q4_kernel<64><<<grid, 32 * kLoadWarps, 0, stream>>>(cache, kc, vc, heads, n_ctx, row_base, rows, dst_ctx, dst_base);
@@ -247,16 +456,16 @@ cudaError_t launch_kv_load_q4(const uint8_t* cache, uint16_t* kc, uint16_t* vc, 
 
 cudaError_t launch_kv_shift_q4(uint8_t* cache, int n_layer, int n_kv, int head_dim, int n_ctx, int n_keep, int shift,
                                cudaStream_t stream, unsigned long long* launches) {
-    const int grid = n_layer * n_kv;
-    if (head_dim == 128) kv_shift_q4_kernel<128><<<grid, kShiftThreads, kShiftBlocks * Q4<128>::BLOCK, stream>>>(cache, n_ctx, n_keep, shift);
-    else                 kv_shift_q4_kernel<64><<<grid, kShiftThreads, kShiftBlocks * Q4<64>::BLOCK, stream>>>(cache, n_ctx, n_keep, shift);
+    const dim3 grid(2, n_layer * n_kv);
+    if (head_dim == 128) kv_shift_q4_kernel<128><<<grid, kShiftThreads, shift_smem(128), stream>>>(cache, n_ctx, n_keep, shift);
+    else                 kv_shift_q4_kernel<64><<<grid, kShiftThreads, shift_smem(64), stream>>>(cache, n_ctx, n_keep, shift);
     if (launches) *launches += 1;
     return cudaGetLastError();
 }
 
 cudaError_t launch_prefill_q4_prologue(const KvQ4PrologueArgs& p, cudaStream_t stream, unsigned long long* launches) {
     const PrefillArgs& a = p.a;
-    const long long jobs = (long long)a.n_kv * ((a.fuse & 4) ? a.n_past : a.n_past + a.batch);
+    const long long jobs = (long long)a.n_kv * q4_blocks((a.fuse & 4) ? a.n_past : a.n_past + a.batch);
     constexpr int W = kPrologueThreads / 32;
     const dim3 grid((unsigned)(a.batch + (jobs + W - 1) / W));
     const cudaError_t e = a.head_dim == 128 ? launch_dependent(prefill_q4_prologue_kernel<128>, grid, kPrologueThreads, 0, stream, 1, p)

@@ -51,9 +51,23 @@ __device__ __forceinline__ int q4_v_byte(int s, int D) {
 
 struct Q4Scale { __half d, m; };
 
+// (d, m) of a group with this minimum and maximum (NaN or infinite where the group has such a value).  The quotient is
+// formed in double and rounded to fp16 in one step; in fp32 one group in a few thousand would get a step that is off by an
+// fp16 ulp.
+__device__ __forceinline__ Q4Scale q4_scale_of(float mn, float mx) {
+    Q4Scale s;
+    s.m = __float2half_rn(mn);
+    if (!(fabsf(mx) <= 3.402823466e38f) || !(fabsf(__half2float(s.m)) <= 65504.f)) {
+        s.d = s.m = __ushort_as_half(0x7fff);
+        return s;
+    }
+    const double step = ((double)mx - (double)__half2float(s.m)) / 15.0;
+    s.d = __double2half(step > 0.0 ? step : 0.0);
+    return s;
+}
+
 // (d, m) of the group whose EPL-value shares lie in the lanes of `x`: lanes of the same half warp (HD = 128) or of the whole
-// warp (HD = 64) hold one group.  Called by full warps.  The quotient is formed in double and rounded to fp16 in one step;
-// in fp32 one group in a few thousand would get a step that is off by an fp16 ulp.
+// warp (HD = 64) hold one group.  Called by full warps.
 template <int HD>
 __device__ __forceinline__ Q4Scale q4_scale(const float (&x)[Q4<HD>::EPL], int lane) {
     constexpr int W = 32 / Q4<HD>::NG;                    // lanes of a group
@@ -71,15 +85,7 @@ __device__ __forceinline__ Q4Scale q4_scale(const float (&x)[Q4<HD>::EPL], int l
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
     }
     const unsigned mask = __ballot_sync(0xffffffffu, bad) & (W == 32 ? 0xffffffffu : (0xffffu << (lane & 16)));
-    Q4Scale s;
-    s.m = __float2half_rn(mn);
-    if (mask || __hisinf(s.m)) {
-        s.d = s.m = __ushort_as_half(0x7fff);
-        return s;
-    }
-    const double step = ((double)mx - (double)__half2float(s.m)) / 15.0;
-    s.d = __double2half(step > 0.0 ? step : 0.0);
-    return s;
+    return q4_scale_of(mask ? CUDART_NAN_F : mn, mx);
 }
 
 // code of x.  The fp32 quotient is off by less than 4e-6 where it is below 16; only next to a border between two codes
@@ -140,6 +146,7 @@ struct KvQ4PrologueArgs {
     float freq[64];            // see rope_freq_table
 };
 
+cudaError_t kv_q4_set_attributes();
 cudaError_t launch_kv_store_q4(uint8_t* cache, const float* k, const float* v, int heads, int head_dim, int n_ctx, int pos_base,
                                int batch, const int* d_pos, cudaStream_t stream, unsigned long long* launches);
 cudaError_t launch_kv_load_q4(const uint8_t* cache, uint16_t* kc, uint16_t* vc, int heads, int head_dim, int n_ctx, int row_base,
