@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "liborin_attn_b200.so")
 SOURCES = ["capi.cu", "decode.cu", "decode_q4.cu", "kv_q4.cu", "prefill_mma.cu", "prefill_tc.cu", "rope_kv.cu"]
-HEADERS = ["common.cuh", "attn_internal.h", "decode_merge.cuh", "kv_q4.cuh", os.path.join("..", "..", "include", "orin_attn_b200.h")]
+HEADERS = ["common.cuh", "attn_internal.h", "decode_merge.cuh", "f32x2.cuh", "kv_q4.cuh", os.path.join("..", "..", "include", "orin_attn_b200.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",

@@ -514,7 +514,7 @@ int oattn_kv_store_q4(void* cache, const float* k, const float* v, int heads, in
     const int rc = check_q4(cache, heads, head_dim, n_ctx);
     if (rc != OATTN_OK) return rc;
     if (!k || !v || batch <= 0) return OATTN_ERR_ARG;
-    if (heads > 65535) return OATTN_ERR_UNSUPPORTED;                   // one grid row per head
+    if ((long long)heads * (batch / 16 + 2) > 0x7fffffffLL) return OATTN_ERR_UNSUPPORTED;    // one CTA per head and 16 rows
     if (((uintptr_t)k | (uintptr_t)v) & 15) return OATTN_ERR_ARG;      // read as float4
     if (d_pos && batch != 1) return OATTN_ERR_ARG;
     if (!d_pos && (pos_base < 0 || pos_base > n_ctx - batch)) return OATTN_ERR_ARG;

@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "decode_merge.cuh"
+#include "f32x2.cuh"
 #include "kv_q4.cuh"
 
 namespace oattn {
@@ -62,18 +63,6 @@ __device__ __forceinline__ Q4Plan q4_plan(int npos, int n_splits) {
     s.active = (s.blocks + s.per_split - 1) / s.per_split;
     return s;
 }
-
-// Pairs of fp32 in one 64-bit register: two-wide add, multiply and fma, each half rounded as the scalar instruction would.
-struct F2 {
-    unsigned long long v;
-    __device__ __forceinline__ F2() {}
-    __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(x), "f"(y)); }
-    __device__ __forceinline__ float x() const { float a, b; asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); return a; }
-    __device__ __forceinline__ float y() const { float a, b; asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); return b; }
-};
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
 
 __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)w)); }
 __device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)(w >> 16))); }

@@ -3,11 +3,22 @@
 
 #include <mutex>
 
+#include "f32x2.cuh"
 #include "kv_q4.cuh"
 
 namespace oattn {
 
 namespace {
+
+// The careful form of a lane's 16 codes, out of line and from the row itself: hardly ever taken.
+__device__ __noinline__ uint2 q4_codes16(const float* src, float m, float d, float inv) {
+    uint2 w = make_uint2(0u, 0u);
+    for (int i = 0; i < 8; ++i) {
+        w.x |= q4_code(src[i], m, d, inv) << (4 * i);
+        w.y |= q4_code(src[32 + i], m, d, inv) << (4 * i);
+    }
+    return w;
+}
 
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
@@ -21,26 +32,26 @@ __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.N
 constexpr int kStoreThreads = 256;
 
 template <int HD>
-__global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(uint8_t* cache, const float* k, const float* v, int heads,
+__global__ void __launch_bounds__(kStoreThreads, 5) kv_store_q4_kernel(uint8_t* cache, const float* k, const float* v, int heads,
                                                                     int n_ctx, int pos_base, int batch, const int* d_pos) {
     using F = Q4<HD>;
     constexpr int LPR = 4 * F::NG;                        // lanes of a row
     __shared__ __align__(16) uint8_t s_blk[F::BLOCK];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int head = blockIdx.y;
+    const int head = blockIdx.x % heads;                  // the heads of a token lie next to each other in k and v
     int first = pos_base;
     if (d_pos) {
         first = *d_pos;
         if (first < 0 || first >= n_ctx) return;
     }
-    const int b = (first >> 4) + blockIdx.x;              // block of the sequence
+    const int b = (first >> 4) + blockIdx.x / heads;      // block of the sequence
     const int row0 = max(first - 16 * b, 0), row1 = min(first + batch - 16 * b, 16);     // its rows that are stored
     const bool is_v = warp >= 4;
     const int s = (warp & 3) * 4 + lane / 8, t = lane & 3, g = (lane % 8) / 4;           // HD 64: lanes with g = 1 idle
     const bool on = g < F::NG && s >= row0 && s < row1;
+    const float* src = (is_v ? v : k) + ((long long)(16 * b + s - first) * heads + head) * HD + 64 * g + 8 * t;
     float x[16];
     if (on) {
-        const float* src = (is_v ? v : k) + ((size_t)(16 * b + s - first) * heads + head) * HD + 64 * g + 8 * t;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float4 q = *reinterpret_cast<const float4*>(src + 32 * (i >> 1) + 4 * (i & 1));
@@ -61,22 +72,26 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_q4_kernel(uint8_t* cac
     const Q4Scale sc = q4_scale_of(mn, mx);
     const float m = __half2float(sc.m), d = __half2float(sc.d), inv = __frcp_rn(d);
     uint32_t w[2] = {0u, 0u};
-    // code = round((x - m) / d): adding 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low bits.
-    // `far` is how close any of the 16 came to a border between two codes.
+    // code = round((x - m) / d): adding 1.5 * 2^23 rounds to an integer, ties to even.  `far`: how close any of the 16 came to a
+    // border between two codes.  Four codes are put together in fp32, 16 bits of an integer.
     float far = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float y = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
-        const float r = y + 12582912.f;
-        far = fmaxf(far, fabsf(y - (r - 12582912.f)));
-        w[i >> 3] |= (__float_as_uint(r) & 15u) << (4 * (i & 7));
+    for (int i = 0; i < 16; i += 4) {
+        const F2 lo(x[i], x[i + 1]), hi(x[i + 2], x[i + 3]), mm(-m, -m), ii(inv, inv), up(12582912.f, 12582912.f), down(-12582912.f, -12582912.f);
+        const F2 y0 = (lo + mm) * ii, y1 = (hi + mm) * ii;
+        const F2 c0 = (y0 + up) + down, c1 = (y1 + up) + down;
+        const F2 e0 = fma2(c0, F2(-1.f, -1.f), y0), e1 = fma2(c1, F2(-1.f, -1.f), y1);
+        far = fmaxf(far, fmaxf(fmaxf(fabsf(e0.x()), fabsf(e0.y())), fmaxf(fabsf(e1.x()), fabsf(e1.y()))));
+        const float four = fmaf(fmaf(fmaf(c1.y(), 16.f, c1.x()), 16.f, c0.y()), 16.f, c0.x());
+        w[i >> 3] |= (__float_as_uint(four + 8388608.f) & 0xffffu) << (4 * (i & 4));
     }
     if (!(d > 0.f)) {
         w[0] = w[1] = 0u;
-    } else if (far > 0.5f - 1e-5f) {
-        w[0] = w[1] = 0u;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[i >> 3] |= q4_code(x[i], m, d, inv) << (4 * (i & 7));
+    } else if (on && (far > 0.5f - 1e-5f || (mn - m) * inv < -0.25f || (mx - m) * inv > 15.25f)) {
+        // next to a border, or a group whose offset is coarse against its step, so that codes have to be clamped
+        const uint2 c = q4_codes16(src, m, d, inv);
+        w[0] = c.x;
+        w[1] = c.y;
     }
     if (on) {
         if (!is_v) {
@@ -213,40 +228,64 @@ __global__ void __launch_bounds__(32 * kLoadWarps) kv_load_q4_kernel(const uint8
 }
 
 // ---- roll -----------------------------------------------------------------------------------------------------------
-// Row r becomes row r + shift for n_keep <= r < n_ctx - shift, the last `shift` rows become zero.  One CTA per (layer, kv head)
-// and tensor: the codes and the scales of K or of V.  It walks the blocks in order; a step brings the blocks that hold
-// the source rows of kShiftBlocks blocks to shared memory and writes those blocks from there.  Sources lie at or behind the
-// place they go to, and those of later steps behind everything a step writes, so the copies of the next steps run
-// while this one writes.
-constexpr int kShiftThreads = 512;
+// Row r becomes row r + shift for n_keep <= r < n_ctx - shift, the last `shift` rows become zero.  One CTA per (layer, kv head),
+// tensor and 64 dims' worth of its bytes: 32 bytes of every K row, or 512 consecutive bytes of V codes, and one group's
+// scales.  It walks the blocks in order; a step brings the blocks that hold the source rows of kShiftBlocks blocks to
+// shared memory and writes those blocks from there.  Sources lie at or behind the place they go to, and those of later
+// steps behind everything a step writes, so the copies of the next steps run while this one writes.
+constexpr int kShiftThreads = 256;
 constexpr int kShiftBlocks = 16;
 constexpr int kShiftWindows = 4;           // steps in flight, this one among them
 
 template <int HD>
+struct ShiftWindow {
+    static constexpr int CODES = 512, SCALES = 16 * Q4<HD>::SROWB, PART = CODES + SCALES;
+    static constexpr int BYTES = (kShiftBlocks + 1) * PART;
+};
+
+constexpr int shift_smem(int head_dim) { return kShiftWindows * (head_dim == 128 ? ShiftWindow<128>::BYTES : ShiftWindow<64>::BYTES); }
+
+template <int HD>
 __global__ void __launch_bounds__(kShiftThreads) kv_shift_q4_kernel(uint8_t* cache, int n_ctx, int n_keep, int shift) {
     using F = Q4<HD>;
-    constexpr int CODES = 16 * F::ROWB, SCALES = 16 * F::SROWB, PART = CODES + SCALES;
-    constexpr int WINDOW = (kShiftBlocks + 1) * PART;
+    using W = ShiftWindow<HD>;
     extern __shared__ __align__(16) uint8_t smem[];       // kShiftWindows windows
-    const bool is_v = blockIdx.x != 0;
-    const int tid = threadIdx.x;
+    const bool is_v = blockIdx.x >= F::NG;
+    const int h = blockIdx.x % F::NG;                      // which 32 bytes of a K row, which 512 of V; group of the scales
+    const int warp = threadIdx.x >> 5, c = threadIdx.x & 31;
     const int nblk = q4_blocks(n_ctx);
     uint8_t* base = cache + (size_t)blockIdx.y * nblk * F::BLOCK;
-    const int c_off = is_v ? F::V_OFF : 0, s_off = is_v ? F::VS_OFF : F::KS_OFF;
     const int first = n_keep >> 4;
     const int last = n_ctx - shift;                       // first row that becomes zero
+    const int skip = shift & 15;                          // row i of a step lies at row i + skip of its window
+    // A warp takes a block, lane c the 16-byte piece c of its codes (two pieces per K row) and row c's scale word
+    const int piece = is_v ? F::V_OFF + 512 * h + 16 * c : (c >> 1) * F::ROWB + 32 * h + 16 * (c & 1);
+    const int s_off = is_v ? F::VS_OFF : F::KS_OFF;
 
     auto load = [&](int step) {
         const int b0 = first + step * kShiftBlocks + (shift >> 4);
-        const uint32_t dst = smem_u32(smem + (step % kShiftWindows) * WINDOW);
-        for (int i = tid; i < (kShiftBlocks + 1) * (PART / 16); i += kShiftThreads) {
-            const int b = b0 + i / (PART / 16), c = i % (PART / 16);
-            if (b >= nblk) break;
-            const uint8_t* src = base + (size_t)b * F::BLOCK + (c < CODES / 16 ? c_off + 16 * c : s_off + 16 * c - CODES);
-            cp_async_16(dst + 16 * i, src, 16);
+        const uint32_t dst = smem_u32(smem + (step % kShiftWindows) * W::BYTES) + 16 * c;
+        for (int i = warp; i < kShiftBlocks + 1; i += kShiftThreads / 32) {
+            if (b0 + i >= nblk) break;
+            const uint8_t* blk = base + (size_t)(b0 + i) * F::BLOCK;
+            cp_async_16(dst + i * W::PART, blk + piece, 16);
+            if (c < W::SCALES / 16) cp_async_16(dst + i * W::PART + W::CODES, blk + s_off + 16 * c, 16);
         }
         cp_async_commit();
     };
+    // Where the lane's bytes come from, relative to the window's block: K one piece, V the words of place t of the four source
+    // rows 2t, 2t + 8, 2t + 1, 2t + 9 (t = c % 4) and which byte of them; the scale word.
+    int from[4];
+    uint32_t sel[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int i = 2 * (c & 3) + 8 * (e & 1) + (e >> 1) + skip, ss = i & 15;
+        from[e] = (i >> 4) * W::PART + ((c & ~3) + ((ss & 7) >> 1)) * 16;
+        sel[e] = (uint32_t)(4 + 2 * (ss & 1) + (ss >> 3)) << (4 * e) | (0x3210u & ~(0xfu << (4 * e)));
+    }
+    const int k_from = (((c >> 1) + skip) >> 4) * W::PART + (((c >> 1) + skip) & 15) * 32 + 16 * (c & 1);
+    const int sc_from = (((c & 15) + skip) >> 4) * W::PART + W::CODES + (((c & 15) + skip) & 15) * F::SROWB + 4 * h;
+
     const int steps = (nblk - first + kShiftBlocks - 1) / kShiftBlocks;
 #pragma unroll
     for (int step = 0; step < kShiftWindows - 1; ++step) {
@@ -257,61 +296,55 @@ __global__ void __launch_bounds__(kShiftThreads) kv_shift_q4_kernel(uint8_t* cac
         __syncthreads();                                  // this step's window has landed, the one before is free
         if (step + kShiftWindows - 1 < steps) load(step + kShiftWindows - 1); else cp_async_commit();
         const int b0 = first + step * kShiftBlocks, nb = min(kShiftBlocks, nblk - b0);
-        const uint8_t* win = smem + (step % kShiftWindows) * WINDOW;
-        const int skip = shift & 15;                      // row i of the step lies at row i + skip of the window
-        auto src_byte = [&](int i) { return win + ((i + skip) >> 4) * PART; };
-        for (int idx = tid; idx < nb * (PART / 16); idx += kShiftThreads) {
-            const int bl = idx / (PART / 16), c = idx % (PART / 16);
+        for (int bl = warp; bl < nb; bl += kShiftThreads / 32) {
+            const uint8_t* win = smem + (step % kShiftWindows) * W::BYTES + bl * W::PART;
+            uint8_t* blk = base + (size_t)(b0 + bl) * F::BLOCK;
             const int row_b = (b0 + bl) * 16;             // first row of the block
-            uint32_t w[4];
-            bool whole = row_b >= n_keep && row_b + 16 <= n_ctx;
-            uint8_t* dst = base + (size_t)(b0 + bl) * F::BLOCK;
-            if (c >= CODES / 16) {
-                // scales: four words, one (row, group) each
-                dst += s_off + 16 * c - CODES;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            uint32_t sw = 0u;
+            // rows from `end` on become zero: their source words may lie outside what was loaded, and are cleared below
+            const int end = last - row_b;
+            if (end > 0) {
+                if (is_v) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int word = 4 * (c - CODES / 16) + k, i = 16 * bl + word / F::NG;
-                    w[k] = b0 * 16 + i < last ? *reinterpret_cast<const uint32_t*>(src_byte(i) + CODES + ((i + skip) & 15) * F::SROWB + 4 * (word % F::NG)) : 0u;
-                    if (!whole) {
-                        const int row = b0 * 16 + i;
-                        if (row >= n_keep && row < n_ctx) reinterpret_cast<uint32_t*>(dst)[k] = w[k];
+                    for (int e = 0; e < 4; ++e) {
+                        const uint4 u = *reinterpret_cast<const uint4*>(win + from[e]);
+                        v.x = __byte_perm(v.x, u.x, sel[e]);
+                        v.y = __byte_perm(v.y, u.y, sel[e]);
+                        v.z = __byte_perm(v.z, u.z, sel[e]);
+                        v.w = __byte_perm(v.w, u.w, sel[e]);
                     }
+                    if (end < 16) {
+                        uint32_t keep = 0u;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (2 * (c & 3) + 8 * (e & 1) + (e >> 1) < end) keep |= 255u << (8 * e);
+                        v.x &= keep; v.y &= keep; v.z &= keep; v.w &= keep;
+                    }
+                } else if ((c >> 1) < end) {
+                    v = *reinterpret_cast<const uint4*>(win + k_from);
                 }
-            } else if (!is_v) {
-                // K codes: 16 bytes of one row
-                dst += c_off + 16 * c;
-                const int i = 16 * bl + 16 * c / F::ROWB, row = b0 * 16 + i;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (row < last) v = *reinterpret_cast<const uint4*>(src_byte(i) + ((i + skip) & 15) * F::ROWB + 16 * c % F::ROWB);
-                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-                if (!whole && row >= n_keep && row < n_ctx) *reinterpret_cast<uint4*>(dst) = v;
-            } else {
-                // V codes: four words of the rows 2t, 2t + 8, 2t + 1, 2t + 9
-                dst += c_off + 16 * c;
+                if ((c & 15) < end) sw = *reinterpret_cast<const uint32_t*>(win + sc_from);
+            }
+            uint8_t* dst = blk + piece;
+            if (row_b >= n_keep && row_b + 16 <= n_ctx) {
+                *reinterpret_cast<uint4*>(dst) = v;
+                if (c < 16) *reinterpret_cast<uint32_t*>(blk + s_off + c * F::SROWB + 4 * h) = sw;
+                continue;
+            }
+            // a block at either end: only the rows that move
+            auto moves = [&](int i) { return row_b + i >= n_keep && row_b + i < n_ctx; };
+            if (is_v) {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = 0u;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = 16 * bl + 2 * (c & 3) + 8 * (e & 1) + (e >> 1), row = b0 * 16 + i;
-                    const int ss = (i + skip) & 15;
-                    // the same pair of dims of the source row: place t of the row, and its byte
-                    const uint8_t* from = src_byte(i) + (c >> 5) * 512 + (((c & 31) & ~3) + ((ss & 7) >> 1)) * 16;
-                    const uint32_t sel = 8 * (2 * (ss & 1) + (ss >> 3));
-                    if (row < last) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(from);
-                        w[0] |= ((v.x >> sel) & 255u) << (8 * e);
-                        w[1] |= ((v.y >> sel) & 255u) << (8 * e);
-                        w[2] |= ((v.z >> sel) & 255u) << (8 * e);
-                        w[3] |= ((v.w >> sel) & 255u) << (8 * e);
-                    }
-                    if (!whole && row >= n_keep && row < n_ctx) {
+                for (int e = 0; e < 4; ++e)
+                    if (moves(2 * (c & 3) + 8 * (e & 1) + (e >> 1)))
 #pragma unroll
                         for (int k = 0; k < 4; ++k) dst[4 * k + e] = (uint8_t)(w[k] >> (8 * e));
-                    }
-                }
+            } else if (moves(c >> 1)) {
+                *reinterpret_cast<uint4*>(dst) = v;
             }
-            if (whole) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (c < 16 && moves(c)) *reinterpret_cast<uint32_t*>(blk + s_off + c * F::SROWB + 4 * h) = sw;
         }
     }
 }
@@ -358,42 +391,81 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
     const float qs = a.scale * LOG2E;
     const int jobs = a.n_head + (append ? 2 * a.n_kv : 0);
     float* row = reinterpret_cast<float*>(s_v[warp]);
-    for (int job = warp; job < jobs; job += kPrologueThreads / 32) {
-        const int kind = job < a.n_head ? 0 : (job < a.n_head + a.n_kv ? 1 : 2);
-        const int head = kind == 0 ? job : (kind == 1 ? job - a.n_head : job - a.n_head - a.n_kv);
-        const int heads = kind == 0 ? a.n_head : a.n_kv;
-        const float* src = (kind == 0 ? a.q : (kind == 1 ? a.k_new : a.v_new)) + ((size_t)b * heads + head) * HD;
-        const float* bias0 = kind == 0 ? a.pre.bias_q : (kind == 1 ? a.pre.bias_k : a.pre.bias_v);
-        const float* bias = bias0 ? bias0 + (size_t)head * HD : nullptr;
-        const float* nw = kind == 0 ? a.pre.norm_q : (kind == 1 ? a.pre.norm_k : nullptr);
-        const float rn = nw ? warp_row_rnorm(src, bias, HD, a.pre.eps, lane) : 1.f;
-        for (int e = lane; e < HD; e += 32) row[e] = pre_value(src, bias, nw, rn, e);
-        __syncwarp();
-        if (kind == 0 ? rope_q : (kind == 1 && rope_k)) {
-            for (int pp = lane; pp < a.rope.n_rot / 2; pp += 32) {
-                int i0, i1;
-                rope_pair_index(a.rope.rope_type, pp, a.rope.n_rot, i0, i1);
-                const double u = row[i0], w = row[i1], c = s_cos[pp], s = s_sin[pp];
-                row[i0] = (float)(u * c - w * s);
-                row[i1] = (float)(u * s + w * c);
+    constexpr int W = kPrologueThreads / 32, RB = 6;      // rows a warp has in flight (32 + 8 + 8 head rows over 8 warps)
+    struct Row { int kind, head; const float* src; const float* bias; };
+    auto describe = [&](int job) {
+        Row r;
+        r.kind = job < a.n_head ? 0 : (job < a.n_head + a.n_kv ? 1 : 2);
+        r.head = r.kind == 0 ? job : (r.kind == 1 ? job - a.n_head : job - a.n_head - a.n_kv);
+        r.src = (r.kind == 0 ? a.q : (r.kind == 1 ? a.k_new : a.v_new)) + ((size_t)b * (r.kind == 0 ? a.n_head : a.n_kv) + r.head) * HD + F::EPL * lane;
+        r.bias = r.kind == 0 ? a.pre.bias_q : (r.kind == 1 ? a.pre.bias_k : a.pre.bias_v);
+        if (r.bias) r.bias += (size_t)r.head * HD + F::EPL * lane;
+        return r;
+    };
+    for (int j0 = warp; j0 < jobs; j0 += W * RB) {
+        float in[RB][F::EPL];
+#pragma unroll
+        for (int u = 0; u < RB; ++u) {
+            if (j0 + u * W >= jobs) continue;
+            const Row r = describe(j0 + u * W);
+#pragma unroll
+            for (int e = 0; e < F::EPL; ++e) in[u][e] = r.src[e];
+            if (r.bias) {
+#pragma unroll
+                for (int e = 0; e < F::EPL; ++e) in[u][e] += r.bias[e];
             }
-            __syncwarp();
         }
-        float x[F::EPL];
 #pragma unroll
-        for (int e = 0; e < F::EPL; ++e) x[e] = row[F::EPL * lane + e];
-        __syncwarp();
-        if (kind == 0) {
-            __half* dst = a.q16 + ((size_t)b * a.n_head + head) * HD + F::EPL * lane;
+        for (int u = 0; u < RB; ++u) {
+            if (j0 + u * W >= jobs) continue;
+            const Row r = describe(j0 + u * W);
+            float (&x)[F::EPL] = in[u];
+            const float* nw = r.kind == 0 ? a.pre.norm_q : (r.kind == 1 ? a.pre.norm_k : nullptr);
+            if (nw) {
+                float ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < F::EPL; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_half2(x[e] * qs, x[e + 1] * qs);
-        } else {
+                for (int e = 0; e < F::EPL; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+                for (int off = 16; off; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+                const float rn = 1.0f / sqrtf(ss / (float)HD + a.pre.eps);
+#pragma unroll
+                for (int e = 0; e < F::EPL; ++e) x[e] = x[e] * rn * nw[F::EPL * lane + e];
+            }
+            if (r.kind == 0 ? rope_q : (r.kind == 1 && rope_k)) {
+                // the row passes through shared memory: a pair's two elements may lie in any two lanes
+#pragma unroll
+                for (int e = 0; e < F::EPL; ++e) row[F::EPL * lane + e] = x[e];
+                __syncwarp();
+                for (int pp = lane; pp < a.rope.n_rot / 2; pp += 32) {
+                    int i0, i1;
+                    rope_pair_index(a.rope.rope_type, pp, a.rope.n_rot, i0, i1);
+                    if (r.kind == 0) {
+                        const float v0 = row[i0], v1 = row[i1], c = (float)s_cos[pp], s = (float)s_sin[pp];
+                        row[i0] = v0 * c - v1 * s;
+                        row[i1] = v0 * s + v1 * c;
+                    } else {
+                        const double v0 = row[i0], v1 = row[i1], c = s_cos[pp], s = s_sin[pp];
+                        row[i0] = (float)(v0 * c - v1 * s);
+                        row[i1] = (float)(v0 * s + v1 * c);
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < F::EPL; ++e) x[e] = row[F::EPL * lane + e];
+                __syncwarp();
+            }
+            if (r.kind == 0) {
+                __half* dst = a.q16 + ((size_t)b * a.n_head + r.head) * HD + F::EPL * lane;
+#pragma unroll
+                for (int e = 0; e < F::EPL; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_half2(x[e] * qs, x[e + 1] * qs);
+                continue;
+            }
             const Q4Scale s = q4_scale<HD>(x, lane);
             const uint32_t codes = q4_codes<HD>(x, s);
-            uint8_t* blk = p.cache + ((size_t)head * nblk + (pos >> 4)) * F::BLOCK;
-            if (kind == 2) q4_store_row<HD, true>(blk, pos & 15, codes, s, lane);
-            else           q4_store_row<HD, false>(blk, pos & 15, codes, s, lane);
-            __half* dst = (kind == 1 ? p.k16 : p.v16) + ((size_t)head * rows + pos) * HD + F::EPL * lane;
+            uint8_t* blk = p.cache + ((size_t)r.head * nblk + (pos >> 4)) * F::BLOCK;
+            if (r.kind == 2) q4_store_row<HD, true>(blk, pos & 15, codes, s, lane);
+            else             q4_store_row<HD, false>(blk, pos & 15, codes, s, lane);
+            __half* dst = (r.kind == 1 ? p.k16 : p.v16) + ((size_t)r.head * rows + pos) * HD + F::EPL * lane;
             const float d = __half2float(s.d), m = __half2float(s.m);
 #pragma unroll
             for (int e = 0; e < F::EPL; e += 2)
@@ -401,8 +473,6 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
         }
     }
 }
-
-constexpr int shift_smem(int head_dim) { return kShiftWindows * (kShiftBlocks + 1) * 9 * head_dim; }
 
 } // namespace
 
@@ -437,7 +507,7 @@ cudaError_t kv_q4_set_attributes() {
 
 cudaError_t launch_kv_store_q4(uint8_t* cache, const float* k, const float* v, int heads, int head_dim, int n_ctx, int pos_base,
                                int batch, const int* d_pos, cudaStream_t stream, unsigned long long* launches) {
-    const dim3 grid(d_pos ? 1 : ((pos_base + batch - 1) >> 4) - (pos_base >> 4) + 1, heads);
+    const dim3 grid((unsigned)heads * (d_pos ? 1 : ((pos_base + batch - 1) >> 4) - (pos_base >> 4) + 1));
     if (head_dim == 128) kv_store_q4_kernel<128><<<grid, kStoreThreads, 0, stream>>>(cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
     else                 kv_store_q4_kernel<64><<<grid, kStoreThreads, 0, stream>>>(cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
     if (launches) *launches += 1;
@@ -456,7 +526,7 @@ cudaError_t launch_kv_load_q4(const uint8_t* cache, uint16_t* kc, uint16_t* vc, 
 
 cudaError_t launch_kv_shift_q4(uint8_t* cache, int n_layer, int n_kv, int head_dim, int n_ctx, int n_keep, int shift,
                                cudaStream_t stream, unsigned long long* launches) {
-    const dim3 grid(2, n_layer * n_kv);
+    const dim3 grid(2 * head_dim / 64, n_layer * n_kv);
     if (head_dim == 128) kv_shift_q4_kernel<128><<<grid, kShiftThreads, shift_smem(128), stream>>>(cache, n_ctx, n_keep, shift);
     else                 kv_shift_q4_kernel<64><<<grid, kShiftThreads, shift_smem(64), stream>>>(cache, n_ctx, n_keep, shift);
     if (launches) *launches += 1;

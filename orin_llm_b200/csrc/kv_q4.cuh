@@ -88,6 +88,8 @@ __device__ __forceinline__ Q4Scale q4_scale(const float (&x)[Q4<HD>::EPL], int l
     return q4_scale_of(mask ? CUDART_NAN_F : mn, mx);
 }
 
+static __device__ __noinline__ float q4_code_at_border(float x, float m, float d) { return (float)rint(((double)x - (double)m) / (double)d); }
+
 // code of x.  The fp32 quotient is off by less than 4e-6 where it is below 16; only next to a border between two codes
 // does that matter, and there the quotient is formed in double (an fp32 value minus an fp16 one and the border times d are
 // both exact in double, or far apart).
@@ -95,7 +97,7 @@ __device__ __forceinline__ uint32_t q4_code(float x, float m, float d, float inv
     if (!(d > 0.f)) return 0u;
     const float y = (x - m) * inv;
     float q = rintf(y);
-    if (fabsf(fabsf(y - q) - 0.5f) < 1e-5f) q = (float)rint(((double)x - (double)m) / (double)d);
+    if (fabsf(fabsf(y - q) - 0.5f) < 1e-5f) q = q4_code_at_border(x, m, d);
     return (uint32_t)fminf(fmaxf(q, 0.f), 15.f);
 }
 
