@@ -319,14 +319,15 @@ class KVCache:
 
 def _q4_check(dev, name, t, dtype, numel):
     """The checks the C entry cannot make: a contiguous tensor of that type and size on CUDA device `dev`; -> its address."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError("%s: a tensor is needed, got %s" % (name, type(t).__name__))
+    try:
+        if t.dtype is dtype and t.numel() >= numel and t.is_contiguous() and t.get_device() == dev:
+            return t.data_ptr()
+    except AttributeError:
+        raise TypeError("%s: a tensor is needed, got %s" % (name, type(t).__name__)) from None
     if t.dtype is not dtype or t.numel() < numel or not t.is_contiguous():
         raise ValueError("%s: a contiguous %s tensor of at least %d elements is needed, got %s %s%s" % (
             name, dtype, numel, t.dtype, list(t.shape), "" if t.is_contiguous() else ", not contiguous"))
-    if t.get_device() != dev:
-        raise ValueError("%s: on %s, the cache on device %d" % (name, t.device, dev))
-    return t.data_ptr()
+    raise ValueError("%s: on %s, the cache on device %d" % (name, t.device, dev))
 
 
 def _q4_cache(cache, layers, n_kv, head_dim, n_ctx):
@@ -336,7 +337,7 @@ def _q4_cache(cache, layers, n_kv, head_dim, n_ctx):
         raise capi.AttnError(capi.ERR_UNSUPPORTED, "4-bit cache: head_dim 64 or 128, at least one head and one position")
     dev = cache.get_device() if isinstance(cache, torch.Tensor) else -1
     ptr = _q4_check(dev, "cache", cache, torch.uint8, layers * nbytes)
-    if dev < 0 or dev != torch.cuda.current_device():
+    if dev < 0 or dev != torch._C._cuda_getDevice():
         raise ValueError("cache: on %s, not on the current CUDA device" % cache.device)
     return dev, ptr
 
@@ -389,7 +390,7 @@ def kv_shift_q4(cache, n_layer, n_kv, head_dim, n_ctx, n_keep, shift):
 
 def decode_q4_workspace(n_head, n_kv, head_dim):
     """Scratch for attn_decode_q4, allocated once per shape and device."""
-    key = (n_head, n_kv, head_dim, torch.cuda.current_device())
+    key = (n_head, n_kv, head_dim, torch._C._cuda_getDevice())
     ws = _state["decode_q4_ws"].get(key)
     if ws is None:
         nbytes = capi.lib().oattn_decode_q4_workspace_bytes(n_head, n_kv, head_dim)
