@@ -623,7 +623,8 @@ int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, voi
     if (!q || (!out && !out_f16 && !mmq) || (out && out_f16) || !(scale > 0.0f)) return OATTN_ERR_ARG;
     if (mmq && (head_dim != 128 || g_prefill_impl != 0 || ((uintptr_t)ext->out_mmq & 15))) return OATTN_ERR_UNSUPPORTED;
     if (batch <= 0 || n_past < 0 || n_past > n_ctx - batch) return OATTN_ERR_ARG;
-    if (((uintptr_t)out | (uintptr_t)out_f16) & 15) return OATTN_ERR_ARG;
+    if (((uintptr_t)out | (uintptr_t)out_f16 | (uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new) & 15) return OATTN_ERR_ARG;
+    if (ext && (((uintptr_t)ext->bias_q | (uintptr_t)ext->bias_k | (uintptr_t)ext->bias_v) & 15)) return OATTN_ERR_ARG;
     if (fuse & ~OATTN_FUSE_ALL) return OATTN_ERR_ARG;
     if ((fuse & OATTN_FUSE_ROPE_K) && !(fuse & OATTN_FUSE_KV_APPEND)) return OATTN_ERR_ARG;
     if ((fuse & OATTN_FUSE_KV_APPEND) && (!k_new || !v_new)) return OATTN_ERR_ARG;

@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kShiftThreads) kv_shift_q4_kernel(uint8_t* cac
 constexpr int kPrologueThreads = 256;
 
 template <int HD>
-__global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(const __grid_constant__ KvQ4PrologueArgs p) {
+__global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kernel(const __grid_constant__ KvQ4PrologueArgs p) {
     using F = Q4<HD>;
     const PrefillArgs& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -365,19 +365,48 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
     const bool rope_q = (a.fuse & 1) != 0, rope_k = (a.fuse & 2) != 0, append = (a.fuse & 4) != 0;
     pdl_trigger();
     __shared__ __align__(16) uint8_t s_v[kPrologueThreads / 32][16 * kVStride<HD>];
-    if ((int)blockIdx.x >= a.batch) {
+    // the two kinds of CTAs alternate, so that an SM has copies to run while its tokens wait for their rows
+    const int n_copy = (int)gridDim.x - a.batch, both = 2 * min(a.batch, n_copy);
+    const int bid = blockIdx.x;
+    const bool copies = bid < both ? (bid & 1) != 0 : n_copy > a.batch;
+    const int idx = bid < both ? bid >> 1 : bid - both / 2;
+    if (copies) {
         pdl_wait();
         const int expand = append ? a.n_past : rows, nb = q4_blocks(expand);
-        const long long job = (long long)(blockIdx.x - a.batch) * (kPrologueThreads / 32) + warp;
+        const long long job = (long long)idx * (kPrologueThreads / 32) + warp;
         if (job >= (long long)a.n_kv * nb) return;
         const int head = (int)(job / nb), b = (int)(job % nb);
         const size_t dst = ((size_t)head * rows + 16 * b) * HD;
         q4_load_block<HD>(p.cache + ((size_t)head * nblk + b) * F::BLOCK, p.k16 + dst, p.v16 + dst, 0, min(expand - 16 * b, 16), s_v[warp], lane);
         return;
     }
+    const int b = idx, pos = a.n_past + b;
+    const float qs = a.scale * LOG2E;
+    const int jobs = a.n_head + (append ? 2 * a.n_kv : 0);
+    // A warp has eight head rows in flight (48 rows over 8 warps is the usual case), in shared memory rather than in registers: the loop
+    // over them is not unrolled, because the instruction cache is what a launch of a few microseconds waits for.
+    constexpr int W = kPrologueThreads / 32, RB = 8;
+    static_assert(RB * HD * 4 <= 16 * kVStride<HD>, "the rows fit in the warp's part of s_v");
+    float* rows_s = reinterpret_cast<float*>(s_v[warp]);
+    struct Row { int kind, head; };                       // q, k or v
+    auto describe = [&](int job) {
+        Row r;
+        r.kind = job < a.n_head ? 0 : (job < a.n_head + a.n_kv ? 1 : 2);
+        r.head = r.kind == 0 ? job : (r.kind == 1 ? job - a.n_head : job - a.n_head - a.n_kv);
+        return r;
+    };
+    auto load_rows = [&](int j0) {
+        for (int u = 0; u < RB && j0 + u * W < jobs; ++u) {
+            const Row r = describe(j0 + u * W);
+            const float* src = (r.kind == 0 ? a.q : (r.kind == 1 ? a.k_new : a.v_new)) + ((size_t)b * (r.kind == 0 ? a.n_head : a.n_kv) + r.head) * HD;
+            if (4 * lane < HD) cp_async_16(smem_u32(rows_s + u * HD + 4 * lane), src + 4 * lane, 16);
+        }
+        cp_async_commit();
+    };
+    pdl_wait();
+    load_rows(warp);
     // cos and sin in double: a key's code is a decision at a border, so the rotated key is rounded to fp32 once
     __shared__ double s_cos[HD / 2], s_sin[HD / 2];
-    const int b = blockIdx.x, pos = a.n_past + b;
     if (rope_q || rope_k) {
         for (int i = tid; i < a.rope.n_rot / 2; i += kPrologueThreads) {
             float f = p.freq[i];
@@ -385,41 +414,24 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
             sincos((double)__fmul_rn((float)pos, f), &s_sin[i], &s_cos[i]);
         }
     }
-    pdl_wait();
     __syncthreads();
     if (b == 0 && tid == 0 && a.status) *a.status = 0;
-    const float qs = a.scale * LOG2E;
-    const int jobs = a.n_head + (append ? 2 * a.n_kv : 0);
-    float* row = reinterpret_cast<float*>(s_v[warp]);
-    constexpr int W = kPrologueThreads / 32, RB = 6;      // rows a warp has in flight (32 + 8 + 8 head rows over 8 warps)
-    struct Row { int kind, head; const float* src; const float* bias; };
-    auto describe = [&](int job) {
-        Row r;
-        r.kind = job < a.n_head ? 0 : (job < a.n_head + a.n_kv ? 1 : 2);
-        r.head = r.kind == 0 ? job : (r.kind == 1 ? job - a.n_head : job - a.n_head - a.n_kv);
-        r.src = (r.kind == 0 ? a.q : (r.kind == 1 ? a.k_new : a.v_new)) + ((size_t)b * (r.kind == 0 ? a.n_head : a.n_kv) + r.head) * HD + F::EPL * lane;
-        r.bias = r.kind == 0 ? a.pre.bias_q : (r.kind == 1 ? a.pre.bias_k : a.pre.bias_v);
-        if (r.bias) r.bias += (size_t)r.head * HD + F::EPL * lane;
-        return r;
-    };
     for (int j0 = warp; j0 < jobs; j0 += W * RB) {
-        float in[RB][F::EPL];
-#pragma unroll
-        for (int u = 0; u < RB; ++u) {
-            if (j0 + u * W >= jobs) continue;
+        if (j0 != warp) load_rows(j0);
+        cp_async_wait<0>();
+        __syncwarp();
+#pragma unroll 1
+        for (int u = 0; u < RB && j0 + u * W < jobs; ++u) {
             const Row r = describe(j0 + u * W);
+            float* row = rows_s + u * HD;
+            float x[F::EPL];
 #pragma unroll
-            for (int e = 0; e < F::EPL; ++e) in[u][e] = r.src[e];
-            if (r.bias) {
+            for (int e = 0; e < F::EPL; ++e) x[e] = row[F::EPL * lane + e];
+            const float* bias = r.kind == 0 ? a.pre.bias_q : (r.kind == 1 ? a.pre.bias_k : a.pre.bias_v);
+            if (bias) {
 #pragma unroll
-                for (int e = 0; e < F::EPL; ++e) in[u][e] += r.bias[e];
+                for (int e = 0; e < F::EPL; ++e) x[e] += bias[(size_t)r.head * HD + F::EPL * lane + e];
             }
-        }
-#pragma unroll
-        for (int u = 0; u < RB; ++u) {
-            if (j0 + u * W >= jobs) continue;
-            const Row r = describe(j0 + u * W);
-            float (&x)[F::EPL] = in[u];
             const float* nw = r.kind == 0 ? a.pre.norm_q : (r.kind == 1 ? a.pre.norm_k : nullptr);
             if (nw) {
                 float ss = 0.f;
@@ -452,7 +464,6 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
                 __syncwarp();
 #pragma unroll
                 for (int e = 0; e < F::EPL; ++e) x[e] = row[F::EPL * lane + e];
-                __syncwarp();
             }
             if (r.kind == 0) {
                 __half* dst = a.q16 + ((size_t)b * a.n_head + r.head) * HD + F::EPL * lane;
@@ -471,6 +482,7 @@ __global__ void __launch_bounds__(kPrologueThreads) prefill_q4_prologue_kernel(c
             for (int e = 0; e < F::EPL; e += 2)
                 *reinterpret_cast<uint32_t*>(dst + e) = pack_half2(q4_value((codes >> (4 * e)) & 15u, d, m), q4_value((codes >> (4 * e + 4)) & 15u, d, m));
         }
+        __syncwarp();                                     // every lane is done with the rows
     }
 }
 
