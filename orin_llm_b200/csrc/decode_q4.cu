@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         pdl_wait();
         load_inputs();
     }
-    const int npos = max(0, min(*p.d_pos + 1, p.n_ctx));
+    const int npos = max(0, min(*p.d_pos, p.n_ctx - 1) + 1);
     const Q4Plan plan = q4_plan(npos, p.n_splits);
     if (split >= max(plan.active, 1)) return;
     const int vh = kvh * p.head_blocks + hb;                 // place of this CTA's heads in the scratch block

@@ -1,0 +1,463 @@
+"""GPU tests of the 4-bit cache's calls as a program makes them: bias, norm and quantised outputs around them, partial rotation,
+launch overlap, graphs, streams, a whole conversation, large caches, and refusals.  Tolerances: test_kv_q4_gpu.py."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import q4_reference as ref
+from test_kv_q4_gpu import decode_bound, dev, filled, prefill_bound, rows
+
+pytestmark = pytest.mark.gpu
+
+
+def dpos(p):
+    return torch.tensor([p], dtype=torch.int32, device="cuda")
+
+
+def normed(x, bias, w, eps):
+    x = x.astype(np.float32) + bias.astype(np.float32)
+    if w is None:
+        return x
+    x = x.astype(np.float64)
+    return (x / np.sqrt((x ** 2).mean(-1, keepdims=True) + eps) * w).astype(np.float32)
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd,n_rot,rope_type,norm", [(12, 2, 128, 128, 1, True), (14, 2, 64, 32, 1, False), (8, 8, 128, 96, 0, False),
+                                                                (20, 2, 64, 64, 0, True)])
+def test_bias_norm_and_partial_rotation_in_front(ops, n_head, n_kv, hd, n_rot, rope_type, norm):
+    """A chunk through the prefill call and one more token through the decode call."""
+    rng = np.random.default_rng(200)
+    past, batch, n_ctx, theta, eps = 19, 21, 64, 1e4, 1e-6
+    cache = filled(rng, n_kv, hd, n_ctx, past)
+    n = batch + 1
+    q, k, v = rng.standard_normal((n, n_head, hd)).astype(np.float32), rows(rng, n, n_kv, hd), rows(rng, n, n_kv, hd)
+    ff = (1 + rng.random(n_rot // 2)).astype(np.float32)
+    b = {m: rng.standard_normal((h, hd)).astype(np.float32) for m, h in (("bias_q", n_head), ("bias_k", n_kv), ("bias_v", n_kv))}
+    w = {m: (1 + 0.2 * rng.standard_normal(hd)).astype(np.float32) for m in ("norm_q", "norm_k")} if norm else {}
+    ext = {m: dev(x) for m, x in {**b, **w}.items()}
+    if norm:
+        ext["norm_eps"] = eps
+    d_cache, d_ff = dev(cache), dev(ff)
+    rope, scale = (rope_type, n_rot, theta, d_ff), 1.0 / math.sqrt(hd)
+    out = torch.empty(n, n_head, hd, device="cuda")
+    ops.attn_prefill_q4(dev(q[:batch]), dev(k[:batch]), dev(v[:batch]), d_cache, out[:batch], n_head, n_kv, hd, n_ctx, past, batch, scale,
+                        ops.FUSE_ALL, rope, ext=ext)
+    ops.attn_decode_q4(dev(q[batch]), dev(k[batch]), dev(v[batch]), d_cache, out[batch], n_head, n_kv, hd, n_ctx, dpos(past + batch), scale,
+                       ops.FUSE_ALL, rope, ext=ext)
+    torch.cuda.synchronize()
+    pos = np.arange(past, past + n)
+    qr = ref.rope(normed(q, b["bias_q"], w.get("norm_q"), eps), pos, rope_type, n_rot, theta, ff)
+    kr = ref.rope(normed(k, b["bias_k"], w.get("norm_k"), eps), pos, rope_type, n_rot, theta, ff).astype(np.float32)
+    want = cache.copy()
+    ref.write_rows(want, hd, pos, kr, v + b["bias_v"])
+    got = d_cache.cpu().numpy()
+    if not norm:                       # (a norm is a sum in fp32: its last bit may move a code)
+        assert np.array_equal(got, want)
+    K, V = ref.read_rows(got, hd, past + n)
+    Kw, _ = ref.read_rows(want, hd, past + n)
+    assert np.abs(K - Kw).max() <= 0.6 * np.abs(Kw).max() / 7 and (np.abs(K - Kw) > 1e-2).mean() < 1e-3
+    res, most = ref.attend(qr, K, V, past, scale)
+    err = np.abs(out.cpu().numpy() - res)
+    assert err[:batch].max() <= prefill_bound(most, scale, V, False)
+    # q's norm is another fp32 sum: 2^-20 of the scores covers it
+    assert err[batch].max() <= 2 * decode_bound(most, scale, V)
+
+
+def test_decode_writes_the_quantised_activation(ops, oracle):
+    rng = np.random.default_rng(201)
+    n_head, n_kv, hd, n = 12, 2, 128, 300
+    cache = dev(filled(rng, n_kv, hd, n, n))
+    q = dev(rng.standard_normal((n_head, hd)).astype(np.float32))
+    out = torch.empty(n_head, hd, device="cuda")
+    qs, sc = torch.empty(n_head * hd, dtype=torch.int8, device="cuda"), torch.empty(n_head * hd // 32, device="cuda")
+    for o in (out, None):
+        ops.attn_decode_q4(q, None, None, cache, o, n_head, n_kv, hd, n, dpos(n - 1), 0.09, ops.FUSE_NONE, ext=dict(out_qs=qs, out_scales=sc))
+        torch.cuda.synchronize()
+        want_q, want_d = oracle.quantize_q8_1(out.cpu().numpy().reshape(-1))
+        assert np.array_equal(qs.cpu().numpy(), want_q) and np.array_equal(sc.cpu().numpy(), want_d)
+
+
+def test_prefill_block_output_and_other_kernel(ops):
+    """out_mmq next to and instead of the fp32 output; the warp-level kernel with both output types."""
+    rng = np.random.default_rng(202)
+    n_head, n_kv, hd, past, batch = 8, 2, 128, 40, 29
+    n_ctx = past + batch
+    base = filled(rng, n_kv, hd, n_ctx, past)
+    q, k, v = (dev(x) for x in (rng.standard_normal((batch, n_head, hd)).astype(np.float32), rows(rng, batch, n_kv, hd), rows(rng, batch, n_kv, hd)))
+    rope = (1, hd, 1e6, None)
+
+    def run(out, **kw):
+        cache = dev(base)
+        ops.attn_prefill_q4(q, k, v, cache, out, n_head, n_kv, hd, n_ctx, past, batch, 0.0884, ops.FUSE_ALL, rope, **kw)
+        torch.cuda.synchronize()
+        assert ops.prefill_status(n_head, n_kv, hd, batch, ops.prefill_q4_workspace(n_head, n_kv, hd, batch, n_ctx)) == 0
+        return cache
+
+    f32, f16 = torch.empty(batch, n_head, hd, device="cuda"), torch.empty(batch, n_head, hd, dtype=torch.float16, device="cuda")
+    blk = [torch.zeros(n_head * batch * 144, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    a = run(f32)
+    assert torch.equal(a, run(f16)) and torch.equal(f16, f32.half())
+    again = torch.empty_like(f32)
+    run(again, ext=dict(out_mmq=blk[0]))
+    run(None, ext=dict(out_mmq=blk[1]))
+    run(f16, ext=dict(out_mmq=blk[2]))
+    assert torch.equal(again, f32) and torch.equal(blk[0], blk[1]) and torch.equal(blk[0], blk[2])
+    b = blk[0].view(n_head, batch, 144)
+    d = b[..., :16].contiguous().view(torch.float32)
+    val = (b[..., 16:].contiguous().view(torch.int8).view(n_head, batch, 4, 32).float() * d[..., None]).reshape(n_head, batch, hd).transpose(0, 1)
+    step = d.transpose(0, 1).repeat_interleave(32, -1)
+    assert ((val - f32).abs() <= 0.5001 * step + 1e-7).all()
+    try:
+        ops.set_prefill_impl(1)
+        m32, m16 = torch.empty_like(f32), torch.empty_like(f16)
+        run(m32)
+        run(m16)
+    finally:
+        ops.set_prefill_impl(0)
+    K, V = ref.read_rows(a.cpu().numpy(), hd, n_ctx)
+    want, most = ref.attend(ref.rope(q.cpu().numpy(), np.arange(past, n_ctx), 1, hd, 1e6), K, V, past, 0.0884)
+    assert np.abs(m32.cpu().numpy() - want).max() <= prefill_bound(most, 0.0884, V, False)
+    assert torch.equal(m16, m32.half())
+
+
+def test_many_heads_in_the_prologue(ops):
+    """More head rows than a prologue CTA has in flight at once."""
+    rng = np.random.default_rng(203)
+    n_head, n_kv, hd, batch = 96, 16, 64, 3
+    q, k, v = rng.standard_normal((batch, n_head, hd)).astype(np.float32), rows(rng, batch, n_kv, hd), rows(rng, batch, n_kv, hd)
+    cache = np.zeros((n_kv, 1, 18 * hd), np.uint8)
+    d_cache, out = dev(cache), torch.empty(batch, n_head, hd, device="cuda")
+    ops.attn_prefill_q4(dev(q), dev(k), dev(v), d_cache, out, n_head, n_kv, hd, 7, 0, batch, 0.125, ops.FUSE_ALL, (1, hd, 1e6, None))
+    pos = np.arange(batch)
+    ref.write_rows(cache, hd, pos, ref.rope(k, pos, 1, hd, 1e6).astype(np.float32), v)
+    assert np.array_equal(d_cache.cpu().numpy(), cache)
+    K, V = ref.read_rows(cache, hd, batch)
+    want, most = ref.attend(ref.rope(q, pos, 1, hd, 1e6), K, V, 0, 0.125)
+    assert np.abs(out.cpu().numpy() - want).max() <= prefill_bound(most, 0.125, V, False)
+
+
+# ------------------------------------------------------------------------------------------------- a run of them together
+@pytest.mark.parametrize("n_head,n_kv,hd", [(12, 2, 128), (18, 2, 64)])
+def test_a_conversation(ops, n_head, n_kv, hd):
+    """Prompt in two chunks, decode steps, the context rolled, more steps, on two layers; the cache's bytes and every output against
+    the 64-bit reference.  The rows one call appends are the bytes another would."""
+    rng = np.random.default_rng(210)
+    n_layer, n_ctx, theta, scale = 2, 75, 1e6, 1.0 / math.sqrt(hd)
+    cache = ops.KVCacheQ4(n_layer, n_kv, n_ctx, hd)
+    want = cache.buf.cpu().numpy()
+    rope = (1, hd, theta, None)
+
+    def step(n_past, n, call):
+        for l in range(n_layer):
+            q, k, v = rng.standard_normal((n, n_head, hd)).astype(np.float32), rows(rng, n, n_kv, hd), rows(rng, n, n_kv, hd)
+            pos = np.arange(n_past, n_past + n)
+            kr = ref.rope(k, pos, 1, hd, theta).astype(np.float32)
+            ref.write_rows(want[l], hd, pos, kr, v)
+            out = torch.empty(n, n_head, hd, device="cuda")
+            if call == "prefill":
+                ops.attn_prefill_q4(dev(q), dev(k), dev(v), cache.layer(l), out, n_head, n_kv, hd, n_ctx, n_past, n, scale, ops.FUSE_ALL, rope)
+            elif call == "decode":
+                ops.attn_decode_q4(dev(q[0]), dev(k[0]), dev(v[0]), cache.layer(l), out[0], n_head, n_kv, hd, n_ctx, dpos(n_past), scale, ops.FUSE_ALL, rope)
+            else:                                          # the unfused sequence
+                ops.kv_store_q4_ind(cache.layer(l), dev(kr[0]), dev(v[0]), n_kv, hd, n_ctx, dpos(n_past))
+                ops.attn_decode_q4(dev(q[0]), None, None, cache.layer(l), out[0], n_head, n_kv, hd, n_ctx, dpos(n_past), scale, ops.FUSE_ROPE_Q, rope)
+            K, V = ref.read_rows(want[l], hd, n_past + n)
+            res, most = ref.attend(ref.rope(q, pos, 1, hd, theta), K, V, n_past, scale)
+            bound = prefill_bound(most, scale, V, False) if call == "prefill" else decode_bound(most, scale, V)
+            assert np.abs(out.cpu().numpy() - res).max() <= bound, (call, n_past)
+        assert np.array_equal(cache.buf.cpu().numpy(), want), (call, n_past)
+
+    step(0, 37, "prefill")
+    step(37, 20, "prefill")
+    for p in range(57, 75):
+        step(p, 1, "decode" if p % 2 else "store")
+    n_keep, shift = 5, 34
+    cache.shift(n_keep, shift)
+    torch.cuda.synchronize()
+    for l in range(n_layer):
+        K, V = ref.read_rows(want[l], hd, n_ctx)
+        gK, gV = ref.read_rows(cache.layer(l).cpu().numpy(), hd, n_ctx)
+        for g, x in ((gK, K), (gV, V)):
+            moved = np.concatenate((x[:, :n_keep], x[:, n_keep + shift:], np.zeros_like(x[:, :shift])), 1)
+            assert np.array_equal(g, moved)
+    want[:] = cache.buf.cpu().numpy()
+    for p in range(n_ctx - shift, n_ctx - shift + 9):
+        step(p, 1, "decode")
+    # taken over into an fp16 cache, the rows are those the reference reads
+    half = ops.KVCache(n_layer, n_kv, 96, hd)
+    for l in range(n_layer):
+        ops.kv_load_q4(cache.layer(l), *half.layer(l), n_kv, hd, n_ctx, 0, n_ctx, 96, 0)
+        for g, x in zip(half.layer(l), ref.read_rows(want[l], hd, n_ctx)):
+            assert np.abs(g[:, :n_ctx].float().cpu().numpy() - x).max() <= 2.0 ** -11 * np.abs(x).max()
+
+
+# ------------------------------------------------------------------------------------------------- order and overlap
+@pytest.mark.parametrize("mode", [0, 1, 2])
+def test_launch_overlap(ops, mode):
+    """The unfused pair and the fused call under every launch mode, back to back over layers of their own, with a decoy in
+    the row the store call overwrites."""
+    rng = np.random.default_rng(220)
+    n_head, n_kv, hd, n, layers = 16, 2, 128, 700, 6
+    scale = 1.0 / math.sqrt(hd)
+    q = [dev(rng.standard_normal((n_head, hd)).astype(np.float32)) for _ in range(layers)]
+    kv = [(rows(rng, 1, n_kv, hd), rows(rng, 1, n_kv, hd)) for _ in range(layers)]
+    base = []
+    for l in range(layers):
+        c = filled(rng, n_kv, hd, n + 3, n - 1)
+        ref.write_rows(c, hd, [n - 1], 100 * np.ones((1, n_kv, hd), np.float32), 100 * np.ones((1, n_kv, hd), np.float32))
+        base.append(c)
+    outs = {}
+    for m in (0, mode):
+        for fused in (False, True):
+            caches = [dev(c) for c in base]
+            new = [(dev(k[0]), dev(v[0])) for k, v in kv]
+            out = torch.empty(layers, n_head, hd, device="cuda")
+            pos = dpos(n - 1)
+            torch.cuda.synchronize()
+            ops.set_decode_overlap(m)
+            try:
+                for l in range(layers):
+                    if fused:
+                        ops.attn_decode_q4(q[l], new[l][0], new[l][1], caches[l], out[l], n_head, n_kv, hd, n + 3, pos, scale, ops.FUSE_KV_APPEND)
+                    else:
+                        ops.kv_store_q4_ind(caches[l], new[l][0], new[l][1], n_kv, hd, n + 3, pos)
+                        ops.attn_decode_q4(q[l], None, None, caches[l], out[l], n_head, n_kv, hd, n + 3, pos, scale, ops.FUSE_NONE)
+                torch.cuda.synchronize()
+            finally:
+                ops.set_decode_overlap(0)
+            outs[m, fused] = (out, torch.stack(caches))
+    first = outs[0, False]
+    for got in outs.values():
+        assert torch.equal(got[0], first[0]) and torch.equal(got[1], first[1])
+    want = base[0].copy()
+    ref.write_rows(want, hd, [n - 1], *kv[0])
+    assert np.array_equal(first[1][0].cpu().numpy(), want)
+
+
+def test_graph_replays_across_block_and_slice_borders(ops):
+    """One captured step with the position in device memory, replayed over 60 tokens: the same outputs and bytes as eager calls."""
+    rng = np.random.default_rng(221)
+    n_head, n_kv, hd, n_ctx, start, steps = 14, 2, 128, 400, 250, 60
+    base = dev(filled(rng, n_kv, hd, n_ctx, start))
+    q, k, v = (dev(rng.standard_normal((steps, h, hd)).astype(np.float32)) for h in (n_head, n_kv, n_kv))
+    rope, scale = (1, hd, 1e6, None), 0.0884
+
+    def program(cache, sq, sk, sv, out, pos, ws):
+        ops.attn_decode_q4(sq, sk, sv, cache, out, n_head, n_kv, hd, n_ctx, pos, scale, ops.FUSE_ALL, rope, ws)
+
+    eager_cache, graph_cache = base.clone(), base.clone()
+    eager, graph = (torch.empty(steps, n_head, hd, device="cuda") for _ in range(2))
+    ws = torch.empty_like(ops.decode_q4_workspace(n_head, n_kv, hd))
+    sq, sk, sv, so, sp = q[0].clone(), k[0].clone(), v[0].clone(), torch.empty(n_head, hd, device="cuda"), dpos(start)
+    program(base.clone(), sq, sk, sv, so, sp, ws)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        program(graph_cache, sq, sk, sv, so, sp, ws)
+    for i in range(steps):
+        program(eager_cache, q[i], k[i], v[i], eager[i], dpos(start + i), None)
+        for dst, src in ((sq, q[i]), (sk, k[i]), (sv, v[i])):
+            dst.copy_(src)
+        sp.fill_(start + i)
+        g.replay()
+        graph[i].copy_(so)
+    torch.cuda.synchronize()
+    assert torch.equal(eager, graph) and torch.equal(eager_cache, graph_cache)
+
+
+def test_two_streams_with_workspaces_of_their_own(ops):
+    rng = np.random.default_rng(222)
+    n_head, n_kv, hd, n = 16, 2, 128, 20000
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    caches, qs, want = [], [], []
+    for i in range(2):
+        c = ops.KVCacheQ4(1, n_kv, n, hd).layer(0)
+        k, v = (torch.randn(n, n_kv, hd, device="cuda", generator=gen) for _ in range(2))
+        ops.kv_store_q4_batch(c, k, v, n_kv, hd, n, 0, n)
+        caches.append(c)
+        qs.append(torch.randn(n_head, hd, device="cuda", generator=gen))
+        o = torch.empty(n_head, hd, device="cuda")
+        ops.attn_decode_q4(qs[i], None, None, c, o, n_head, n_kv, hd, n, dpos(n - 1), 0.0884, ops.FUSE_NONE)
+        want.append(o)
+    pos = dpos(n - 1)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ws = [torch.empty_like(ops.decode_q4_workspace(n_head, n_kv, hd)) for _ in range(2)]
+    out = torch.zeros(2, 20, n_head, hd, device="cuda")
+    torch.cuda.synchronize()
+    for r in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                ops.attn_decode_q4(qs[i], None, None, caches[i], out[i, r], n_head, n_kv, hd, n, pos, 0.0884, ops.FUSE_NONE, None, ws[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(out[i, r], want[i]) for r in range(20))
+    # and through set_stream, which the other calls of this module take as well
+    try:
+        ops.set_stream(streams[0])
+        o = torch.empty(n_head, hd, device="cuda")
+        torch.cuda.synchronize()
+        ops.attn_decode_q4(qs[1], None, None, caches[1], o, n_head, n_kv, hd, n, pos, 0.0884, ops.FUSE_NONE)
+        streams[0].synchronize()
+        assert torch.equal(o, want[1])
+    finally:
+        ops.set_stream(None)
+
+
+def test_prefill_captured(ops):
+    rng = np.random.default_rng(223)
+    n_head, n_kv, hd, past, batch = 8, 2, 128, 50, 40
+    n_ctx = past + batch
+    base = dev(filled(rng, n_kv, hd, n_ctx, past))
+    q, k, v = (dev(rng.standard_normal((batch, h, hd)).astype(np.float32)) for h in (n_head, n_kv, n_kv))
+    ws = torch.empty(2 * ops.prefill_q4_workspace(n_head, n_kv, hd, batch, n_ctx).numel(), dtype=torch.uint8, device="cuda")
+    want, got = (torch.zeros(batch, n_head, hd, dtype=torch.float16, device="cuda") for _ in range(2))
+
+    def call(cache, out):
+        ops.attn_prefill_q4(q, k, v, cache, out, n_head, n_kv, hd, n_ctx, past, batch, 0.0884, ops.FUSE_ALL, (0, hd, 5e5, None), ws)
+
+    a, b = base.clone(), base.clone()
+    call(a, want)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(b, got)
+    for _ in range(3):
+        b.copy_(base)
+        got.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------- large caches, odd positions
+def test_offsets_beyond_two_gigabytes(ops):
+    n_kv, hd, n_ctx, n_head = 8, 128, 2_000_016, 8
+    assert ops.kv_q4_bytes(n_kv, hd, n_ctx) > 2 ** 31
+    cache = ops.KVCacheQ4(1, n_kv, n_ctx, hd).layer(0)
+    rng = np.random.default_rng(230)
+    n = 40
+    k, v = rows(rng, n, n_kv, hd), rows(rng, n, n_kv, hd)
+    ops.kv_store_q4_batch(cache, dev(k), dev(v), n_kv, hd, n_ctx, n_ctx - n, n)
+    kh, vh = (torch.zeros(n_kv, n, hd, dtype=torch.float16, device="cuda") for _ in range(2))
+    ops.kv_load_q4(cache, kh, vh, n_kv, hd, n_ctx, n_ctx - n, n)
+    vals = [ref.values(*ref.quantise(np.transpose(x, (1, 0, 2)))) for x in (k, v)]
+    for g, w in zip((kh, vh), vals):
+        assert (np.abs(g.float().cpu().numpy() - w) <= 2.0 ** -11 * (1 + 2.0 ** -11) * np.abs(w) + 2.0 ** -25).all()
+    assert not cache[:, : (n_ctx - n) // 16].any()
+    # all other rows are zero: their scores are 0 and their values add nothing
+    q = rng.standard_normal((n_head, hd)).astype(np.float32)
+    out = torch.empty(n_head, hd, device="cuda")
+    scale = 0.3
+    ops.attn_decode_q4(dev(q), None, None, cache, out, n_head, n_kv, hd, n_ctx, dpos(n_ctx - 1), scale, ops.FUSE_NONE)
+    s = np.einsum("hd,hnd->hn", q.astype(np.float64), vals[0]) * np.float32(scale)
+    want = np.einsum("hn,hnd->hd", np.exp(s), vals[1]) / (np.exp(s).sum(-1) + n_ctx - n)[:, None]
+    most = np.einsum("hd,hnd->hn", np.abs(q), np.abs(vals[0])).max()
+    err = np.abs(out.cpu().numpy() - want)
+    # the weights of the 40 rows among two million: the bound scales with the largest output instead of the largest value
+    assert err.max() <= (2 * (2.0 ** -20 * scale * most + 2.0 ** -21) + 2.0 ** -20) * np.abs(want).max() * 4, (err.max(), np.abs(want).max())
+
+
+def test_positions_outside_the_cache(ops):
+    rng = np.random.default_rng(231)
+    n_head, n_kv, hd, n_ctx = 4, 2, 64, 50
+    host = filled(rng, n_kv, hd, n_ctx, n_ctx)
+    q = dev(rng.standard_normal((n_head, hd)).astype(np.float32))
+    outs = []
+    for p in (n_ctx - 1, n_ctx, n_ctx + 1000, 2 ** 31 - 1):
+        cache, out = dev(host), torch.empty(n_head, hd, device="cuda")
+        ops.attn_decode_q4(q, None, None, cache, out, n_head, n_kv, hd, n_ctx, dpos(p), 0.125, ops.FUSE_NONE)
+        outs.append(out)
+        assert np.array_equal(cache.cpu().numpy(), host)
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+def test_more_workspaces_than_counter_slots(ops):
+    rng = np.random.default_rng(232)
+    n_head, n_kv, hd, n = 8, 1, 128, 5000
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    cache = ops.KVCacheQ4(1, n_kv, n, hd).layer(0)
+    ops.kv_store_q4_batch(cache, *(torch.randn(n, n_kv, hd, device="cuda", generator=gen) for _ in range(2)), n_kv, hd, n, 0, n)
+    q = torch.randn(n_head, hd, device="cuda", generator=gen)
+    pos, size = dpos(n - 1), ops.decode_q4_workspace(n_head, n_kv, hd).numel()
+    ws = [torch.empty(size, dtype=torch.uint8, device="cuda").fill_(255) for _ in range(70)]
+    out = torch.empty(70, n_head, hd, device="cuda")
+    for i in range(70):
+        ops.attn_decode_q4(q, None, None, cache, out[i], n_head, n_kv, hd, n, pos, 0.0884, ops.FUSE_NONE, None, ws[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(out[i], out[0]) for i in range(70))
+
+
+def test_refusals(ops):
+    from orin_llm_b200 import capi
+    L = capi.lib()
+    t = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    p = t.data_ptr()
+    s = torch.cuda.current_stream().cuda_stream
+    A, U, W = capi.ERR_ARG, capi.ERR_UNSUPPORTED, capi.ERR_WORKSPACE
+
+    def store(c=p, k=p, v=p, heads=2, hd=128, n_ctx=64, base=0, batch=1, d=None):
+        return L.oattn_kv_store_q4(c, k, v, heads, hd, n_ctx, base, batch, d, s)
+    assert [store(c=None), store(k=None), store(heads=0), store(n_ctx=0), store(batch=0), store(base=-1), store(base=64), store(base=1, batch=64),
+            store(c=p + 8), store(k=p + 4), store(d=p, batch=2), store(base=2 ** 31 - 1, batch=2)] == [A] * 12
+    assert [store(hd=96), store(hd=0), store(n_ctx=(1 << 30) + 1)] == [U] * 3
+
+    def load(c=p, k=p, v=p, heads=2, hd=128, n_ctx=64, base=0, n=1, dc=1, db=0):
+        return L.oattn_kv_load_q4(c, k, v, heads, hd, n_ctx, base, n, dc, db, s)
+    assert [load(c=None), load(k=None), load(n=0), load(base=64), load(base=-1), load(base=60, n=5, dc=5), load(n=2), load(db=1), load(db=-1), load(dc=0),
+            load(c=p + 4), load(v=p + 2)] == [A] * 12
+    assert load(hd=32) == U
+
+    def shift(c=p, layers=1, n_kv=2, hd=128, n_ctx=64, keep=0, sh=1):
+        return L.oattn_kv_shift_q4(c, layers, n_kv, hd, n_ctx, keep, sh, s)
+    assert [shift(c=None), shift(layers=0), shift(n_kv=0), shift(keep=-1), shift(sh=0), shift(keep=64), shift(keep=60, sh=5), shift(c=p + 1)] == [A] * 8
+    assert [shift(hd=256), shift(layers=40000)] == [U] * 2
+
+    rp = capi.RopeParams(1, 128, 1e6, 0)
+
+    def decode(q=p, k=p, v=p, c=p, o=p, nh=8, nkv=2, hd=128, n_ctx=64, d=p, sc=0.1, fuse=7, rope=rp, ext=None, w=p, wb=1 << 20):
+        return L.oattn_decode_q4(q, k, v, c, o, nh, nkv, hd, n_ctx, d, sc, fuse, rope, ext, w, wb, s)
+    assert [decode(q=None), decode(k=None), decode(c=None), decode(o=None), decode(d=None), decode(sc=0.0), decode(sc=float("nan")), decode(fuse=8),
+            decode(fuse=2), decode(rope=None), decode(q=p + 4), decode(o=p + 8), decode(n_ctx=0), decode(nkv=0)] == [A] * 14
+    assert [decode(hd=80), decode(nh=7), decode(nh=34, nkv=2), decode(rope=capi.RopeParams(1, 130, 1e6, 0))] == [U] * 4
+    assert [decode(w=None), decode(w=p + 128), decode(wb=1000)] == [W] * 3
+    ext = capi.Ext()
+    ext.bias_k = p
+    assert decode(fuse=0, ext=ext) == A                                # a bias of a row that is not appended
+    ext = capi.Ext()
+    ext.out_mmq = p
+    assert decode(ext=ext) == U                                        # the prefill form
+
+    need = L.oattn_prefill_q4_workspace_bytes(8, 2, 128, 4, 20)
+
+    def prefill(q=p, k=p, v=p, c=p, o=p, h=None, nh=8, nkv=2, hd=128, n_ctx=64, past=16, batch=4, sc=0.1, fuse=7, rope=rp, ext=None, w=p, wb=1 << 20):
+        return L.oattn_prefill_q4(q, k, v, c, o, h, nh, nkv, hd, n_ctx, past, batch, sc, fuse, rope, ext, w, wb, s)
+    assert [prefill(q=None), prefill(v=None), prefill(c=None), prefill(o=None), prefill(h=p), prefill(past=61), prefill(past=-1), prefill(batch=0),
+            prefill(sc=-1.0), prefill(fuse=16), prefill(fuse=3), prefill(q=p + 4), prefill(o=None, h=p + 2), prefill(past=2 ** 31 - 2)] == [A] * 14
+    assert [prefill(hd=96), prefill(nh=9)] == [U] * 2
+    assert [prefill(w=None), prefill(w=p + 64), prefill(wb=need - 1)] == [W] * 3
+    torch.cuda.synchronize()
+    assert not t.any()                                                 # nothing was written
+
+    # what only the Python layer can see
+    c = ops.KVCacheQ4(1, 2, 64, 128).layer(0)
+    x = torch.zeros(1, 2, 128, device="cuda")
+    with pytest.raises(ValueError, match="k:"):
+        ops.kv_store_q4_batch(c, x.cpu(), x, 2, 128, 64, 0, 1)
+    with pytest.raises(ValueError, match="float32"):
+        ops.kv_store_q4_batch(c, x.half(), x, 2, 128, 64, 0, 1)
+    with pytest.raises(ValueError, match="at least"):
+        ops.kv_store_q4_batch(c, x, x, 2, 128, 64, 0, 2)
+    with pytest.raises(ValueError, match="not contiguous"):
+        ops.kv_store_q4_ind(c, torch.zeros(128, 2, device="cuda").t(), x, 2, 128, 64, dpos(0))
+    with pytest.raises(ValueError, match="int32"):
+        ops.kv_store_q4_ind(c, x, x, 2, 128, 64, torch.zeros(1, dtype=torch.int64, device="cuda"))
+    with pytest.raises(capi.AttnError):
+        ops.kv_store_q4_batch(c, x, x, 2, 128, 64, 64, 1)
+    with pytest.raises(TypeError, match="out"):
+        ops.attn_decode_q4(x, x, x, c, None, 2, 2, 128, 64, dpos(0), 0.1, ops.FUSE_KV_APPEND)
+    with pytest.raises(ValueError, match="kc"):
+        ops.kv_load_q4(c, x.half(), torch.zeros(2, 9, 128, dtype=torch.float16, device="cuda"), 2, 128, 64, 0, 9)
+    with pytest.raises(ValueError, match="unknown extension"):
+        ops.attn_decode_q4(x, x, x, c, x.clone(), 2, 2, 128, 64, dpos(0), 0.1, ops.FUSE_KV_APPEND, ext=dict(nonsense=1))
