@@ -48,6 +48,38 @@ def build_host(force=False):
     return HOST_LIB
 
 
+BINDING_LIB = os.path.join(LIBDIR, "_q4_binding.so")
+BINDING_SRC = os.path.join(HERE, "host", "torch_binding.cpp")
+
+
+def build_binding(force=False):
+    """The torch binding of the 4-bit cache's calls (host/torch_binding.cpp), linked against the C-ABI library."""
+    import sysconfig
+
+    import torch
+    build(force=False)
+    stamp = "%s %s" % (torch.__version__, sys.version.split()[0])       # it is bound to both
+    stamp_file = BINDING_LIB + ".for"
+    deps = [BINDING_SRC, os.path.join(HERE, "..", "include", "orin_attn_b200.h")]
+    if (not force and os.path.exists(BINDING_LIB) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp
+            and all(os.path.getmtime(d) <= os.path.getmtime(BINDING_LIB) for d in deps)):
+        return BINDING_LIB
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-o", BINDING_LIB, BINDING_SRC,
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+           "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
+           "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+           "-L" + LIBDIR, "-lorin_attn_b200", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
+    with open(stamp_file, "w") as f:
+        f.write(stamp)
+    return BINDING_LIB
+
+
 def needs_build():
     if not os.path.exists(LIB):
         return True
@@ -73,3 +105,4 @@ def build(force=False, verbose=False):
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
     print(build_host(force="--force" in sys.argv))
+    print(build_binding(force="--force" in sys.argv))

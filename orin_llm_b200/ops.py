@@ -7,6 +7,7 @@ torch is used only for device memory and streams.  There is no CPU implementatio
 """
 import ctypes
 import math
+import os
 
 import torch
 
@@ -317,34 +318,28 @@ class KVCache:
 # The counterparts of kv_store_*, kv_shift, attn_decode and attn_prefill over a cache of 4.5 bits a value (format in
 # include/orin_attn_b200.h), and its read-back.  No counterpart in the reference.
 
-def _q4_check(dev, name, t, dtype, numel):
-    """The checks the C entry cannot make: a contiguous tensor of that type and size on CUDA device `dev`; -> its address."""
-    try:
-        if t.dtype is dtype and t.numel() >= numel and t.is_contiguous() and t.get_device() == dev:
-            return t.data_ptr()
-    except AttributeError:
-        raise TypeError("%s: a tensor is needed, got %s" % (name, type(t).__name__)) from None
-    if t.dtype is not dtype or t.numel() < numel or not t.is_contiguous():
-        raise ValueError("%s: a contiguous %s tensor of at least %d elements is needed, got %s %s%s" % (
-            name, dtype, numel, t.dtype, list(t.shape), "" if t.is_contiguous() else ", not contiguous"))
-    raise ValueError("%s: on %s, the cache on device %d" % (name, t.device, dev))
+_binding = None
 
 
-def _q4_cache(cache, layers, n_kv, head_dim, n_ctx):
-    """Checks a cache of `layers` layers; -> its device, which has to be the current one, and its address."""
-    nbytes = kv_q4_bytes(n_kv, head_dim, n_ctx)
-    if nbytes == 0 or layers <= 0:
-        raise capi.AttnError(capi.ERR_UNSUPPORTED, "4-bit cache: head_dim 64 or 128, at least one head and one position")
-    dev = cache.get_device() if isinstance(cache, torch.Tensor) else -1
-    ptr = _q4_check(dev, "cache", cache, torch.uint8, layers * nbytes)
-    if dev < 0 or dev != torch._C._cuda_getDevice():
-        raise ValueError("cache: on %s, not on the current CUDA device" % cache.device)
-    return dev, ptr
+def _q4():
+    """The module that checks the tensors and makes the C calls (host/torch_binding.cpp); built with the library, or on first use."""
+    global _binding
+    if _binding is None:
+        import importlib.util
+
+        from . import build
+        capi.lib()
+        path = build.BINDING_LIB if os.path.exists(build.BINDING_LIB) else build.build_binding()
+        spec = importlib.util.spec_from_file_location("_q4_binding", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _binding = module
+    return _binding
 
 
-def _q4_stream(dev):
-    s = _state["stream"]
-    return torch._C._cuda_getCurrentRawStream(dev) if s is None else s
+def _ext_address(ext):
+    ref, keep = _ext_params(ext)
+    return (None if ref is None else ctypes.addressof(keep)), keep
 
 
 def kv_q4_bytes(n_kv, head_dim, n_ctx):
@@ -356,36 +351,26 @@ def kv_q4_bytes(n_kv, head_dim, n_ctx):
 
 def kv_store_q4_batch(cache, k, v, heads, head_dim, n_ctx, pos_base, batch):
     """kv_store_batch into a 4-bit cache: k, v [batch][heads][head_dim] fp32 at positions pos_base + b."""
-    dev, cp = _q4_cache(cache, 1, heads, head_dim, n_ctx)
-    n = batch * heads * head_dim
-    kp, vp = _q4_check(dev, "k", k, torch.float32, n), _q4_check(dev, "v", v, torch.float32, n)
-    capi.check(capi.lib().oattn_kv_store_q4(cp, kp, vp, heads, head_dim, n_ctx, pos_base, batch, None, _q4_stream(dev)))
+    capi.check(_q4().kv_store_q4(cache, k, v, heads, head_dim, n_ctx, pos_base, batch, None, _state["stream"]))
 
 
 def kv_store_q4_ind(cache, k, v, heads, head_dim, n_ctx, d_pos):
     """kv_store_ind into a 4-bit cache: one row at *d_pos."""
-    dev, cp = _q4_cache(cache, 1, heads, head_dim, n_ctx)
-    n = heads * head_dim
-    kp, vp = _q4_check(dev, "k", k, torch.float32, n), _q4_check(dev, "v", v, torch.float32, n)
-    pp = _q4_check(dev, "d_pos", d_pos, torch.int32, 1)
-    capi.check(capi.lib().oattn_kv_store_q4(cp, kp, vp, heads, head_dim, n_ctx, 0, 1, pp, _q4_stream(dev)))
+    if d_pos is None:
+        raise TypeError("d_pos: a tensor is needed, got NoneType")
+    capi.check(_q4().kv_store_q4(cache, k, v, heads, head_dim, n_ctx, 0, 1, d_pos, _state["stream"]))
 
 
 def kv_load_q4(cache, kc, vc, heads, head_dim, n_ctx, row_base, rows, dst_ctx=None, dst_base=0):
     """Rows [row_base, row_base + rows) of a 4-bit cache as fp16, into kc, vc [heads][dst_ctx][head_dim] from row dst_base
     on (default: a block of exactly these rows)."""
-    if dst_ctx is None:
-        dst_ctx = rows
-    dev, cp = _q4_cache(cache, 1, heads, head_dim, n_ctx)
-    n = heads * dst_ctx * head_dim
-    kp, vp = _q4_check(dev, "kc", kc, torch.float16, n), _q4_check(dev, "vc", vc, torch.float16, n)
-    capi.check(capi.lib().oattn_kv_load_q4(cp, kp, vp, heads, head_dim, n_ctx, row_base, rows, dst_ctx, dst_base, _q4_stream(dev)))
+    capi.check(_q4().kv_load_q4(cache, kc, vc, heads, head_dim, n_ctx, row_base, rows, rows if dst_ctx is None else dst_ctx, dst_base,
+                                _state["stream"]))
 
 
 def kv_shift_q4(cache, n_layer, n_kv, head_dim, n_ctx, n_keep, shift):
     """kv_shift on the 4-bit cache of n_layer layers, in place."""
-    dev, cp = _q4_cache(cache, n_layer, n_kv, head_dim, n_ctx)
-    capi.check(capi.lib().oattn_kv_shift_q4(cp, n_layer, n_kv, head_dim, n_ctx, n_keep, shift, _q4_stream(dev)))
+    capi.check(_q4().kv_shift_q4(cache, n_layer, n_kv, head_dim, n_ctx, n_keep, shift, _state["stream"]))
 
 
 def decode_q4_workspace(n_head, n_kv, head_dim):
@@ -404,59 +389,38 @@ def decode_q4_workspace(n_head, n_kv, head_dim):
 def prefill_q4_workspace(n_head, n_kv, head_dim, batch, rows):
     """Scratch for attn_prefill_q4 calls with n_past + batch <= rows; it serves every layer.  A block that became too small is
     kept: work on a stream torch does not know of, or a captured graph, may still be using it."""
-    key = (n_head, n_kv, head_dim, torch.cuda.current_device())
-    blocks = _state["prefill_q4_ws"].setdefault(key, [])
+    key = (n_head, n_kv, head_dim, torch._C._cuda_getDevice())
+    have = _state["prefill_q4_ws"].setdefault(key, [])           # [(batch, rows, block)], the newest last
+    if have and batch <= have[-1][0] and rows <= have[-1][1]:
+        return have[-1][2]
+    if have:
+        batch, rows = max(batch, have[-1][0]), max(rows, 2 * have[-1][1] if rows > have[-1][1] else have[-1][1])
     nbytes = capi.lib().oattn_prefill_q4_workspace_bytes(n_head, n_kv, head_dim, batch, rows)
     if nbytes == 0:
         raise capi.AttnError(capi.ERR_UNSUPPORTED, "prefill shape not supported")
-    if not blocks or blocks[-1].numel() < nbytes:
-        grown = max(nbytes, 2 * blocks[-1].numel()) if blocks else nbytes
-        blocks.append(torch.empty(grown, dtype=torch.uint8, device="cuda"))
-    return blocks[-1]
+    have.append((batch, rows, torch.empty(nbytes, dtype=torch.uint8, device="cuda")))
+    return have[-1][2]
 
 
 def attn_decode_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, d_pos, scale, fuse=FUSE_ALL, rope=None,
                    workspace=None, ext=None):
     """attn_decode over one layer of a 4-bit cache, the new row quantised and appended in the same launch."""
-    dev, cp = _q4_cache(cache, 1, n_kv, head_dim, n_ctx)
-    qp = _q4_check(dev, "q", q, torch.float32, n_head * head_dim)
-    kp = vp = op = None
-    if fuse & FUSE_KV_APPEND:
-        kp = _q4_check(dev, "k_new", k_new, torch.float32, n_kv * head_dim)
-        vp = _q4_check(dev, "v_new", v_new, torch.float32, n_kv * head_dim)
-    if out is not None or not ext or ext.get("out_qs") is None:
-        op = _q4_check(dev, "out", out, torch.float32, n_head * head_dim)
-    pp = _q4_check(dev, "d_pos", d_pos, torch.int32, 1)
     ws = workspace if workspace is not None else decode_q4_workspace(n_head, n_kv, head_dim)
-    wp = _q4_check(dev, "workspace", ws, torch.uint8, 0)
-    ref, keep = _rope_params(rope)
-    eref, ekeep = _ext_params(ext)
-    capi.check(capi.lib().oattn_decode_q4(qp, kp, vp, cp, op, n_head, n_kv, head_dim, n_ctx, pp, scale, fuse, ref, eref, wp,
-                                          ws.numel(), _q4_stream(dev)))
-    del keep, ekeep
+    ea, keep = _ext_address(ext) if ext else (None, None)
+    capi.check(_q4().decode_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, d_pos, scale, fuse, rope, ea, ws,
+                               _state["stream"]))
+    del keep
 
 
 def attn_prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse=FUSE_ALL, rope=None,
                     workspace=None, ext=None):
     """attn_prefill over one layer of a 4-bit cache, the chunk's rows quantised and appended first.  out: fp32 or fp16
     [batch][n_head][head_dim] (the attention runs on fp16 operands either way)."""
-    dev, cp = _q4_cache(cache, 1, n_kv, head_dim, n_ctx)
-    qp = _q4_check(dev, "q", q, torch.float32, batch * n_head * head_dim)
-    kp = vp = op = hp = None
-    if fuse & FUSE_KV_APPEND:
-        kp = _q4_check(dev, "k_new", k_new, torch.float32, batch * n_kv * head_dim)
-        vp = _q4_check(dev, "v_new", v_new, torch.float32, batch * n_kv * head_dim)
-    if isinstance(out, torch.Tensor) and out.dtype is torch.float16:
-        hp = _q4_check(dev, "out", out, torch.float16, batch * n_head * head_dim)
-    elif out is not None or not ext or ext.get("out_mmq") is None:
-        op = _q4_check(dev, "out", out, torch.float32, batch * n_head * head_dim)
     ws = workspace if workspace is not None else prefill_q4_workspace(n_head, n_kv, head_dim, batch, max(n_ctx, batch))
-    wp = _q4_check(dev, "workspace", ws, torch.uint8, 0)
-    ref, keep = _rope_params(rope)
-    eref, ekeep = _ext_params(ext)
-    capi.check(capi.lib().oattn_prefill_q4(qp, kp, vp, cp, op, hp, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse, ref,
-                                           eref, wp, ws.numel(), _q4_stream(dev)))
-    del keep, ekeep
+    ea, keep = _ext_address(ext) if ext else (None, None)
+    capi.check(_q4().prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse, rope, ea, ws,
+                                _state["stream"]))
+    del keep
 
 
 class KVCacheQ4:
