@@ -602,8 +602,8 @@ cudaError_t decode_q4_set_attributes() {
 
 cudaError_t launch_decode_q4(const DecodeQ4Args& a, int head_dim, cudaStream_t stream, unsigned long long* launches) {
     const dim3 grid(a.n_splits * a.head_blocks, a.n_kv);
-    const cudaError_t e = head_dim == 128 ? launch_dependent(decode_q4_kernel<128>, grid, kThreads, Q4Smem<128>::TOTAL, stream, a.overlap, a)
-                                          : launch_dependent(decode_q4_kernel<64>, grid, kThreads, Q4Smem<64>::TOTAL, stream, a.overlap, a);
+    const cudaError_t e = head_dim == 128 ? launch_dependent(decode_q4_kernel<128>, grid, kThreads, Q4Smem<128>::TOTAL, stream, 1, a)
+                                          : launch_dependent(decode_q4_kernel<64>, grid, kThreads, Q4Smem<64>::TOTAL, stream, 1, a);
     if (launches) *launches += 1;
     return e;
 }

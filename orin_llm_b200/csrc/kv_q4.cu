@@ -38,6 +38,8 @@ __global__ void __launch_bounds__(kStoreThreads, 5) kv_store_q4_kernel(uint8_t* 
     constexpr int LPR = 4 * F::NG;                        // lanes of a row
     __shared__ __align__(16) uint8_t s_blk[F::BLOCK];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_trigger();
+    pdl_wait();
     const int head = blockIdx.x % heads;                  // the heads of a token lie next to each other in k and v
     int first = pos_base;
     if (d_pos) {
@@ -216,6 +218,8 @@ __global__ void __launch_bounds__(32 * kLoadWarps) kv_load_q4_kernel(const uint8
                                                                      int n_ctx, int row_base, int rows, int dst_ctx, int dst_base) {
     __shared__ __align__(16) uint8_t s_v[kLoadWarps][16 * kVStride<HD>];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_trigger();
+    pdl_wait();
     const int b0 = row_base >> 4, nb = ((row_base + rows - 1) >> 4) - b0 + 1;
     const long long job = (long long)blockIdx.x * kLoadWarps + warp;
     if (job >= (long long)heads * nb) return;
@@ -250,6 +254,8 @@ __global__ void __launch_bounds__(kShiftThreads) kv_shift_q4_kernel(uint8_t* cac
     using F = Q4<HD>;
     using W = ShiftWindow<HD>;
     extern __shared__ __align__(16) uint8_t smem[];       // kShiftWindows windows
+    pdl_trigger();
+    pdl_wait();
     const bool is_v = blockIdx.x >= F::NG;
     const int h = blockIdx.x % F::NG;                      // which 32 bytes of a K row, which 512 of V; group of the scales
     const int warp = threadIdx.x >> 5, c = threadIdx.x & 31;
@@ -520,29 +526,29 @@ cudaError_t kv_q4_set_attributes() {
 cudaError_t launch_kv_store_q4(uint8_t* cache, const float* k, const float* v, int heads, int head_dim, int n_ctx, int pos_base,
                                int batch, const int* d_pos, cudaStream_t stream, unsigned long long* launches) {
     const dim3 grid((unsigned)heads * (d_pos ? 1 : ((pos_base + batch - 1) >> 4) - (pos_base >> 4) + 1));
-    if (head_dim == 128) kv_store_q4_kernel<128><<<grid, kStoreThreads, 0, stream>>>(cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
-    else                 kv_store_q4_kernel<64><<<grid, kStoreThreads, 0, stream>>>(cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
+    const cudaError_t e = head_dim == 128 ? launch_dependent(kv_store_q4_kernel<128>, grid, kStoreThreads, 0, stream, 1, cache, k, v, heads, n_ctx, pos_base, batch, d_pos)
+                                          : launch_dependent(kv_store_q4_kernel<64>, grid, kStoreThreads, 0, stream, 1, cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
     if (launches) *launches += 1;
-    return cudaGetLastError();
+    return e;
 }
 
 cudaError_t launch_kv_load_q4(const uint8_t* cache, uint16_t* kc, uint16_t* vc, int heads, int head_dim, int n_ctx, int row_base,
                               int rows, int dst_ctx, int dst_base, cudaStream_t stream, unsigned long long* launches) {
     const long long jobs = (long long)heads * (((row_base + rows - 1) >> 4) - (row_base >> 4) + 1);
     const dim3 grid((unsigned)((jobs + kLoadWarps - 1) / kLoadWarps));
-    if (head_dim == 128) kv_load_q4_kernel<128><<<grid, 32 * kLoadWarps, 0, stream>>>(cache, kc, vc, heads, n_ctx, row_base, rows, dst_ctx, dst_base);
-    else                 kv_load_q4_kernel<64><<<grid, 32 * kLoadWarps, 0, stream>>>(cache, kc, vc, heads, n_ctx, row_base, rows, dst_ctx, dst_base);
+    const cudaError_t e = head_dim == 128 ? launch_dependent(kv_load_q4_kernel<128>, grid, 32 * kLoadWarps, 0, stream, 1, cache, kc, vc, heads, n_ctx, row_base, rows, dst_ctx, dst_base)
+                                          : launch_dependent(kv_load_q4_kernel<64>, grid, 32 * kLoadWarps, 0, stream, 1, cache, kc, vc, heads, n_ctx, row_base, rows, dst_ctx, dst_base);
     if (launches) *launches += 1;
-    return cudaGetLastError();
+    return e;
 }
 
 cudaError_t launch_kv_shift_q4(uint8_t* cache, int n_layer, int n_kv, int head_dim, int n_ctx, int n_keep, int shift,
                                cudaStream_t stream, unsigned long long* launches) {
     const dim3 grid(2 * head_dim / 64, n_layer * n_kv);
-    if (head_dim == 128) kv_shift_q4_kernel<128><<<grid, kShiftThreads, shift_smem(128), stream>>>(cache, n_ctx, n_keep, shift);
-    else                 kv_shift_q4_kernel<64><<<grid, kShiftThreads, shift_smem(64), stream>>>(cache, n_ctx, n_keep, shift);
+    const cudaError_t e = head_dim == 128 ? launch_dependent(kv_shift_q4_kernel<128>, grid, kShiftThreads, shift_smem(128), stream, 1, cache, n_ctx, n_keep, shift)
+                                          : launch_dependent(kv_shift_q4_kernel<64>, grid, kShiftThreads, shift_smem(64), stream, 1, cache, n_ctx, n_keep, shift);
     if (launches) *launches += 1;
-    return cudaGetLastError();
+    return e;
 }
 
 cudaError_t launch_prefill_q4_prologue(const KvQ4PrologueArgs& p, cudaStream_t stream, unsigned long long* launches) {
