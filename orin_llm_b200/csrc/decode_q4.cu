@@ -34,10 +34,8 @@ struct Q4Smem {
     static constexpr int RING = kWarps * kTurns * 2 * BLOCK;
     static constexpr int QF_OFF = RING;                                // q fragments [HD/16 steps][32 lanes][4 words]
     static constexpr int QF_BYTES = HD / 16 * 512;
-    static constexpr int IN_OFF = QF_OFF + QF_BYTES;                   // fp32 rows: q [8], k_new, v_new
-    static constexpr int CS_OFF = IN_OFF + 10 * HD * 4;                // cos, sin of q's angles [2][HD/2] fp32
-    static constexpr int CD_OFF = CS_OFF + HD * 4;                     // the same for k_new in double
-    static constexpr int NEW_OFF = CD_OFF + HD * 8;                    // codes of the new row per lane: [2][32] u32, scales [2][2] u32
+    static constexpr int IN_OFF = QF_OFF + QF_BYTES;                   // an fp32 row per warp
+    static constexpr int NEW_OFF = IN_OFF + kWarps * HD * 4;           // codes of the new row per lane: [2][32] u32, scales [2][2] u32
     static constexpr int QS_OFF = NEW_OFF + 2 * 32 * 4 + 32;           // per head: group sums of q [8][2], unit [8]
     static constexpr int TOTAL = QS_OFF + 8 * 2 * 4 + 8 * 4;
     // merge buffers over the ring once it has drained: [warps][8 rows][HD + 8] fp32, then (m, l) [warps][8][2]
@@ -111,33 +109,30 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     const int head0 = kvh * GA + hb * p.heads_per_cta;
     const int G = min(p.heads_per_cta, GA - hb * p.heads_per_cta);
 
-    // Inputs of the step, one or two float4 pieces per thread (8 q rows of 128; k_new and v_new by the first threads), all issued
-    // together and, where the order against preceding kernels allows it, along with the position word.
-    constexpr int C4 = HD / 4;
+    // Inputs of the step: warp h has the row of head h, the last two warps the new rows of V and K as well, a lane EPL
+    // consecutive dims.  All are issued together and, where the order against preceding kernels allows it, along with the
+    // position word; from there to the barrier in front of the loop a warp waits for nobody.
+    static_assert(kWarps == 8, "one warp per head");
+    constexpr int E = F::EPL, kWarpK = kWarps - 1, kWarpV = kWarps - 2;
     const bool append = (p.fuse & 4) != 0;
-    constexpr int NQ = (8 * C4 + kThreads - 1) / kThreads;
-    float4 in_q[NQ], in_kv;
-    auto load_inputs = [&]() {
+    float in_q[E], in_kv[E];
+    auto load_lane = [&](float (&x)[E], const float* src, const float* bias, size_t row) {
+        const size_t at = row * HD + E * lane;
+        if constexpr (E == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src + at);
+            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else {
+            const float2 v = *reinterpret_cast<const float2*>(src + at);
+            x[0] = v.x; x[1] = v.y;
+        }
+        if (bias) {
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int piece = tid + i * kThreads;
-            if (piece >= G * C4) continue;
-            const size_t at = (size_t)head0 * HD + piece * 4;
-            in_q[i] = *reinterpret_cast<const float4*>(p.q + at);
-            if (p.pre.bias_q) {
-                const float4 b = *reinterpret_cast<const float4*>(p.pre.bias_q + at);
-                in_q[i].x += b.x; in_q[i].y += b.y; in_q[i].z += b.z; in_q[i].w += b.w;
-            }
+            for (int e = 0; e < E; ++e) x[e] += bias[at + e];
         }
-        if (append && tid < 2 * C4) {
-            const size_t at = (size_t)kvh * HD + (tid % C4) * 4;
-            in_kv = *reinterpret_cast<const float4*>((tid < C4 ? p.k_new : p.v_new) + at);
-            const float* bias = tid < C4 ? p.pre.bias_k : p.pre.bias_v;
-            if (bias) {
-                const float4 b = *reinterpret_cast<const float4*>(bias + at);
-                in_kv.x += b.x; in_kv.y += b.y; in_kv.z += b.z; in_kv.w += b.w;
-            }
-        }
+    };
+    auto load_inputs = [&]() {
+        if (warp < G) load_lane(in_q, p.q, p.pre.bias_q, (size_t)head0 + warp);
+        if (append && warp >= kWarpV) load_lane(in_kv, warp == kWarpK ? p.k_new : p.v_new, warp == kWarpK ? p.pre.bias_k : p.pre.bias_v, (size_t)kvh);
     };
 
     pdl_trigger();
@@ -191,122 +186,124 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     }
 
     // ---- prologue -----------------------------------------------------------------------------------------------
-    float* s_cos = reinterpret_cast<float*>(smem + L::CS_OFF);
-    float* s_sin = s_cos + HD / 2;
-    double* s_cd = reinterpret_cast<double*>(smem + L::CD_OFF);
-    double* s_sd = s_cd + HD / 2;
     const bool rope_q = (p.fuse & 1) != 0, rope_k = (p.fuse & 2) != 0;
-    if (tid < HD) {
-        const int pair = tid & (HD / 2 - 1);
-        if (pair < p.rope.n_rot / 2 && (tid < HD / 2 ? rope_q : rope_k && owner)) {
-            float f = p.freq[pair];
-            if (p.rope.freq_factors) f = __fdiv_rn(f, p.rope.freq_factors[pair]);
-            if (tid < HD / 2) rope_cs(new_pos, f, s_cos[pair], s_sin[pair]);
-            else sincos((double)__fmul_rn((float)new_pos, f), &s_sd[pair], &s_cd[pair]);
+    float* s_row = reinterpret_cast<float*>(smem + L::IN_OFF) + warp * HD;       // this warp's row on its way
+    float* s_qsum = reinterpret_cast<float*>(smem + L::QS_OFF);
+    float* s_unit = s_qsum + 16;
+    uint32_t* s_new = reinterpret_cast<uint32_t*>(smem + L::NEW_OFF);
+    // angles of pairs lane, lane + 32: the fp32 product of position and frequency
+    float angle[HD / 64];
+    if (rope_q || rope_k) {
+#pragma unroll
+        for (int u = 0; u < HD / 64; ++u) {
+            const int pp = lane + 32 * u;
+            float f = pp < p.rope.n_rot / 2 ? p.freq[pp] : 0.f;
+            if (p.rope.freq_factors && pp < p.rope.n_rot / 2) f = __fdiv_rn(f, p.rope.freq_factors[pp]);
+            angle[u] = __fmul_rn((float)new_pos, f);
         }
     }
     if (p.overlap == 2) {
         pdl_wait();
         load_inputs();
     }
-    float* s_in = reinterpret_cast<float*>(smem + L::IN_OFF);
-    float* s_qsum = reinterpret_cast<float*>(smem + L::QS_OFF);
-    float* s_unit = s_qsum + 16;
-    uint32_t* s_new = reinterpret_cast<uint32_t*>(smem + L::NEW_OFF);
+    auto norm_lane = [&](float (&x)[E], const float* w) {
+        float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < NQ; ++i)
-        if (tid + i * kThreads < G * C4) *reinterpret_cast<float4*>(s_in + (tid + i * kThreads) * 4) = in_q[i];
-    if (owner && tid < 2 * C4) *reinterpret_cast<float4*>(s_in + 8 * HD + tid * 4) = in_kv;
-    __syncthreads();
-    // One warp per head.  Norm, rotation, then the power of two that brings the largest |q| to [2^13, 2^14), and the group sums.
-    for (int h = warp; h < 8; h += kWarps) {
-        float* row = s_in + h * HD;
-        if (h >= G) {
-            for (int e = lane; e < HD; e += 32) row[e] = 0.f;
-            if (lane < 2) s_qsum[h * 2 + lane] = 0.f;
-            if (lane == 0) s_unit[h] = 1.f;
-            continue;
-        }
-        if (p.pre.norm_q) {
-            const float rn = warp_row_rnorm(row, nullptr, HD, p.pre.eps, lane);
-            __syncwarp();
-            for (int e = lane; e < HD; e += 32) row[e] = row[e] * rn * p.pre.norm_q[e];
-            __syncwarp();
-        }
-        if (rope_q) {
-            for (int pp = lane; pp < p.rope.n_rot / 2; pp += 32) {
+        for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        const float rn = 1.0f / sqrtf(ss / (float)HD + p.pre.eps);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = x[e] * rn * w[E * lane + e];
+    };
+    // rotates the row through shared memory: a pair's elements may lie in any two lanes
+    auto rotate_lane = [&](float (&x)[E], bool precise) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_row[E * lane + e] = x[e];
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < HD / 64; ++u) {
+            const int pp = lane + 32 * u;
+            if (pp < p.rope.n_rot / 2) {
                 int i0, i1;
                 rope_pair_index(p.rope.rope_type, pp, p.rope.n_rot, i0, i1);
-                const float a = row[i0], b = row[i1], c = s_cos[pp], s = s_sin[pp];
-                row[i0] = a * c - b * s;
-                row[i1] = a * s + b * c;
+                if (precise) {
+                    double sn, cs;
+                    sincos((double)angle[u], &sn, &cs);
+                    const double a = s_row[i0], b = s_row[i1];
+                    s_row[i0] = (float)(a * cs - b * sn);
+                    s_row[i1] = (float)(a * sn + b * cs);
+                } else {
+                    float sn, cs;
+                    sincosf(angle[u], &sn, &cs);
+                    const float a = s_row[i0], b = s_row[i1];
+                    s_row[i0] = a * cs - b * sn;
+                    s_row[i1] = a * sn + b * cs;
+                }
             }
-            __syncwarp();
         }
-        float amax = 0.f;
-        for (int e = lane; e < HD; e += 32) amax = fmaxf(amax, fabsf(row[e]));
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = s_row[E * lane + e];
+        __syncwarp();
+    };
+    uint4* s_frag = reinterpret_cast<uint4*>(smem + L::QF_OFF);
+    if (warp < G) {
+        if (p.pre.norm_q) norm_lane(in_q, p.pre.norm_q);
+        if (rope_q) rotate_lane(in_q, false);
+        // the power of two that brings the largest |q| to [2^13, 2^14), and the group sums
+        float amax = fabsf(in_q[0]);
+#pragma unroll
+        for (int e = 1; e < E; ++e) amax = fmaxf(amax, fabsf(in_q[e]));
 #pragma unroll
         for (int off = 16; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
         int k = 13 - ((int)(__float_as_uint(amax) >> 23) - 127);
         k = amax == 0.f ? 0 : max(-100, min(100, k));
         const float up = __uint_as_float((uint32_t)(127 + k) << 23);
-        float sum[2] = {0.f, 0.f};
+        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-            const float v = row[lane + 32 * i] * up;
-            row[lane + 32 * i] = v;
-            sum[i >> 1] += v;
+        for (int e = 0; e < E; ++e) {
+            in_q[e] *= up;
+            sum += in_q[e];
+            s_row[E * lane + e] = in_q[e];
         }
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-#pragma unroll
-            for (int off = 16; off; off >>= 1) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], off);
-            if (lane == 0) s_qsum[h * 2 + g] = sum[g] * 9.5367431640625e-7f;              // 2^-20
+        for (int off = 16 / NG; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane % (32 / NG) == 0) s_qsum[warp * 2 + lane / (32 / NG)] = sum * 9.5367431640625e-7f;              // 2^-20
+        if (lane == 0) s_unit[warp] = __uint_as_float((uint32_t)(127 + 20 - k) << 23);     // back to q . k
+        __syncwarp();
+        // Fragments of this head: step 2i + o of word i takes the nibbles 0, 4 | 2, 6 (o = 0) or 1, 5 | 3, 7 (o = 1); words: row r
+        // hi, row r lo (as row r + 8), and the same for k + 8
+        if (lane < HD / 16 * 4) {
+            const int step = lane >> 2;
+            const float* row = s_row + 32 * (step >> 1) + 8 * t + (step & 1);
+            uint4 w;
+            split_half2(F2(row[0], row[4]), w.x, w.y);
+            split_half2(F2(row[2], row[6]), w.z, w.w);
+            s_frag[step * 32 + 4 * warp + t] = w;
         }
-        if (lane == 0) s_unit[h] = __uint_as_float((uint32_t)(127 + 20 - k) << 23);         // back to q . k
+        __syncwarp();
+    } else {
+        if (lane < HD / 16 * 4) s_frag[(lane >> 2) * 32 + 4 * warp + t] = make_uint4(0u, 0u, 0u, 0u);
+        if (lane < 2) s_qsum[warp * 2 + lane] = 0.f;
+        if (lane == 0) s_unit[warp] = 1.f;
     }
-    // the new row of K (warp 0) and V (warp 1): codes, into the cache and into s_new for this CTA's copy of the block
-    if (owner && warp < 2) {
-        float* row = s_in + (8 + warp) * HD;
-        if (warp == 0 && p.pre.norm_k) {
-            const float rn = warp_row_rnorm(row, nullptr, HD, p.pre.eps, lane);
-            __syncwarp();
-            for (int e = lane; e < HD; e += 32) row[e] = row[e] * rn * p.pre.norm_k[e];
-            __syncwarp();
+    // the new row of K or V: codes, into the cache and into s_new for this CTA's copy of the block
+    if (owner && warp >= kWarpV) {
+        const bool is_v = warp == kWarpV;
+        if (!is_v) {
+            if (p.pre.norm_k) norm_lane(in_kv, p.pre.norm_k);
+            if (rope_k) rotate_lane(in_kv, true);
         }
-        if (warp == 0 && rope_k) {
-            for (int pp = lane; pp < p.rope.n_rot / 2; pp += 32) {
-                int i0, i1;
-                rope_pair_index(p.rope.rope_type, pp, p.rope.n_rot, i0, i1);
-                const double a = row[i0], b = row[i1], c = s_cd[pp], s = s_sd[pp];
-                row[i0] = (float)(a * c - b * s);
-                row[i1] = (float)(a * s + b * c);
-            }
-            __syncwarp();
-        }
-        float x[F::EPL];
-#pragma unroll
-        for (int e = 0; e < F::EPL; ++e) x[e] = row[F::EPL * lane + e];
-        const Q4Scale sc = q4_scale<HD>(x, lane);
-        const uint32_t codes = q4_codes<HD>(x, sc);
-        s_new[warp * 32 + lane] = codes;
-        if (F::EPL * lane % 64 == 0) s_new[64 + warp * 2 + F::EPL * lane / 64] = q4_scale_word(sc);
+        const Q4Scale sc = q4_scale<HD>(in_kv, lane);
+        const uint32_t codes = q4_codes<HD>(in_kv, sc);
+        s_new[is_v * 32 + lane] = codes;
+        if (E * lane % 64 == 0) s_new[64 + is_v * 2 + E * lane / 64] = q4_scale_word(sc);
         if (hb == 0) {
             uint8_t* blk = cache + (size_t)(new_pos >> 4) * F::BLOCK;
-            if (warp == 0) q4_store_row<HD, false>(blk, new_pos & 15, codes, sc, lane);
-            else           q4_store_row<HD, true>(blk, new_pos & 15, codes, sc, lane);
+            if (is_v) q4_store_row<HD, true>(blk, new_pos & 15, codes, sc, lane);
+            else      q4_store_row<HD, false>(blk, new_pos & 15, codes, sc, lane);
         }
-    }
-    __syncthreads();
-    // q fragments: step 2i + o of word i takes the nibbles 0, 4 | 2, 6 (o = 0) or 1, 5 | 3, 7 (o = 1); words: row r hi, row r lo
-    // (as row r + 8), and the same for k + 8
-    for (int idx = tid; idx < HD / 16 * 32; idx += kThreads) {
-        const int step = idx >> 5, ln = idx & 31, o = step & 1;
-        const float* row = s_in + (ln >> 2) * HD + 32 * (step >> 1) + 8 * (ln & 3) + o;
-        uint4 w;
-        split_half2(F2(row[0], row[4]), w.x, w.y);
-        split_half2(F2(row[2], row[6]), w.z, w.w);
-        *reinterpret_cast<uint4*>(smem + L::QF_OFF + idx * 16) = w;
     }
     __syncthreads();
 
