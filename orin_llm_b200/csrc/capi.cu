@@ -530,6 +530,7 @@ int oattn_kv_load_q4(const void* cache, uint16_t* kc, uint16_t* vc, int heads, i
     if (rc != OATTN_OK) return rc;
     if (!kc || !vc || rows <= 0 || row_base < 0 || row_base > n_ctx - rows) return OATTN_ERR_ARG;
     if (dst_ctx <= 0 || dst_base < 0 || dst_base > dst_ctx - rows) return OATTN_ERR_ARG;
+    if ((long long)heads * (rows / 16 + 2) > 0x7fffffffLL) return OATTN_ERR_UNSUPPORTED;     // one warp per head and 16 rows
     if (((uintptr_t)kc | (uintptr_t)vc) & 15) return OATTN_ERR_ARG;    // written in 16-byte pieces
     cudaError_t e = launch_kv_load_q4(reinterpret_cast<const uint8_t*>(cache), kc, vc, heads, head_dim, n_ctx, row_base, rows,
                                       dst_ctx, dst_base, (cudaStream_t)stream, &g_launches);

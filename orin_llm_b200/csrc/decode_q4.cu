@@ -47,12 +47,28 @@ struct Q4Smem {
 struct Q4Plan {
     int blocks, per_split, active, step; // 16-row blocks in all, of one slice, slices that have any; blocks a warp takes at a time
 };
-// A warp works on pairs of blocks (half the softmax bookkeeping); while there are no more blocks than warps it takes one.
+// A warp works on pairs of blocks (half the softmax bookkeeping) where there are enough of them.  A merge across CTAs costs about
+// 2.3 us and a second level 1.5, one turn of a CTA's eight warps 0.7 (one block each) or 1.4 (two), so up to 512 rows stay in one
+// CTA (28/4 heads, 256 rows: 6.6 us against 7.8 from two CTAs), up to 4096 in 16, which merge in one level (4096 rows: 10.3
+// us against 10.7 from 32); behind that the blocks are spread evenly over all slices.
 __device__ __forceinline__ Q4Plan q4_plan(int npos, int n_splits) {
     Q4Plan s;
     s.blocks = (npos + 15) >> 4;
-    s.step = s.blocks <= n_splits * kWarps ? 1 : 2;
-    s.per_split = s.step == 1 ? kWarps : 2 * (((s.blocks + 1) / 2 + n_splits - 1) / n_splits);
+    const int even = 2 * (((s.blocks + 1) / 2 + n_splits - 1) / n_splits);           // no slice may be left without a CTA
+    s.step = 2;
+    s.per_split = even;
+    if (s.blocks <= 32) {
+        s.step = s.blocks <= kWarps ? 1 : 2;
+        s.per_split = 32;
+    } else if (s.blocks <= 16 * kWarps && s.blocks <= n_splits * kWarps) {
+        s.step = 1;
+        s.per_split = kWarps;
+    } else if (s.blocks <= 32 * kWarps) {
+        s.per_split = max(2 * kWarps, even);
+    } else if (s.blocks <= n_splits * kWarps) {
+        s.step = 1;
+        s.per_split = kWarps;
+    }
     s.active = (s.blocks + s.per_split - 1) / s.per_split;
     return s;
 }

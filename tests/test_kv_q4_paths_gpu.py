@@ -373,6 +373,27 @@ def test_positions_outside_the_cache(ops):
     assert all(torch.equal(o, outs[0]) for o in outs)
 
 
+@pytest.mark.parametrize("n_head,n_kv,hd", [(40, 40, 64), (128, 64, 128), (100, 100, 64), (160, 160, 64)])
+@pytest.mark.parametrize("length", [300, 600, 1500, 3000, 5000])
+def test_more_kv_heads_than_slices(ops, n_head, n_kv, hd, length):
+    """Many kv heads leave few slices to each: every row has to be in one of them."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    cache = ops.KVCacheQ4(1, n_kv, length, hd).layer(0)
+    k, v = (torch.randn(length, n_kv, hd, device="cuda", generator=gen) for _ in range(2))
+    ops.kv_store_q4_batch(cache, k, v, n_kv, hd, length, 0, length)
+    kh, vh = (torch.zeros(n_kv, length, hd, dtype=torch.float16, device="cuda") for _ in range(2))
+    ops.kv_load_q4(cache, kh, vh, n_kv, hd, length, 0, length)
+    q = torch.randn(n_head, hd, device="cuda", generator=gen)
+    out = torch.empty(n_head, hd, device="cuda")
+    ops.attn_decode_q4(q, None, None, cache, out, n_head, n_kv, hd, length, dpos(length - 1), 0.1, ops.FUSE_NONE)
+    qd, K, V = q.double().view(n_kv, -1, hd), kh.double(), vh.double()
+    want = torch.softmax(qd @ K.transpose(1, 2) * 0.1, -1) @ V
+    # kh and vh are the rows rounded to fp16: 2^-11 of a value, and of a score's sum of products
+    most = float((qd.abs() @ K.abs().transpose(1, 2)).max())
+    err = float((out.view_as(want) - want).abs().max())
+    assert err <= (2 * 2.0 ** -11 * 0.1 * most + 2.0 ** -11) * float(V.abs().max())
+
+
 def test_more_workspaces_than_counter_slots(ops):
     rng = np.random.default_rng(232)
     n_head, n_kv, hd, n = 8, 1, 128, 5000
