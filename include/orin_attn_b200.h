@@ -331,9 +331,11 @@ int oattn_kv_shift_q4(void* cache, int n_layer, int n_kv, int head_dim, int n_ct
 /* oattn_decode_ex on the 4-bit cache (ext may be NULL): q attends over rows 0..*d_pos; with OATTN_FUSE_KV_APPEND the new row is
  * [biased, normed, rotated,] quantised and stored at row *d_pos in the same launch.  k_new is rotated in double and rounded
  * to fp32 before it is quantised (q in fp32, as in oattn_decode).  The result has fp32 accuracy: the codes are exact, q and the
- * softmax weights enter the products as two fp16 halves.  ONE launch; oattn_set_decode_overlap applies.  The workspace rules
- * are those of oattn_decode_workspace_bytes: calls that may run at the same time, graph replays among them, need
- * workspaces of their own. */
+ * softmax weights enter the products as two fp16 halves.  A NaN in a visible row or in a query shows in the output.  ONE launch,
+ * always a programmatic dependent one (as the store, read-back and roll calls): oattn_set_decode_overlap modes 0 and 1 are the
+ * same here, mode 2 means what it says there.  *d_pos beyond the cache is taken as n_ctx - 1, below zero there is no row
+ * and the output is zero.  The workspace rules are those of oattn_decode_workspace_bytes: calls that may run at the same
+ * time, graph replays among them, need workspaces of their own. */
 size_t oattn_decode_q4_workspace_bytes(int n_head, int n_kv, int head_dim);
 int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, int n_head, int n_kv,
                     int head_dim, int n_ctx, const int* d_pos, float scale, int fuse, const oattn_rope_params* rope,

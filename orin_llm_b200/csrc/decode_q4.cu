@@ -1,18 +1,26 @@
 // Single-token decode attention over the 4-bit KV cache (format: kv_q4.cuh), split over the sequence, in ONE launch.
 //
 // The sequence of every kv head is cut into slices, one CTA of eight warps each (grid = slices x kv heads, two CTAs per SM);
-// a warp takes every eighth 16-position block of the slice and brings it to shared memory with cp.async, one contiguous
-// piece, four blocks deep, for itself alone: no barrier across warps until the end.  The grid never depends on the
+// a warp takes every eighth pair of 16-position blocks of the slice and brings it to shared memory with cp.async, one contiguous
+// piece, two pairs deep, for itself alone: no barrier across warps until the end.  The grid never depends on the
 // position, so the launch replays from a CUDA graph.  The slices are merged as in decode.cu (decode_merge.cuh).
 //
 // The codes are never turned into values.  With x = m + d * code per row and 64-dim group g,
 //     q . k  = sum_g d_g (q_g . code_g) + m_g sum(q_g)            P V = sum_k (P_k d_gk) code_k + sum_k P_k m_gk
-// so the matrix instructions (m16n8k16, fp16 in, fp32 out) take the codes as they are: a masked nibble is an fp16
-// subnormal, exactly code * 2^-24 or code * 2^-20, and the powers of two go into q and the final scale.  The left operands q and
+// so the matrix instructions (m16n8k16, fp16 in, fp32 out) take the codes as they are: a masked nibble in bits 4..7
+// is an fp16 subnormal, exactly code * 2^-20, and the powers of two go into q and the final scale.  The left operands q and
 // P d are fp32; a decode step has at most eight heads per CTA, so the other eight rows of the tile hold what the rounding of the
 // first eight to fp16 left over (x = hi + lo, 22 bits together): the result keeps fp32 accuracy and the instruction count is
-// the same.  q is scaled by a power of two per head, P d by a power of two that is lowered when a step of 2 or more is met,
+// the same.  q is scaled by a power of two per head, P d by a fixed one that a warp lowers, starting over, when its sums overflowed,
 // so that neither half leaves the fp16 range.
+//
+// What bounds it: the warp-level matrix instruction takes its scheduler 8.1 cycles and lets nothing else issue beside it (measured:
+// with 8 fp32 multiply-adds per product 16.0 cycles, with 4 logic operations 13.2), so a 16-position block costs a scheduler its
+// 32 products plus about 220 other instructions, 640 cycles; at the measured copy bandwidth the bytes would arrive in 400.  One
+// million rows of 16/2 heads: 86 us, 3.5 TB/s of cache, 0.53 of the copy bandwidth (the fp16 cache: 158 us).  Eight warps per
+// SM instead of sixteen run as fast (91 us), so latency is not the limit.  The 8-bit float form of the instruction is emulated
+// (21 cycles); the 8-bit integer form takes the same 8.1 for twice the depth, but q needs three digits, so nothing is won.
+// At a few thousand rows a call is a chain of dependent round trips: 5.3 us from launch to output in one CTA, 2.3 more for a merge.
 #include <type_traits>
 
 #include "decode_merge.cuh"

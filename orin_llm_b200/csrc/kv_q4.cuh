@@ -9,10 +9,10 @@
 //
 // The code order is the one the decode kernel's m16n8k16 products read without moving anything between lanes:
 //   K: row s at word s * HD/8; word t * HD/32 + i (t < 4: the lane's place in its quad) holds dims 32 i + 8 t + e, dim e in
-//      bits 4e..4e+3.  Masking a word (and the word shifted by 8) with 0x000F000F and 0x00F000F0 gives the four B registers
-//      of two k-steps: a nibble on its own is the fp16 subnormal code * 2^-24, in bits 4..7 it is code * 2^-20, exactly.
+//      bits 4e..4e+3.  Nibbles i and i + 4 of a word, shifted to bits 4..7 of its halves, are a B register: a pair of fp16
+//      subnormals code * 2^-20, exactly; the four pairs make two k-steps.
 //   V: a byte holds dims 2p (low half) and 2p + 1 of one row; the four bytes of a word belong to rows 2t, 2t+8, 2t+1, 2t+9 of
-//      the block, so that the same masks give the k-pairs (2t, 2t+1) and (2t+8, 2t+9).  With p = 8 j + r the word sits at
+//      the block, so that the same pairs are rows (2t, 2t+1) and (2t+8, 2t+9) of an even and an odd dim.  With p = 8 j + r the word sits at
 //      (j/4) * 512 + (4 r + t) * 16 + (j%4) * 4: lane 4r + t reads 16 bytes.  One byte belongs to one row, so appending a
 //      row never reads what its neighbours hold.
 //   scales: fp16 [16 rows][HD/64][d, m] for K, then for V.
