@@ -91,9 +91,9 @@ __device__ __forceinline__ void merge_parts(const float* o_base, const float* ml
 #pragma unroll
             for (int kk = 0; kk < KB; ++kk) {
                 RunState& r = st[k0 + kk];
-                float mx = ml[kk].x;
+                float mx = ml[kk].x;          // (over all lanes of the row: those past the parts hold -inf and need it just as well)
 #pragma unroll
-                for (int off = PASS / 2; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off, LPR));
+                for (int off = LPR / 2; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off, LPR));
                 const float m_new = fmaxf(r.M, mx);
                 const bool empty = m_new == -CUDART_INF_F;
                 const float a = (empty || r.M == -CUDART_INF_F) ? 0.f : fast_exp2((r.M - m_new) * c);

@@ -394,6 +394,29 @@ def test_more_kv_heads_than_slices(ops, n_head, n_kv, hd, length):
     assert err <= (2 * 2.0 ** -11 * 0.1 * most + 2.0 ** -11) * float(V.abs().max())
 
 
+@pytest.mark.parametrize("n_head,hd,length", [(4, 128, 40000), (16, 128, 70001), (3, 64, 40000)])
+def test_one_kv_head_merges_more_than_sixteen_groups(ops, n_head, hd, length):
+    """One kv head at a long context has 19 groups of slices, which merge in two passes: both caches."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    cache = ops.KVCacheQ4(1, 1, length, hd).layer(0)
+    k, v = (torch.randn(length, 1, hd, device="cuda", generator=gen) for _ in range(2))
+    v[..., hd // 2:] += 1.0
+    ops.kv_store_q4_batch(cache, k, v, 1, hd, length, 0, length)
+    kh, vh = (torch.zeros(1, length, hd, dtype=torch.float16, device="cuda") for _ in range(2))
+    ops.kv_load_q4(cache, kh, vh, 1, hd, length, 0, length)
+    q = torch.randn(n_head, hd, device="cuda", generator=gen).half().float()
+    qd, K, V = q.double(), kh[0].double(), vh[0].double()
+    want = torch.softmax(qd @ K.T * 0.1, -1) @ V
+    most = float((qd.abs() @ K.abs().T).max())
+    # the rows of the 4-bit cache are within 2^-11 of kh and vh; the fp16 kernel rounds its weights to fp16, 2^-11 as well
+    bound = (2 * 2.0 ** -11 * 0.1 * most + 2 * 2.0 ** -11) * float(V.abs().max())
+    out = torch.empty(n_head, hd, device="cuda")
+    ops.attn_decode_q4(q, None, None, cache, out, n_head, 1, hd, length, dpos(length - 1), 0.1, ops.FUSE_NONE)
+    assert float((out - want).abs().max()) <= bound and float((out - want).norm() / want.norm()) < 1e-3
+    ops.flash_attention_decode_ind(q, kh, vh, out, n_head, 1, hd, length, dpos(length - 1), 0.1)
+    assert float((out - want).abs().max()) <= bound and float((out - want).norm() / want.norm()) < 1e-3
+
+
 def test_more_workspaces_than_counter_slots(ops):
     rng = np.random.default_rng(232)
     n_head, n_kv, hd, n = 8, 1, 128, 5000
