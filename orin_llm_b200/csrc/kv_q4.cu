@@ -42,8 +42,7 @@ __global__ void __launch_bounds__(kStoreThreads, 5) kv_store_q4_kernel(uint8_t* 
     constexpr int LPR = 4 * F::NG;                        // lanes of a row
     __shared__ __align__(16) uint8_t s_blk[F::BLOCK];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    pdl_trigger();
-    pdl_wait();
+    pdl_wait();                                           // no early trigger: with it a read-back behind this call took 4 us longer
     const int head = blockIdx.x % heads;                  // the heads of a token lie next to each other in k and v
     int first = pos_base;
     if (d_pos) {
@@ -259,7 +258,6 @@ __global__ void __launch_bounds__(kShiftThreads) kv_shift_q4_kernel(uint8_t* cac
     using F = Q4<HD>;
     using W = ShiftWindow<HD>;
     extern __shared__ __align__(16) uint8_t smem[];       // kShiftWindows windows
-    pdl_trigger();
     pdl_wait();
     const bool is_v = blockIdx.x >= F::NG;
     const int h = blockIdx.x % F::NG;                      // which 32 bytes of a K row, which 512 of V; group of the scales
