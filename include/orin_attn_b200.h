@@ -300,7 +300,7 @@ int oattn_prefill_status(const void* workspace, int n_head, int head_dim, int ba
  * into groups of 64 dims; a group keeps an fp16 offset m and an fp16 step d, a value is m + d * code, code 0..15:
  *     m = fp16(min x)    d = fp16(max(0, (max x - m) / 15))    code = clamp(round((x - m) / d), 0, 15), 0 where d = 0,
  * each evaluated exactly and rounded once, ties to even: the bytes depend on the row alone, not on the call that wrote
- * it.  A group that holds a NaN, an infinity or a minimum beyond the fp16 range reads back as NaN.  Bytes of a block,
+ * it.  A group that holds a NaN, an infinity, or a minimum or a step beyond the fp16 range reads back as NaN.  Bytes of a block,
  * with hd = head_dim and NG = hd/64 (little endian):
  *     [0, 8 hd)       K codes: row s at 32-bit word s * hd/8; word t * hd/32 + i of a row (t < 4) holds dims
  *                     32 i + 8 t + e, dim e in bits 4e..4e+3

@@ -514,7 +514,6 @@ int oattn_kv_store_q4(void* cache, const float* k, const float* v, int heads, in
     const int rc = check_q4(cache, heads, head_dim, n_ctx);
     if (rc != OATTN_OK) return rc;
     if (!k || !v || batch <= 0) return OATTN_ERR_ARG;
-    if ((long long)heads * (batch / 16 + 2) > 0x7fffffffLL) return OATTN_ERR_UNSUPPORTED;    // one CTA per head and 16 rows
     if (((uintptr_t)k | (uintptr_t)v) & 15) return OATTN_ERR_ARG;      // read as float4
     if (d_pos && batch != 1) return OATTN_ERR_ARG;
     if (!d_pos && (pos_base < 0 || pos_base > n_ctx - batch)) return OATTN_ERR_ARG;
@@ -557,7 +556,7 @@ static void q4_head_split(int n_head, int n_kv, int& per_cta, int& blocks) {
 static DecodeWsLayout decode_q4_ws(int n_head, int n_kv, int head_dim, int sm_count) {
     int per_cta, blocks;
     q4_head_split(n_head, n_kv, per_cta, blocks);
-    return decode_ws_layout(n_kv * blocks * per_cta, n_kv * blocks, head_dim, decode_q4_num_splits(n_kv, sm_count));
+    return decode_ws_layout(n_kv * blocks * per_cta, n_kv * blocks, head_dim, decode_q4_num_splits(n_kv * blocks, sm_count));
 }
 
 size_t oattn_decode_q4_workspace_bytes(int n_head, int n_kv, int head_dim) {

@@ -611,9 +611,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
 
 } // namespace
 
-int decode_q4_num_splits(int n_kv, int sm_count) {
-    return max(1, min(DECODE_MAX_SPLITS, kCtas * sm_count / n_kv));
-}
+// One wave: kCtas per SM over the kv heads, or over their halves where a kv head's query heads take two CTAs (32/2 heads, 32768
+// rows: 14.8 us against 21.5 from two waves).
+int decode_q4_num_splits(int head_blocks, int sm_count) { return max(1, min(DECODE_MAX_SPLITS, kCtas * sm_count / head_blocks)); }
 
 cudaError_t decode_q4_set_attributes() {
     cudaError_t e = cudaFuncSetAttribute(decode_q4_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<128>::TOTAL);

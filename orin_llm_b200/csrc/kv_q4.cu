@@ -20,8 +20,9 @@ __device__ __noinline__ uint2 q4_codes16(const float* src, float m, float d, flo
     return w;
 }
 
-__device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
+// of three, NaN where any of them is
+__device__ __forceinline__ float min_nan(float a, float b, float c) { float r; asm("min.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+__device__ __forceinline__ float max_nan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 
 // ---- store --------------------------------------------------------------------------------------------------------
 // One CTA per (block of 16 positions, kv head): warps 0..3 four rows of K each, warps 4..7 four rows of V.  Eight lanes (HD 128)
@@ -43,14 +44,15 @@ __global__ void __launch_bounds__(kStoreThreads, 5) kv_store_q4_kernel(uint8_t* 
     __shared__ __align__(16) uint8_t s_blk[F::BLOCK];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();                                           // no early trigger: with it a read-back behind this call took 4 us longer
-    const int head = blockIdx.x % heads;                  // the heads of a token lie next to each other in k and v
+    const int head = blockIdx.x;                          // the heads of a token lie next to each other in k and v
     int first = pos_base;
     if (d_pos) {
         first = *d_pos;
         if (first < 0 || first >= n_ctx) return;
     }
-    const int b = (first >> 4) + blockIdx.x / heads;      // block of the sequence
+    const int b = (first >> 4) + blockIdx.y + 65535 * blockIdx.z;      // block of the sequence
     const int row0 = max(first - 16 * b, 0), row1 = min(first + batch - 16 * b, 16);     // its rows that are stored
+    if (row1 <= 0) return;                                // the grid's last plane is not full
     const bool is_v = warp >= 4;
     const int s = (warp & 3) * 4 + lane / 8, t = lane & 3, g = (lane % 8) / 4;           // HD 64: lanes with g = 1 idle
     const bool on = g < F::NG && s >= row0 && s < row1;
@@ -68,11 +70,12 @@ __global__ void __launch_bounds__(kStoreThreads, 5) kv_store_q4_kernel(uint8_t* 
     }
     float mn = x[0], mx = x[0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) { mn = min_nan(mn, x[i]); mx = max_nan(mx, x[i]); }
+    for (int i = 0; i < 16; i += 2) { mn = min_nan(mn, x[i], x[i + 1]); mx = max_nan(mx, x[i], x[i + 1]); }
 #pragma unroll
     for (int off = 1; off <= 2; off <<= 1) {
-        mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, off));
-        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float u = __shfl_xor_sync(0xffffffffu, mn, off), w = __shfl_xor_sync(0xffffffffu, mx, off);
+        mn = min_nan(mn, u, u);
+        mx = max_nan(mx, w, w);
     }
     const Q4Scale sc = q4_scale_of(mn, mx);
     const float m = __half2float(sc.m), d = __half2float(sc.d), inv = __frcp_rn(d);
@@ -531,7 +534,8 @@ cudaError_t kv_q4_set_attributes() {
 
 cudaError_t launch_kv_store_q4(uint8_t* cache, const float* k, const float* v, int heads, int head_dim, int n_ctx, int pos_base,
                                int batch, const int* d_pos, cudaStream_t stream, unsigned long long* launches) {
-    const dim3 grid((unsigned)heads * (d_pos ? 1 : ((pos_base + batch - 1) >> 4) - (pos_base >> 4) + 1));
+    const int blocks = d_pos ? 1 : ((pos_base + batch - 1) >> 4) - (pos_base >> 4) + 1;
+    const dim3 grid(heads, min(blocks, 65535), (blocks + 65534) / 65535);
     const cudaError_t e = head_dim == 128 ? launch_dependent(kv_store_q4_kernel<128>, grid, kStoreThreads, 0, stream, 1, cache, k, v, heads, n_ctx, pos_base, batch, d_pos)
                                           : launch_dependent(kv_store_q4_kernel<64>, grid, kStoreThreads, 0, stream, 1, cache, k, v, heads, n_ctx, pos_base, batch, d_pos);
     if (launches) *launches += 1;

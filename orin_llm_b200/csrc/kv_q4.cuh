@@ -51,18 +51,23 @@ __device__ __forceinline__ int q4_v_byte(int s, int D) {
 
 struct Q4Scale { __half d, m; };
 
-// (d, m) of a group with this minimum and maximum (NaN or infinite where the group has such a value).  The quotient is
-// formed in double and rounded to fp16 in one step; in fp32 one group in a few thousand would get a step that is off by an
-// fp16 ulp.
+// fp16((max - m) / 15) in one rounding, out of line: next to the midpoint of two fp16 numbers, and among the subnormal ones.
+static __device__ __noinline__ __half q4_step_exact(float mx, float m) { return __double2half(((double)mx - (double)m) / 15.0); }
+
+// (d, m) of a group with this minimum and maximum (NaN or infinite where the group has such a value).  The fp32 quotient is off
+// by at most two of its last places, so its rounding to fp16 (13 places fewer) is the exact quotient's unless it lies within
+// four of a midpoint.  Without that case one group in about 4000 would get a step that is off by an fp16 place.
 __device__ __forceinline__ Q4Scale q4_scale_of(float mn, float mx) {
     Q4Scale s;
     s.m = __float2half_rn(mn);
-    if (!(fabsf(mx) <= 3.402823466e38f) || !(fabsf(__half2float(s.m)) <= 65504.f)) {
+    const float m = __half2float(s.m);
+    if (!(fabsf(mx) <= 3.402823466e38f) || !(fabsf(m) <= 65504.f)) {
         s.d = s.m = __ushort_as_half(0x7fff);
         return s;
     }
-    const double step = ((double)mx - (double)__half2float(s.m)) / 15.0;
-    s.d = __double2half(step > 0.0 ? step : 0.0);
+    const float step = __fmul_rn(__fsub_rn(mx, m), 1.0f / 15.0f);
+    s.d = __float2half_rn(fmaxf(step, 0.f));
+    if (((__float_as_uint(step) - 0xffcu) & 0x1fffu) <= 8u || (step > 0.f && step < 6.2e-5f)) s.d = step > 0.f ? q4_step_exact(mx, m) : __ushort_as_half(0);
     return s;
 }
 
@@ -181,7 +186,7 @@ struct DecodeQ4Args {
     int8_t* out_qs = nullptr;
     float* out_scales = nullptr;
 };
-int decode_q4_num_splits(int n_kv, int sm_count);
+int decode_q4_num_splits(int head_blocks, int sm_count);
 cudaError_t decode_q4_set_attributes();
 cudaError_t launch_decode_q4(const DecodeQ4Args& a, int head_dim, cudaStream_t stream, unsigned long long* launches);
 
