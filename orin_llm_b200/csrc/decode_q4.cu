@@ -17,7 +17,7 @@
 // What bounds it: the warp-level matrix instruction takes its scheduler 8.1 cycles and lets nothing else issue beside it (measured:
 // with 8 fp32 multiply-adds per product 16.0 cycles, with 4 logic operations 13.2), so a 16-position block costs a scheduler its
 // 32 products plus about 220 other instructions, 640 cycles; at the measured copy bandwidth the bytes would arrive in 400.  One
-// million rows of 16/2 heads: 86 us, 3.5 TB/s of cache, 0.53 of the copy bandwidth (the fp16 cache: 158 us).  Eight warps per
+// million rows of 16/2 heads: 85 us, 3.55 TB/s of cache, 0.54 of the copy bandwidth (the fp16 cache: 158 us).  Eight warps per
 // SM instead of sixteen run as fast (91 us), so latency is not the limit.  The 8-bit float form of the instruction is emulated
 // (21 cycles); the 8-bit integer form takes the same 8.1 for twice the depth, but q needs three digits, so nothing is won.
 // At a few thousand rows a call is a chain of dependent round trips: 5.3 us from launch to output in one CTA, 2.3 more for a merge.
@@ -118,7 +118,21 @@ struct Nibbles {
     }
 };
 
-template <int HD>
+__device__ __forceinline__ F2 shfl_xor(F2 v, int mask) { return F2(__shfl_xor_sync(0xffffffffu, v.x(), mask), __shfl_xor_sync(0xffffffffu, v.y(), mask)); }
+
+// Transposes an 8 x 8 matrix of 16-bit values held as one row per quad of lanes.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// TURNED (at most four heads): the codes are the 16-row operand of both products -- 16 positions by 16 dims, 16 dims by 16
+// positions, the same words in the same lanes -- and the heads with their low halves its eight columns, so there are half as
+// many products.  A lane then has two heads' scores of positions r and r + 8 instead of one head's of four, and P has to be
+// transposed between the products.  32/8 heads of 128, 131072 rows: 43.8 us against 47.4; 32/8 heads of 64, 32001 rows: 12.4
+// against 12.7; below a few thousand rows no difference.
+template <int HD, bool TURNED>
 __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid_constant__ DecodeQ4Args p) {
     using F = Q4<HD>;
     using L = Q4Smem<HD>;
@@ -304,11 +318,23 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
             uint4 w;
             split_half2(F2(row[0], row[4]), w.x, w.y);
             split_half2(F2(row[2], row[6]), w.z, w.w);
-            s_frag[step * 32 + 4 * warp + t] = w;
+            if (TURNED) {                                    // columns: head, and head + 4 for what its rounding left
+                reinterpret_cast<uint2*>(s_frag)[step * 32 + 4 * warp + t] = make_uint2(w.x, w.z);
+                reinterpret_cast<uint2*>(s_frag)[step * 32 + 4 * (warp + 4) + t] = make_uint2(w.y, w.w);
+            } else {
+                s_frag[step * 32 + 4 * warp + t] = w;
+            }
         }
         __syncwarp();
     } else {
-        if (lane < HD / 16 * 4) s_frag[(lane >> 2) * 32 + 4 * warp + t] = make_uint4(0u, 0u, 0u, 0u);
+        if (lane < HD / 16 * 4) {
+            if (!TURNED) {
+                s_frag[(lane >> 2) * 32 + 4 * warp + t] = make_uint4(0u, 0u, 0u, 0u);
+            } else if (warp < 4) {
+                reinterpret_cast<uint2*>(s_frag)[(lane >> 2) * 32 + 4 * warp + t] = make_uint2(0u, 0u);
+                reinterpret_cast<uint2*>(s_frag)[(lane >> 2) * 32 + 4 * (warp + 4) + t] = make_uint2(0u, 0u);
+            }
+        }
         if (lane < 2) s_qsum[warp * 2 + lane] = 0.f;
         if (lane == 0) s_unit[warp] = 1.f;
     }
@@ -331,16 +357,21 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     }
     __syncthreads();
 
-    float qsum[NG];
+    // a lane's head, or its two heads
+    const int hA = TURNED ? 2 * (t & 1) : r, hB = TURNED ? hA + 1 : r;
+    F2 qsum[NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) qsum[g] = s_qsum[r * 2 + g];
-    const float unit = s_unit[r];
-    const float c = p.scale * LOG2E * unit;
+    for (int g = 0; g < NG; ++g) qsum[g] = F2(s_qsum[hA * 2 + g], s_qsum[hB * 2 + g]);
+    const F2 unit(s_unit[hA], s_unit[hB]);
+    const float c_raw = p.scale * LOG2E;
+    const F2 c = unit * F2(c_raw, c_raw);
     const uint4* qf = reinterpret_cast<const uint4*>(smem + L::QF_OFF) + lane;
+    const uint2* qt = reinterpret_cast<const uint2*>(smem + L::QF_OFF) + lane;
 
-    // O of head r, dims 16 j + 4 t + {0, 2} (o[2j]) and {1, 3} (o[2j+1]), in the scale of the codes
+    // O in the scale of the codes: of head r, dims 16 j + 4 t + {0, 2} (o[2j]) and {1, 3} (o[2j+1]); TURNED: of the two heads (their
+    // low halves in lanes t >= 2), dim 16 j + 2 r (o[2j]) and the next (o[2j+1])
     F2 o[HD / 8], om[NG];
-    float m_run, l_run;
+    F2 m_run, l_run;                                         // per head (the same twice, and the two keys' shares, where a lane has one)
     float pscale = 8192.f;                                   // P d is carried times this
 
     // One turn over NB blocks that lie next to each other in the ring.
@@ -377,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
                         mma_16816(acc[j], a1.x, a1.y, a1.z, a1.w, n.x[1], n.x[3]);
                     }
                 }
-                const F2 qs(qsum[g], qsum[g]);
+                const F2 qs = qsum[g];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     const F2 m(half_hi(ks[j][0][g]), half_hi(ks[j][1][g])), d(half_lo(ks[j][0][g]), half_lo(ks[j][1][g]));
@@ -393,23 +424,23 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         }
 
         // ---- online softmax -------------------------------------------------------------------------------------
-        float mx = m_run;
+        float mx = m_run.x();
 #pragma unroll
         for (int j = 0; j < NT; ++j) mx = fmaxf(mx, fmaxf(s[j].x(), s[j].y()));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float m_safe = mx == -CUDART_INF_F ? 0.f : mx;
-        const float alpha = fast_exp2((m_run - m_safe) * c);
+        const float alpha = fast_exp2((m_run.x() - m_safe) * c.x());
         const F2 alpha2(alpha, alpha);
-        m_run = mx;
+        m_run = F2(mx, mx);
         F2 sum(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const F2 x = (s[j] + F2(-m_safe, -m_safe)) * F2(c, c);
+            const F2 x = (s[j] + F2(-m_safe, -m_safe)) * c;
             s[j] = F2(fast_exp2(x.x()), fast_exp2(x.y()));
             sum = j == 0 ? s[j] : sum + s[j];
         }
-        l_run = fmaf(l_run, alpha, sum.x() + sum.y());
+        l_run = fma2(l_run, alpha2, sum);
 
         // ---- O = alpha O + (P d) codes, and P m -----------------------------------------------------------------
         uint32_t vs[NT][2][NG];
@@ -452,6 +483,132 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         }
     };
 
+    // The same with the operands turned around.
+    auto turn_turned = [&](auto nb_c, const uint8_t* blk, int nrow) {
+        constexpr int NB = decltype(nb_c)::value, NT = 2 * NB;         // tiles of eight positions; a lane has position r of each
+        F2 s[NT];
+        {
+            uint32_t w[NT][NW], ks[NT][NG];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const uint8_t* b = blk + (j >> 1) * F::BLOCK;
+                const int row = 8 * (j & 1) + r;
+                if constexpr (NW == 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(b + row * F::ROWB + t * 16);
+                    w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+                    const uint2 k = *reinterpret_cast<const uint2*>(b + F::KS_OFF + row * F::SROWB);
+                    ks[j][0] = k.x; ks[j][NG - 1] = k.y;
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2*>(b + row * F::ROWB + t * 8);
+                    w[j][0] = v.x; w[j][1] = v.y;
+                    ks[j][0] = *reinterpret_cast<const uint32_t*>(b + F::KS_OFF + row * F::SROWB);
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float acc[NB][4];
+#pragma unroll
+                for (int h = 0; h < NB; ++h) acc[h][0] = acc[h][1] = acc[h][2] = acc[h][3] = 0.f;
+#pragma unroll
+                for (int i = 2 * g; i < 2 * g + 2; ++i) {
+                    const uint2 b0 = qt[(2 * i) * 32], b1 = qt[(2 * i + 1) * 32];
+#pragma unroll
+                    for (int h = 0; h < NB; ++h) {
+                        const Nibbles n(w[2 * h][i]), u(w[2 * h + 1][i]);
+                        mma_16816(acc[h], n.x[0], u.x[0], n.x[2], u.x[2], b0.x, b0.y);
+                        mma_16816(acc[h], n.x[1], u.x[1], n.x[3], u.x[3], b1.x, b1.y);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const float d = half_lo(ks[j][g]);
+                    const F2 x(acc[j >> 1][2 * (j & 1)], acc[j >> 1][2 * (j & 1) + 1]);
+                    s[j] = g == 0 ? F2(d, d) * x : fma2(F2(d, d), x, s[j]);
+                }
+            }
+            // what the rounding of q left over comes from the lane two places on
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                s[j] = s[j] + shfl_xor(s[j], 2);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const float m = half_hi(ks[j][g]);
+                    s[j] = fma2(F2(m, m), qsum[g], s[j]);
+                }
+            }
+        }
+        if (nrow < 16 * NB) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                if (8 * j + r >= nrow) s[j] = F2(-CUDART_INF_F, -CUDART_INF_F);
+        }
+
+        float mx = m_run.x(), my = m_run.y();
+#pragma unroll
+        for (int j = 0; j < NT; ++j) { mx = fmaxf(mx, s[j].x()); my = fmaxf(my, s[j].y()); }
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, off));
+        }
+        const F2 neg(mx == -CUDART_INF_F ? 0.f : -mx, my == -CUDART_INF_F ? 0.f : -my);
+        const F2 xa = (m_run + neg) * c;
+        const F2 alpha(fast_exp2(xa.x()), fast_exp2(xa.y()));
+        m_run = F2(mx, my);
+        F2 sum(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const F2 x = (s[j] + neg) * c;
+            s[j] = F2(fast_exp2(x.x()), fast_exp2(x.y()));
+            sum = j == 0 ? s[j] : sum + s[j];
+        }
+        l_run = fma2(l_run, alpha, sum);
+
+        uint32_t vs[NT][NG];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const uint8_t* at = blk + (j >> 1) * F::BLOCK + F::VS_OFF + (8 * (j & 1) + r) * F::SROWB;
+            if constexpr (NG == 2) {
+                const uint2 v = *reinterpret_cast<const uint2*>(at);
+                vs[j][0] = v.x; vs[j][NG - 1] = v.y;
+            } else {
+                vs[j][0] = *reinterpret_cast<const uint32_t*>(at);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            uint32_t b[NT];
+            om[g] = om[g] * alpha;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const float m = half_hi(vs[j][g]), d = half_lo(vs[j][g]) * pscale;
+                om[g] = fma2(s[j], F2(m, m), om[g]);
+                uint32_t hi, lo;
+                split_half2(s[j] * F2(d, d), hi, lo);
+                b[j] = transpose8(t < 2 ? hi : lo);          // position r, heads in pairs -> column r, positions 2t, 2t + 1
+            }
+            uint32_t w[NB][4];
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
+                const uint4 v = *reinterpret_cast<const uint4*>(blk + h * F::BLOCK + F::V_OFF + g * 512 + lane * 16);
+                w[h][0] = v.x; w[h][1] = v.y; w[h][2] = v.z; w[h][3] = v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < NB; ++h) {
+                    const Nibbles n(w[h][i]);
+                    mma_16816(x, n.x[0], n.x[1], n.x[2], n.x[3], b[2 * h], b[2 * h + 1]);
+                }
+                F2& oe = o[2 * (4 * g + i)];
+                F2& od = o[2 * (4 * g + i) + 1];
+                oe = fma2(oe, alpha, F2(x[0], x[1]));
+                od = fma2(od, alpha, F2(x[2], x[3]));
+            }
+        }
+    };
+
     // Twice at most: P d is carried times 2^13, which overflows fp16 where a step is 8 or more (values of V spread over
     // more than 120).  Infinities cannot leave the sums again, so one look at the end finds them, and the warp starts over with
     // 2^-2, which holds for every fp16 step, and still has 23 bits below the largest.
@@ -460,8 +617,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     for (int j = 0; j < HD / 8; ++j) o[j] = F2(0.f, 0.f);
 #pragma unroll
     for (int g = 0; g < NG; ++g) om[g] = F2(0.f, 0.f);
-    m_run = -CUDART_INF_F;
-    l_run = 0.f;
+    m_run = F2(-CUDART_INF_F, -CUDART_INF_F);
+    l_run = F2(0.f, 0.f);
     if (pass) {
 #pragma unroll
         for (int k = 0; k < kTurns; ++k) {
@@ -504,8 +661,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
             }
             __syncwarp();
         }
-        if (two) turn(std::integral_constant<int, 2>{}, blk, nrow);
-        else     turn(std::integral_constant<int, 1>{}, blk, nrow);
+        if constexpr (TURNED) {
+            if (two) turn_turned(std::integral_constant<int, 2>{}, blk, nrow);
+            else     turn_turned(std::integral_constant<int, 1>{}, blk, nrow);
+        } else {
+            if (two) turn(std::integral_constant<int, 2>{}, blk, nrow);
+            else     turn(std::integral_constant<int, 1>{}, blk, nrow);
+        }
         __syncwarp();                                        // every lane has read the ring slots
         if (it + kTurns < turns) load_turn(it + kTurns);
         cp_async_commit();
@@ -523,31 +685,59 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     __syncthreads();
     float* mO = reinterpret_cast<float*>(smem);
     float* mML = reinterpret_cast<float*>(smem + L::ML_OFF);
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-    float oms[NG];
+    // a head's sums lie in the four lanes of a quad, or (TURNED) in the eight of one place t
+    F2 total[NG + 1];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        float v = om[g].x() + om[g].y();
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        oms[g] = v + __shfl_xor_sync(0xffffffffu, v, 2);
+    for (int g = 0; g <= NG; ++g) {
+        F2 v = g < NG ? om[g < NG ? g : 0] : l_run;
+        if constexpr (TURNED) {
+#pragma unroll
+            for (int off = 4; off <= 16; off <<= 1) v = v + shfl_xor(v, off);
+        } else {
+            float x = v.x() + v.y();
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            v = F2(x, x);
+        }
+        total[g] = v;
     }
-    const float m_raw = m_run * unit;                        // q . k, the unit the CTAs share
-    if (t == 0) *reinterpret_cast<float2*>(&mML[(warp * 8 + r) * 2]) = make_float2(m_raw, l_run);
+    const F2 m_raw = m_run * unit;                           // q . k, the unit the CTAs share
+    if (TURNED ? (r == 0 && t < 2) : t == 0) {
+        *reinterpret_cast<float2*>(&mML[(warp * 8 + hA) * 2]) = make_float2(m_raw.x(), total[NG].x());
+        if (TURNED) *reinterpret_cast<float2*>(&mML[(warp * 8 + hB) * 2]) = make_float2(m_raw.y(), total[NG].y());
+    }
     __syncthreads();
-    const float c_raw = p.scale * LOG2E;
     {
-        float M = -CUDART_INF_F;
+        float M[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mML[(w * 8 + r) * 2]);
-        const float wgt = m_raw == -CUDART_INF_F ? 0.f : fast_exp2((m_raw - M) * c_raw);
-        const float f = 1048576.f / pscale * wgt;            // 2^20: the scale of the codes
-        float* dst = mO + (size_t)(warp * 8 + r) * L::MSTRIDE + 4 * t;
+        for (int w = 0; w < kWarps; ++w) {
+            M[0] = fmaxf(M[0], mML[(w * 8 + hA) * 2]);
+            if (TURNED) M[1] = fmaxf(M[1], mML[(w * 8 + hB) * 2]);
+        }
+        const float wx = m_raw.x() == -CUDART_INF_F ? 0.f : fast_exp2((m_raw.x() - M[0]) * c_raw);
+        const float f = 1048576.f / pscale;                  // 2^20: the scale of the codes
+        if constexpr (TURNED) {
+            const float wy = m_raw.y() == -CUDART_INF_F ? 0.f : fast_exp2((m_raw.y() - M[1]) * c_raw);
+            const F2 wgt(wx, wy), fw = F2(f, f) * wgt;
+            float* dst = mO + (size_t)(warp * 8 + hA) * L::MSTRIDE + 2 * r;
 #pragma unroll
-        for (int j = 0; j < HD / 16; ++j) {
-            const float a = oms[j / 4] * wgt;
-            *reinterpret_cast<float4*>(dst + 16 * j) = make_float4(fmaf(o[2 * j].x(), f, a), fmaf(o[2 * j + 1].x(), f, a),
-                                                                   fmaf(o[2 * j].y(), f, a), fmaf(o[2 * j + 1].y(), f, a));
+            for (int j = 0; j < HD / 16; ++j) {
+                const F2 a = total[j / 4] * wgt;
+                const F2 e = fma2(o[2 * j] + shfl_xor(o[2 * j], 2), fw, a), d = fma2(o[2 * j + 1] + shfl_xor(o[2 * j + 1], 2), fw, a);
+                if (t < 2) {
+                    *reinterpret_cast<float2*>(dst + 16 * j) = make_float2(e.x(), d.x());
+                    *reinterpret_cast<float2*>(dst + L::MSTRIDE + 16 * j) = make_float2(e.y(), d.y());
+                }
+            }
+        } else {
+            const float fw = f * wx;
+            float* dst = mO + (size_t)(warp * 8 + r) * L::MSTRIDE + 4 * t;
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) {
+                const float a = total[j / 4].x() * wx;
+                *reinterpret_cast<float4*>(dst + 16 * j) = make_float4(fmaf(o[2 * j].x(), fw, a), fmaf(o[2 * j + 1].x(), fw, a),
+                                                                       fmaf(o[2 * j].y(), fw, a), fmaf(o[2 * j + 1].y(), fw, a));
+            }
         }
     }
     __syncthreads();
@@ -615,16 +805,28 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
 // rows: 14.8 us against 21.5 from two waves).
 int decode_q4_num_splits(int head_blocks, int sm_count) { return max(1, min(DECODE_MAX_SPLITS, kCtas * sm_count / head_blocks)); }
 
+namespace {
+template <int HD, bool TURNED>
+cudaError_t set_attributes() {
+    return cudaFuncSetAttribute(decode_q4_kernel<HD, TURNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<HD>::TOTAL);
+}
+template <int HD, bool TURNED>
+cudaError_t launch(const DecodeQ4Args& a, cudaStream_t stream) {
+    return launch_dependent(decode_q4_kernel<HD, TURNED>, dim3(a.n_splits * a.head_blocks, a.n_kv), kThreads, Q4Smem<HD>::TOTAL, stream, 1, a);
+}
+} // namespace
+
 cudaError_t decode_q4_set_attributes() {
-    cudaError_t e = cudaFuncSetAttribute(decode_q4_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<128>::TOTAL);
-    if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(decode_q4_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<64>::TOTAL);
+    cudaError_t e;
+    if ((e = set_attributes<128, false>()) != cudaSuccess || (e = set_attributes<128, true>()) != cudaSuccess) return e;
+    if ((e = set_attributes<64, false>()) != cudaSuccess) return e;
+    return set_attributes<64, true>();
 }
 
 cudaError_t launch_decode_q4(const DecodeQ4Args& a, int head_dim, cudaStream_t stream, unsigned long long* launches) {
-    const dim3 grid(a.n_splits * a.head_blocks, a.n_kv);
-    const cudaError_t e = head_dim == 128 ? launch_dependent(decode_q4_kernel<128>, grid, kThreads, Q4Smem<128>::TOTAL, stream, 1, a)
-                                          : launch_dependent(decode_q4_kernel<64>, grid, kThreads, Q4Smem<64>::TOTAL, stream, 1, a);
+    const bool turned = a.heads_per_cta <= 4;
+    const cudaError_t e = head_dim == 128 ? (turned ? launch<128, true>(a, stream) : launch<128, false>(a, stream))
+                                          : (turned ? launch<64, true>(a, stream) : launch<64, false>(a, stream));
     if (launches) *launches += 1;
     return e;
 }
