@@ -325,7 +325,8 @@ int oattn_kv_load_q4(const void* cache, uint16_t* kc, uint16_t* vc, int heads, i
                      int dst_ctx, int dst_base, void* stream);
 
 /* oattn_kv_shift on the 4-bit cache of all layers: rows [n_keep, n_keep + shift) are dropped, the rest slides left, the last
- * `shift` rows read back as zero.  The codes move as they are: nothing is quantised again.  In place, no scratch. */
+ * `shift` rows read back as zero.  The codes move as they are: nothing is quantised again.  In place, no scratch; n_layer * n_kv
+ * up to 65535. */
 int oattn_kv_shift_q4(void* cache, int n_layer, int n_kv, int head_dim, int n_ctx, int n_keep, int shift, void* stream);
 
 /* oattn_decode_ex on the 4-bit cache (ext may be NULL): q attends over rows 0..*d_pos; with OATTN_FUSE_KV_APPEND the new row is

@@ -609,9 +609,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         }
     };
 
-    // Twice at most: P d is carried times 2^13, which overflows fp16 where a step is 8 or more (values of V spread over
-    // more than 120).  Infinities cannot leave the sums again, so one look at the end finds them, and the warp starts over with
-    // 2^-2, which holds for every fp16 step, and still has 23 bits below the largest.
+    // P d is carried times 2^13, which overflows fp16 where a step is 8 or more (values of V spread over more than 120).
+    // Infinities cannot leave the sums again, so one look at the end finds them; the warp then looks its steps up and
+    // starts over with a power of two that holds for them, unless it is the data that are not finite.
     for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) o[j] = F2(0.f, 0.f);
@@ -678,7 +678,22 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     for (int j = 1; j < HD / 8; ++j) any = any + o[j];
     // (an infinity or a NaN in any of them leaves no finite sum)
     if (!__any_sync(0xffffffffu, !(fabsf(any.x()) + fabsf(any.y()) <= 3.402823466e38f))) break;
-    pscale = 0.25f;
+    float d_max = 0.f;
+    for (int it = 0; it < turns; ++it) {
+        const int b0 = first(it), nb = plan.step == 2 && b0 + 1 < blk1 ? 2 : 1;
+        for (int i = lane; i < nb * 16 * NG; i += 32) {
+            const int row = b0 * 16 + i / NG;
+            uint32_t w = 0u;
+            if (owner && row == new_pos) w = s_new[64 + 2 + i % NG];
+            else if (row < npos) w = *reinterpret_cast<const uint32_t*>(cache + (size_t)(row >> 4) * F::BLOCK + F::VS_OFF + (row & 15) * F::SROWB + 4 * (i % NG));
+            const float d = half_lo(w);
+            if (d <= 65504.f) d_max = fmaxf(d_max, d);
+        }
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) d_max = fmaxf(d_max, __shfl_xor_sync(0xffffffffu, d_max, off));
+    if (!(d_max * pscale > 65000.f)) break;                  // nothing overflowed: the data are not finite
+    pscale = __uint_as_float((uint32_t)(127 + 14 - ((int)(__float_as_uint(d_max) >> 23) - 127)) << 23);     // d_max * pscale in [2^14, 2^15)
     }
 
     // ---- merge the warps: O of a warp scaled by e^(m_w - M), sums in warp order ----------------------------------

@@ -331,7 +331,84 @@ def test_prefill_captured(ops):
         assert torch.equal(got, want) and torch.equal(a, b)
 
 
+@pytest.mark.parametrize("n_head,n_kv,hd", [(8, 2, 128), (12, 4, 64)])
+def test_unfused_prefill_reads_what_the_store_call_wrote(ops, n_head, n_kv, hd):
+    """Rows stored by the unfused call, then the chunk with and without the rotation of q: the fused call's bytes and outputs."""
+    rng = np.random.default_rng(224)
+    past, batch = 21, 30
+    n_ctx, scale, rope = past + batch, 1.0 / math.sqrt(hd), (1, hd, 1e6, None)
+    base = filled(rng, n_kv, hd, n_ctx, past)
+    q, k, v = rng.standard_normal((batch, n_head, hd)).astype(np.float32), rows(rng, batch, n_kv, hd), rows(rng, batch, n_kv, hd)
+    pos = np.arange(past, n_ctx)
+    kr = ref.rope(k, pos, 1, hd, 1e6).astype(np.float32)
+    a, b = dev(base), dev(base)
+    fused, unfused, raw = (torch.empty(batch, n_head, hd, device="cuda") for _ in range(3))
+    ops.attn_prefill_q4(dev(q), dev(k), dev(v), a, fused, n_head, n_kv, hd, n_ctx, past, batch, scale, ops.FUSE_ALL, rope)
+    ops.kv_store_q4_batch(b, dev(kr), dev(v), n_kv, hd, n_ctx, past, batch)
+    ops.attn_prefill_q4(dev(q), None, None, b, unfused, n_head, n_kv, hd, n_ctx, past, batch, scale, ops.FUSE_ROPE_Q, rope)
+    ops.attn_prefill_q4(dev(ref.rope(q, pos, 1, hd, 1e6).astype(np.float32)), None, None, b, raw, n_head, n_kv, hd, n_ctx, past, batch, scale,
+                        ops.FUSE_NONE)
+    torch.cuda.synchronize()
+    assert torch.equal(a, b) and torch.equal(fused, unfused)
+    K, V = ref.read_rows(b.cpu().numpy(), hd, n_ctx)
+    want, most = ref.attend(ref.rope(q, pos, 1, hd, 1e6), K, V, past, scale)
+    for got in (fused, raw):
+        assert np.abs(got.cpu().numpy() - want).max() <= prefill_bound(most, scale, V, False)
+    # the append without any rotation
+    c, out = dev(base), torch.empty(n_head, hd, device="cuda")
+    ops.attn_decode_q4(dev(q[0]), dev(k[0]), dev(v[0]), c, out, n_head, n_kv, hd, n_ctx, dpos(past), scale, ops.FUSE_KV_APPEND)
+    w = base.copy()
+    ref.write_rows(w, hd, [past], k[:1], v[:1])
+    assert np.array_equal(c.cpu().numpy(), w)
+    K, V = ref.read_rows(w, hd, past + 1)
+    want, most = ref.attend(q[:1], K, V, past, scale)
+    assert np.abs(out.cpu().numpy() - want[0]).max() <= decode_bound(most, scale, V)
+
+
+@pytest.mark.parametrize("n_head,n_kv", [(4, 1), (7, 1)])
+def test_a_bad_query_head_stays_alone(ops, n_head, n_kv):
+    rng = np.random.default_rng(225)
+    hd, n = 128, 100
+    cache = dev(filled(rng, n_kv, hd, n, n))
+    q = rng.standard_normal((n_head, hd)).astype(np.float32)
+    good, out = torch.empty(n_head, hd, device="cuda"), torch.empty(n_head, hd, device="cuda")
+    ops.attn_decode_q4(dev(q), None, None, cache, good, n_head, n_kv, hd, n, dpos(n - 1), 0.0884, ops.FUSE_NONE)
+    for bad in (np.nan, np.inf, -np.inf):
+        x = q.copy()
+        x[1, 77] = bad
+        ops.attn_decode_q4(dev(x), None, None, cache, out, n_head, n_kv, hd, n, dpos(n - 1), 0.0884, ops.FUSE_NONE)
+        assert torch.isnan(out[1]).all() and torch.equal(out[2:], good[2:]) and torch.equal(out[0], good[0])
+    # the same over rows whose steps are all zero
+    flat = np.zeros((n_kv, (n + 15) // 16, 18 * hd), np.uint8)
+    same = np.ones((n, n_kv, hd), np.float32)
+    ref.write_rows(flat, hd, range(n), same, 3 * same)
+    x = q.copy()
+    x[1, 77] = np.nan
+    ops.attn_decode_q4(dev(x), None, None, dev(flat), out, n_head, n_kv, hd, n, dpos(n - 1), 0.0884, ops.FUSE_NONE)
+    rest = [h for h in range(n_head) if h != 1]
+    assert torch.isnan(out[1]).all() and float((out[rest] - 3).abs().max()) <= decode_bound(hd * 4, 0.0884, np.float64(3))
+    x = q.copy()
+    x[2] = 0                                              # all scores alike: the mean of the values
+    ops.attn_decode_q4(dev(x), None, None, cache, out, n_head, n_kv, hd, n, dpos(n - 1), 0.0884, ops.FUSE_NONE)
+    V = ref.read_rows(cache.cpu().numpy(), hd, n)[1]
+    assert np.abs(out[2].cpu().numpy() - V[0].mean(0)).max() <= decode_bound(0, 1, V)
+
+
 # ------------------------------------------------------------------------------------------------- large caches, odd positions
+def test_store_of_more_blocks_than_one_grid_plane(ops):
+    n_kv, hd, n, base = 1, 64, 65535 * 16 + 300, 5
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    k, v = (torch.randn(n, n_kv, hd, device="cuda", generator=gen) for _ in range(2))
+    cache = ops.KVCacheQ4(1, n_kv, n + 10, hd).layer(0)
+    ops.kv_store_q4_batch(cache, k, v, n_kv, hd, n + 10, base, n)
+    for at, m in ((0, 40), (65535 * 16 - 60, 120), (n - 50, 50)):
+        kh, vh = (torch.zeros(n_kv, m, hd, dtype=torch.float16, device="cuda") for _ in range(2))
+        ops.kv_load_q4(cache, kh, vh, n_kv, hd, n + 10, base + at, m)
+        for g, x in ((kh, k), (vh, v)):
+            w = ref.values(*ref.quantise(np.ascontiguousarray(x[at: at + m].cpu().numpy().transpose(1, 0, 2))))
+            assert (np.abs(g.float().cpu().numpy() - w) <= 2.0 ** -11 * (1 + 2.0 ** -11) * np.abs(w) + 2.0 ** -25).all()
+
+
 def test_offsets_beyond_two_gigabytes(ops):
     n_kv, hd, n_ctx, n_head = 8, 128, 2_000_016, 8
     assert ops.kv_q4_bytes(n_kv, hd, n_ctx) > 2 ** 31
