@@ -244,8 +244,8 @@ __global__ void __launch_bounds__(32 * kLoadWarps) kv_load_q4_kernel(const uint8
 // scales.  It walks the blocks in order; a step brings the blocks that hold the source rows of kShiftBlocks blocks to
 // shared memory and writes those blocks from there.  Sources lie at or behind the place they go to, and those of later
 // steps behind everything a step writes, so the copies of the next steps run while this one writes.
-constexpr int kShiftThreads = 256;
-constexpr int kShiftBlocks = 16;
+constexpr int kShiftThreads = 512;
+constexpr int kShiftBlocks = 32;
 constexpr int kShiftWindows = 4;           // steps in flight, this one among them
 
 template <int HD>
