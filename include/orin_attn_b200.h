@@ -336,7 +336,8 @@ int oattn_kv_shift_q4(void* cache, int n_layer, int n_kv, int head_dim, int n_ct
  * always a programmatic dependent one (as the store, read-back and roll calls): oattn_set_decode_overlap modes 0 and 1 are the
  * same here, mode 2 means what it says there.  *d_pos beyond the cache is taken as n_ctx - 1, below zero there is no row
  * and the output is zero.  The workspace rules are those of oattn_decode_workspace_bytes: calls that may run at the same
- * time, graph replays among them, need workspaces of their own. */
+ * time, graph replays among them, need workspaces of their own; the library keeps arrival counters for the 64 workspaces
+ * of a device that decode calls were given last, so no more of them may be in use at a time, captured graphs' among them. */
 size_t oattn_decode_q4_workspace_bytes(int n_head, int n_kv, int head_dim);
 int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, int n_head, int n_kv,
                     int head_dim, int n_ctx, const int* d_pos, float scale, int fuse, const oattn_rope_params* rope,
@@ -344,9 +345,12 @@ int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void
 
 /* oattn_prefill_ex on the 4-bit cache (ext may be NULL): the chunk's rows are quantised into the cache, and every query sees the
  * rows as the cache holds them, its own chunk's among them.  The output is fp32 (`out`) or fp16 (`out_f16`, [batch][n_head]
- * [head_dim]): pass one of them; with ext->out_mmq both may be NULL.  The attention itself runs on fp16 copies of the
- * rows, which the first of the two launches makes in the workspace; the workspace is sized for `max_rows` = the largest n_past + batch and serves
- * all layers.  oattn_prefill_status reads its status word (same n_head, head_dim, batch). */
+ * [head_dim]): pass one of them; with ext->out_mmq both may be NULL.  A short chunk (up to 1024 (token, head) pairs for
+ * head_dim 128, 2048 for 64; a few less when kv heads do not divide them into eights) is attended from the 4-bit rows
+ * themselves, with the accuracy of oattn_decode_q4; a longer one, or one with ext->out_mmq, on fp16 copies of the rows, which the
+ * first of the two launches makes in the workspace.  The workspace is sized for `max_rows` = the largest n_past + batch and
+ * serves all layers; it need not be cleared, and calls that may run at the same time need one each.  oattn_prefill_status reads
+ * its status word (same n_head, head_dim, batch). */
 size_t oattn_prefill_q4_workspace_bytes(int n_head, int n_kv, int head_dim, int max_batch, int max_rows);
 int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, uint16_t* out_f16, int n_head,
                      int n_kv, int head_dim, int n_ctx, int n_past, int batch, float scale, int fuse,

@@ -604,11 +604,27 @@ int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void
     return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "decode (4-bit cache) launch");
 }
 
-// [fp16 queries][status word, 256 bytes][fp16 K rows][fp16 V rows]: the first two as in oattn_prefill
+// A short chunk is walked by the decode kernel, eight (token, head) pairs per CTA, straight from the 4-bit rows; a long one by the
+// prefill kernels, which take more pairs at a time but read fp16 copies, on one CTA per kv head and 128 pairs.  The limit is on
+// the eights of pairs of all kv heads; the smaller for heads of 128, whose prefill kernel is the tensor-core one.  Microseconds
+// per call, short way against long way: 32/8 heads of 128 behind 8192 rows, 8 tokens 22 against 63, 32 tokens (128 eights) 55
+// against 66, 64 tokens 93 against 67; behind 64 rows 10.4 against 11.8 and 11.1 against 12.3.  32/8 heads of 64 behind 8192 rows,
+// 8 tokens 16 against 112, 64 tokens (256 eights) 56 against 114.  The worst inside the limit is 28/4 heads, 32 tokens behind 512
+// rows: 15.4 against 14.5.
+static int chunk_blocks(int n_head, int n_kv, int head_dim, int batch) {
+    const long long blocks = ((long long)batch * (n_head / n_kv) + 7) / 8;
+    return blocks * n_kv <= (head_dim == 128 ? 128 : 256) ? (int)blocks : 0;
+}
+constexpr size_t kChunkScratch = 4u << 20;      // partial results of a chunk's slices: at most 2 * 160 slices of 8 rows, and their groups
+
+// [fp16 queries][status word, 256 bytes][fp16 K rows][fp16 V rows]: the first two as in oattn_prefill.  A short chunk has its fp32
+// queries and partial results behind the status word instead of the rows.
 size_t oattn_prefill_q4_workspace_bytes(int n_head, int n_kv, int head_dim, int max_batch, int max_rows) {
     const size_t head = oattn_prefill_workspace_bytes(n_head, n_kv, head_dim, max_batch);
     if (!head || max_rows < max_batch) return 0;
-    return head + 2 * align256((size_t)n_kv * max_rows * head_dim * sizeof(__half));
+    const size_t copies = 2 * align256((size_t)n_kv * max_rows * head_dim * sizeof(__half));
+    const size_t chunk = align256((size_t)max_batch * n_head * head_dim * sizeof(float)) + kChunkScratch;
+    return head + (copies > chunk ? copies : chunk);
 }
 
 int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, uint16_t* out_f16, int n_head,
@@ -652,7 +668,36 @@ int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, voi
     p.cache_ctx = n_ctx;
     rope_freq_table(a.rope, p.freq);
     cudaStream_t s = (cudaStream_t)stream;
-    cudaError_t e = launch_prefill_q4_prologue(p, s, &g_launches);
+    cudaError_t e;
+    const int blocks = mmq || g_prefill_impl != 0 ? 0 : chunk_blocks(n_head, n_kv, head_dim, batch);
+    p.q32 = nullptr; p.tickets = nullptr; p.n_tickets = 0;
+    if (blocks) {
+        DecodeQ4Args c;
+        c.heads_per_cta = 8;
+        c.head_blocks = blocks;
+        const DecodeWsLayout w = decode_ws_layout(n_kv * blocks * 8, n_kv * blocks, head_dim, decode_q4_num_splits(n_kv * blocks, dev->sm_count));
+        uint8_t* scratch = wsb + head + align256((size_t)batch * n_head * head_dim * sizeof(float));
+        const size_t tickets = (size_t)n_kv * blocks * (w.n_groups + 1);      // in the workspace: the first launch can clear them
+        if (align256(w.total) + tickets * sizeof(unsigned) <= kChunkScratch) {
+            p.q32 = reinterpret_cast<float*>(wsb + head);
+            p.tickets = c.tickets = reinterpret_cast<unsigned*>(scratch + align256(w.total));
+            p.n_tickets = (int)tickets;
+            e = launch_prefill_q4_prologue(p, s, &g_launches);
+            if (e != cudaSuccess) return cuda_fail(e, "prefill (4-bit cache) prologue launch");
+            c.q = p.q32; c.k_new = nullptr; c.v_new = nullptr; c.cache = p.cache; c.out = out; c.out16 = a.out16;
+            c.ws_o = reinterpret_cast<float*>(scratch + w.part_o);
+            c.ws_ml = reinterpret_cast<float*>(scratch + w.part_ml);
+            c.grp_o = reinterpret_cast<float*>(scratch + w.grp_o);
+            c.grp_ml = reinterpret_cast<float*>(scratch + w.grp_ml);
+            c.d_pos = nullptr;
+            c.n_head = n_head; c.n_kv = n_kv; c.n_ctx = n_ctx; c.n_past = n_past; c.batch = batch;
+            c.n_splits = w.n_splits; c.group = w.group; c.n_groups = w.n_groups;
+            c.scale = scale; c.fuse = OATTN_FUSE_NONE; c.overlap = 0; c.rope = a.rope;
+            e = launch_decode_q4(c, head_dim, s, &g_launches);
+            return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "prefill (short chunk) launch");
+        }
+    }
+    e = launch_prefill_q4_prologue(p, s, &g_launches);
     if (e != cudaSuccess) return cuda_fail(e, "prefill (4-bit cache) prologue launch");
     if (g_prefill_impl == 0) {
         e = launch_prefill_tc(a, dev->sm_count, s, &g_launches);

@@ -132,8 +132,12 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 // many products.  A lane then has two heads' scores of positions r and r + 8 instead of one head's of four, and P has to be
 // transposed between the products.  32/8 heads of 128, 131072 rows: 43.8 us against 47.4; 32/8 heads of 64, 32001 rows: 12.4
 // against 12.7; below a few thousand rows no difference.
-template <int HD, bool TURNED>
+//
+// CHUNK: a few tokens behind a long context.  The tile's eight rows are (token, head) pairs, each with the positions up to its own
+// token; everything else is as for one token.  32/8 heads behind 8192 rows: 16 us with its prologue for one token, 22 for eight.
+template <int HD, bool TURNED, bool CHUNK>
 __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid_constant__ DecodeQ4Args p) {
+    static_assert(!(TURNED && CHUNK), "a chunk fills the tile");
     using F = Q4<HD>;
     using L = Q4Smem<HD>;
     constexpr int MT = HD == 128 && kThreads >= 256 ? 256 : 128;    // threads that hold pieces of the merged block
@@ -145,14 +149,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     const int hb = blockIdx.x % p.head_blocks, split = blockIdx.x / p.head_blocks, kvh = blockIdx.y;
     const int GA = p.n_head / p.n_kv;                        // heads of the kv head, and of this CTA
     const int head0 = kvh * GA + hb * p.heads_per_cta;
-    const int G = min(p.heads_per_cta, GA - hb * p.heads_per_cta);
+    const int row0 = hb * p.heads_per_cta;                   // CHUNK: first (token, head) pair
+    const int G = min(p.heads_per_cta, (CHUNK ? p.batch * GA : GA) - row0);
+    // head row `i` of this CTA in q and in the output, in units of HD
+    auto head_row = [&](int i) { return CHUNK ? (size_t)((row0 + i) / GA) * p.n_head + kvh * GA + (row0 + i) % GA : (size_t)head0 + i; };
 
     // Inputs of the step: warp h has the row of head h, the last two warps the new rows of V and K as well, a lane EPL
     // consecutive dims.  All are issued together and, where the order against preceding kernels allows it, along with the
     // position word; from there to the barrier in front of the loop a warp waits for nobody.
     static_assert(kWarps == 8, "one warp per head");
     constexpr int E = F::EPL, kWarpK = kWarps - 1, kWarpV = kWarps - 2;
-    const bool append = (p.fuse & 4) != 0;
+    const bool append = !CHUNK && (p.fuse & 4) != 0;
     float in_q[E], in_kv[E];
     auto load_lane = [&](float (&x)[E], const float* src, const float* bias, size_t row) {
         const size_t at = row * HD + E * lane;
@@ -169,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         }
     };
     auto load_inputs = [&]() {
-        if (warp < G) load_lane(in_q, p.q, p.pre.bias_q, (size_t)head0 + warp);
+        if (warp < G) load_lane(in_q, p.q, CHUNK ? nullptr : p.pre.bias_q, head_row(warp));
         if (append && warp >= kWarpV) load_lane(in_kv, warp == kWarpK ? p.k_new : p.v_new, warp == kWarpK ? p.pre.bias_k : p.pre.bias_v, (size_t)kvh);
     };
 
@@ -178,7 +185,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         pdl_wait();
         load_inputs();
     }
-    const int npos = max(0, min(*p.d_pos, p.n_ctx - 1) + 1);
+    const int npos = CHUNK ? p.n_past + (row0 + G - 1) / GA + 1 : max(0, min(*p.d_pos, p.n_ctx - 1) + 1);
+    // CHUNK: positions that this lane's row sees, and that every row of the CTA sees
+    const int lim = CHUNK ? p.n_past + (row0 + min(r, G - 1)) / GA + 1 : npos, lim_all = CHUNK ? p.n_past + row0 / GA + 1 : npos;
     const Q4Plan plan = q4_plan(npos, p.n_splits);
     if (split >= max(plan.active, 1)) return;
     const int vh = kvh * p.head_blocks + hb;                 // place of this CTA's heads in the scratch block
@@ -224,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     }
 
     // ---- prologue -----------------------------------------------------------------------------------------------
-    const bool rope_q = (p.fuse & 1) != 0, rope_k = (p.fuse & 2) != 0;
+    const bool rope_q = !CHUNK && (p.fuse & 1) != 0, rope_k = !CHUNK && (p.fuse & 2) != 0;
     float* s_row = reinterpret_cast<float*>(smem + L::IN_OFF) + warp * HD;       // this warp's row on its way
     float* s_qsum = reinterpret_cast<float*>(smem + L::QS_OFF);
     float* s_unit = s_qsum + 16;
@@ -287,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     };
     uint4* s_frag = reinterpret_cast<uint4*>(smem + L::QF_OFF);
     if (warp < G) {
-        if (p.pre.norm_q) norm_lane(in_q, p.pre.norm_q);
+        if (!CHUNK && p.pre.norm_q) norm_lane(in_q, p.pre.norm_q);
         if (rope_q) rotate_lane(in_q, false);
         // the power of two that brings the largest |q| to [2^13, 2^14), and the group sums
         float amax = fabsf(in_q[0]);
@@ -375,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     float pscale = 8192.f;                                   // P d is carried times this
 
     // One turn over NB blocks that lie next to each other in the ring.
-    auto turn = [&](auto nb_c, const uint8_t* blk, int nrow) {
+    auto turn = [&](auto nb_c, const uint8_t* blk, int nrow, int nrow_all) {
         constexpr int NB = decltype(nb_c)::value, NT = 2 * NB;         // tiles of eight rows
         // ---- S = q . K ------------------------------------------------------------------------------------------
         F2 s[NT];                                            // rows 8j + 2t, + 1
@@ -417,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
                 }
             }
         }
-        if (nrow < 16 * NB) {
+        if (nrow_all < 16 * NB) {
 #pragma unroll
             for (int j = 0; j < NT; ++j)
                 s[j] = F2(8 * j + 2 * t >= nrow ? -CUDART_INF_F : s[j].x(), 8 * j + 2 * t + 1 >= nrow ? -CUDART_INF_F : s[j].y());
@@ -665,8 +674,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
             if (two) turn_turned(std::integral_constant<int, 2>{}, blk, nrow);
             else     turn_turned(std::integral_constant<int, 1>{}, blk, nrow);
         } else {
-            if (two) turn(std::integral_constant<int, 2>{}, blk, nrow);
-            else     turn(std::integral_constant<int, 1>{}, blk, nrow);
+            if (two) turn(std::integral_constant<int, 2>{}, blk, lim - b * 16, lim_all - b * 16);
+            else     turn(std::integral_constant<int, 1>{}, blk, lim - b * 16, lim_all - b * 16);
         }
         __syncwarp();                                        // every lane has read the ring slots
         if (it + kTurns < turns) load_turn(it + kTurns);
@@ -810,7 +819,19 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
 #pragma unroll
         for (int k = 0; k < S::N; ++k)
             if (st[k].L != st[k].L) { st[k].acc = make_float4(st[k].L, st[k].L, st[k].L, st[k].L); st[k].L = 1.f; }
-        emit_final<HD, false, MT>(p, head0, G, st);
+        if constexpr (CHUNK) {
+#pragma unroll
+            for (int k = 0; k < S::N; ++k) {
+                const int row = S::row(tid, k), c4 = S::col4(tid, k);
+                if (row >= G) continue;
+                const float4 v = normalised(st[k]);
+                const size_t at = head_row(row) * HD + c4 * 4;
+                if (p.out16) *reinterpret_cast<uint2*>(p.out16 + at) = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+                else         *reinterpret_cast<float4*>(p.out + at) = v;
+            }
+        } else {
+            emit_final<HD, false, MT>(p, head0, G, st);
+        }
     }
 }
 
@@ -821,27 +842,34 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
 int decode_q4_num_splits(int head_blocks, int sm_count) { return max(1, min(DECODE_MAX_SPLITS, kCtas * sm_count / head_blocks)); }
 
 namespace {
-template <int HD, bool TURNED>
+template <int HD, bool TURNED, bool CHUNK>
 cudaError_t set_attributes() {
-    return cudaFuncSetAttribute(decode_q4_kernel<HD, TURNED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<HD>::TOTAL);
+    return cudaFuncSetAttribute(decode_q4_kernel<HD, TURNED, CHUNK>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<HD>::TOTAL);
 }
-template <int HD, bool TURNED>
+template <int HD, bool TURNED, bool CHUNK>
 cudaError_t launch(const DecodeQ4Args& a, cudaStream_t stream) {
-    return launch_dependent(decode_q4_kernel<HD, TURNED>, dim3(a.n_splits * a.head_blocks, a.n_kv), kThreads, Q4Smem<HD>::TOTAL, stream, 1, a);
+    return launch_dependent(decode_q4_kernel<HD, TURNED, CHUNK>, dim3(a.n_splits * a.head_blocks, a.n_kv), kThreads, Q4Smem<HD>::TOTAL, stream, 1, a);
+}
+template <int HD>
+cudaError_t set_attributes_hd() {
+    cudaError_t e;
+    if ((e = set_attributes<HD, false, false>()) != cudaSuccess || (e = set_attributes<HD, true, false>()) != cudaSuccess) return e;
+    return set_attributes<HD, false, true>();
+}
+template <int HD>
+cudaError_t launch_hd(const DecodeQ4Args& a, cudaStream_t stream) {
+    if (a.batch > 0) return launch<HD, false, true>(a, stream);
+    return a.heads_per_cta <= 4 ? launch<HD, true, false>(a, stream) : launch<HD, false, false>(a, stream);
 }
 } // namespace
 
 cudaError_t decode_q4_set_attributes() {
-    cudaError_t e;
-    if ((e = set_attributes<128, false>()) != cudaSuccess || (e = set_attributes<128, true>()) != cudaSuccess) return e;
-    if ((e = set_attributes<64, false>()) != cudaSuccess) return e;
-    return set_attributes<64, true>();
+    const cudaError_t e = set_attributes_hd<128>();
+    return e != cudaSuccess ? e : set_attributes_hd<64>();
 }
 
 cudaError_t launch_decode_q4(const DecodeQ4Args& a, int head_dim, cudaStream_t stream, unsigned long long* launches) {
-    const bool turned = a.heads_per_cta <= 4;
-    const cudaError_t e = head_dim == 128 ? (turned ? launch<128, true>(a, stream) : launch<128, false>(a, stream))
-                                          : (turned ? launch<64, true>(a, stream) : launch<64, false>(a, stream));
+    const cudaError_t e = head_dim == 128 ? launch_hd<128>(a, stream) : launch_hd<64>(a, stream);
     if (launches) *launches += 1;
     return e;
 }

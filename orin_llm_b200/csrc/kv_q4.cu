@@ -368,6 +368,7 @@ __global__ void __launch_bounds__(kShiftThreads) kv_shift_q4_kernel(uint8_t* cac
 // the attention kernel would repeat that for each of its tiles (16 for 512 tokens of a 4-head group), on the warps that bound it.
 // 512 tokens of 32/8 heads behind 8192 rows: 18 us on a cold cache, 12 for the tokens alone (a chain of loads, angles and
 // rows) and 9.6 for the rows alone (43 MB); the attention behind it takes 70.
+// For a short chunk (see DecodeQ4Args) the queries stay fp32 and nothing is copied: the decode kernel reads the 4-bit rows.
 constexpr int kPrologueThreads = 256;
 
 template <int HD>
@@ -430,7 +431,10 @@ __global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kerne
         }
     }
     __syncthreads();
-    if (b == 0 && tid == 0 && a.status) *a.status = 0;
+    if (b == 0) {
+        if (tid == 0 && a.status) *a.status = 0;
+        for (int i = tid; i < p.n_tickets; i += kPrologueThreads) p.tickets[i] = 0;
+    }
     for (int j0 = warp; j0 < jobs; j0 += W * RB) {
         if (j0 != warp) load_rows(j0);
         cp_async_wait<0>();
@@ -480,6 +484,12 @@ __global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kerne
 #pragma unroll
                 for (int e = 0; e < F::EPL; ++e) x[e] = row[F::EPL * lane + e];
             }
+            if (r.kind == 0 && p.q32) {
+                float* dst = p.q32 + ((size_t)b * a.n_head + r.head) * HD + F::EPL * lane;
+#pragma unroll
+                for (int e = 0; e < F::EPL; ++e) dst[e] = x[e];
+                continue;
+            }
             if (r.kind == 0) {
                 __half* dst = a.q16 + ((size_t)b * a.n_head + r.head) * HD + F::EPL * lane;
 #pragma unroll
@@ -491,6 +501,7 @@ __global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kerne
             uint8_t* blk = p.cache + ((size_t)r.head * nblk + (pos >> 4)) * F::BLOCK;
             if (r.kind == 2) q4_store_row<HD, true>(blk, pos & 15, codes, s, lane);
             else             q4_store_row<HD, false>(blk, pos & 15, codes, s, lane);
+            if (p.q32) continue;
             __half* dst = (r.kind == 1 ? p.k16 : p.v16) + ((size_t)r.head * rows + pos) * HD + F::EPL * lane;
             const float d = __half2float(s.d), m = __half2float(s.m);
 #pragma unroll
@@ -563,7 +574,7 @@ cudaError_t launch_kv_shift_q4(uint8_t* cache, int n_layer, int n_kv, int head_d
 
 cudaError_t launch_prefill_q4_prologue(const KvQ4PrologueArgs& p, cudaStream_t stream, unsigned long long* launches) {
     const PrefillArgs& a = p.a;
-    const long long jobs = (long long)a.n_kv * q4_blocks((a.fuse & 4) ? a.n_past : a.n_past + a.batch);
+    const long long jobs = p.q32 ? 0 : (long long)a.n_kv * q4_blocks((a.fuse & 4) ? a.n_past : a.n_past + a.batch);
     constexpr int W = kPrologueThreads / 32;
     const dim3 grid((unsigned)(a.batch + (jobs + W - 1) / W));
     const cudaError_t e = a.head_dim == 128 ? launch_dependent(prefill_q4_prologue_kernel<128>, grid, kPrologueThreads, 0, stream, 1, p)

@@ -149,6 +149,9 @@ struct KvQ4PrologueArgs {
     uint8_t* cache;
     __half* k16;               // fp16 copies of the cache rows [n_kv][n_past + batch][hd]
     __half* v16;
+    float* q32;                // or nullptr; the queries as fp32, rotated and not scaled, instead of a.q16, and no copies
+    unsigned* tickets;         // arrival counters of the launch behind this one, set to zero
+    int n_tickets;
     int cache_ctx;             // positions of the 4-bit cache
     float freq[64];            // see rope_freq_table
 };
@@ -182,6 +185,10 @@ struct DecodeQ4Args {
     RopeArgs rope;
     PreArgs pre;
     float freq[64];                     // RoPE frequencies before the optional factors, theta^(-2i/n_rot) rounded to fp32
+    // A chunk of `batch` tokens behind n_past rows instead of one token at *d_pos (batch 0): the rows of a kv head are its
+    // (token, head) pairs, heads_per_cta = 8 of them per CTA, q is rotated already and the chunk's rows are in the cache.
+    int n_past = 0, batch = 0;
+    __half* out16 = nullptr;            // fp16 output of a chunk, instead of `out`
     int emit_partial = 0;
     int8_t* out_qs = nullptr;
     float* out_scales = nullptr;

@@ -24,12 +24,13 @@ def normed(x, bias, w, eps):
     return (x / np.sqrt((x ** 2).mean(-1, keepdims=True) + eps) * w).astype(np.float32)
 
 
+@pytest.mark.parametrize("batch", [21, 140])
 @pytest.mark.parametrize("n_head,n_kv,hd,n_rot,rope_type,norm", [(12, 2, 128, 128, 1, True), (14, 2, 64, 32, 1, False), (8, 8, 128, 96, 0, False),
                                                                 (20, 2, 64, 64, 0, True)])
-def test_bias_norm_and_partial_rotation_in_front(ops, n_head, n_kv, hd, n_rot, rope_type, norm):
+def test_bias_norm_and_partial_rotation_in_front(ops, n_head, n_kv, hd, n_rot, rope_type, norm, batch):
     """A chunk through the prefill call and one more token through the decode call."""
     rng = np.random.default_rng(200)
-    past, batch, n_ctx, theta, eps = 19, 21, 64, 1e4, 1e-6
+    past, n_ctx, theta, eps = 19, 200, 1e4, 1e-6
     cache = filled(rng, n_kv, hd, n_ctx, past)
     n = batch + 1
     q, k, v = rng.standard_normal((n, n_head, hd)).astype(np.float32), rows(rng, n, n_kv, hd), rows(rng, n, n_kv, hd)
@@ -82,7 +83,7 @@ def test_decode_writes_the_quantised_activation(ops, oracle):
 def test_prefill_block_output_and_other_kernel(ops):
     """out_mmq next to and instead of the fp32 output; the warp-level kernel with both output types."""
     rng = np.random.default_rng(202)
-    n_head, n_kv, hd, past, batch = 8, 2, 128, 40, 29
+    n_head, n_kv, hd, past, batch = 8, 2, 128, 40, 149      # (too many pairs to be taken from the 4-bit rows)
     n_ctx = past + batch
     base = filled(rng, n_kv, hd, n_ctx, past)
     q, k, v = (dev(x) for x in (rng.standard_normal((batch, n_head, hd)).astype(np.float32), rows(rng, batch, n_kv, hd), rows(rng, batch, n_kv, hd)))
@@ -122,14 +123,86 @@ def test_prefill_block_output_and_other_kernel(ops):
     assert torch.equal(m16, m32.half())
 
 
-def test_many_heads_in_the_prologue(ops):
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("n_head,n_kv,hd,past,batch", [(12, 2, 128, 600, 5), (8, 8, 128, 512, 1), (32, 8, 64, 1003, 3), (16, 1, 128, 2000, 9),
+                                                       (28, 4, 128, 900, 18), (9, 1, 64, 700, 40), (5, 5, 64, 527, 17)])
+def test_short_chunk_behind_a_long_context(ops, n_head, n_kv, hd, past, batch, half):
+    """Walked from the 4-bit rows themselves: fp32 accuracy, each token with the positions up to its own."""
+    rng = np.random.default_rng(204)
+    n_ctx, rope_type, theta = past + batch + 9, past % 2, 5e5
+    cache = filled(rng, n_kv, hd, n_ctx, past)
+    q, k, v = rng.standard_normal((batch, n_head, hd)).astype(np.float32), rows(rng, batch, n_kv, hd), rows(rng, batch, n_kv, hd)
+    scale = 1.0 / math.sqrt(hd)
+    d_cache = dev(cache)
+    out = torch.full((batch + 1, n_head, hd), 9.0, dtype=torch.float16 if half else torch.float32, device="cuda")
+    ops.attn_prefill_q4(dev(q), dev(k), dev(v), d_cache, out, n_head, n_kv, hd, n_ctx, past, batch, scale, ops.FUSE_ALL, (rope_type, hd, theta, None))
+    torch.cuda.synchronize()
+    pos = np.arange(past, past + batch)
+    ref.write_rows(cache, hd, pos, ref.rope(k, pos, rope_type, hd, theta).astype(np.float32), v)
+    assert np.array_equal(d_cache.cpu().numpy(), cache)
+    K, V = ref.read_rows(cache, hd, past + batch)
+    want, most = ref.attend(ref.rope(q, pos, rope_type, hd, theta), K, V, past, scale)
+    got = out.float().cpu().numpy()
+    bound = decode_bound(most, scale, V) + (2.0 ** -11 * np.abs(want).max() if half else 0)
+    assert np.abs(got[:batch] - want).max() <= bound
+    assert (got[batch] == 9).all()
+    assert ops.prefill_status(n_head, n_kv, hd, batch, ops.prefill_q4_workspace(n_head, n_kv, hd, batch, n_ctx)) == 0
+
+
+def test_short_chunk_over_many_slices_and_in_a_graph(ops):
+    """20000 rows, so that a chunk's slices merge in two levels; the same bits from a graph, and from both kernels to their bounds."""
+    n_head, n_kv, hd, past, batch = 8, 2, 128, 20000, 6
+    n_ctx = past + batch
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    base = ops.KVCacheQ4(1, n_kv, n_ctx, hd).layer(0)
+    k, v = (torch.randn(past, n_kv, hd, device="cuda", generator=gen) for _ in range(2))
+    ops.kv_store_q4_batch(base, k, v, n_kv, hd, n_ctx, 0, past)
+    q = torch.randn(batch, n_head, hd, device="cuda", generator=gen)
+    kn, vn = (torch.randn(batch, n_kv, hd, device="cuda", generator=gen) for _ in range(2))
+    ws = torch.empty(ops.prefill_q4_workspace(n_head, n_kv, hd, batch, n_ctx).numel(), dtype=torch.uint8, device="cuda")
+
+    def call(cache, out):
+        ops.attn_prefill_q4(q, kn, vn, cache, out, n_head, n_kv, hd, n_ctx, past, batch, 0.0884, ops.FUSE_KV_APPEND, None, ws)
+
+    a, b = base.clone(), base.clone()
+    want, got, other = (torch.zeros(batch, n_head, hd, device="cuda") for _ in range(3))
+    call(a, want)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(b, got)
+    for _ in range(3):
+        b.copy_(base)
+        got.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(a, b)
+    kh, vh = (torch.zeros(n_kv, n_ctx, hd, dtype=torch.float16, device="cuda") for _ in range(2))
+    ops.kv_load_q4(a, kh, vh, n_kv, hd, n_ctx, 0, n_ctx)
+    K, V = kh.double().repeat_interleave(n_head // n_kv, 0), vh.double().repeat_interleave(n_head // n_kv, 0)
+    s = torch.einsum("bhd,hnd->bhn", q.double(), K) * 0.0884
+    s.masked_fill_(torch.arange(n_ctx, device="cuda")[None, None] > torch.arange(past, n_ctx, device="cuda")[:, None, None], -math.inf)
+    exact = torch.einsum("bhn,hnd->bhd", torch.softmax(s, -1), V)
+    most = float(torch.einsum("bhd,hnd->bhn", q.double().abs(), K.abs()).max())
+    bound = prefill_bound(most, 0.0884, vh.float().cpu().numpy(), False)          # (kh and vh are the rows rounded to fp16)
+    assert float((want - exact).abs().max()) <= bound
+    try:
+        ops.set_prefill_impl(1)                            # the fp16 copies and the warp-level kernel
+        call(b, other)
+    finally:
+        ops.set_prefill_impl(0)
+    assert float((other - exact).abs().max()) <= bound
+
+
+@pytest.mark.parametrize("batch", [3, 25])
+def test_many_heads_in_the_prologue(ops, batch):
     """More head rows than a prologue CTA has in flight at once."""
     rng = np.random.default_rng(203)
-    n_head, n_kv, hd, batch = 96, 16, 64, 3
+    n_head, n_kv, hd = 96, 16, 64
     q, k, v = rng.standard_normal((batch, n_head, hd)).astype(np.float32), rows(rng, batch, n_kv, hd), rows(rng, batch, n_kv, hd)
-    cache = np.zeros((n_kv, 1, 18 * hd), np.uint8)
+    cache = np.zeros((n_kv, 2, 18 * hd), np.uint8)
     d_cache, out = dev(cache), torch.empty(batch, n_head, hd, device="cuda")
-    ops.attn_prefill_q4(dev(q), dev(k), dev(v), d_cache, out, n_head, n_kv, hd, 7, 0, batch, 0.125, ops.FUSE_ALL, (1, hd, 1e6, None))
+    ops.attn_prefill_q4(dev(q), dev(k), dev(v), d_cache, out, n_head, n_kv, hd, 27, 0, batch, 0.125, ops.FUSE_ALL, (1, hd, 1e6, None))
     pos = np.arange(batch)
     ref.write_rows(cache, hd, pos, ref.rope(k, pos, 1, hd, 1e6).astype(np.float32), v)
     assert np.array_equal(d_cache.cpu().numpy(), cache)
@@ -305,9 +378,10 @@ def test_two_streams_with_workspaces_of_their_own(ops):
         ops.set_stream(None)
 
 
-def test_prefill_captured(ops):
+@pytest.mark.parametrize("batch", [40, 160])
+def test_prefill_captured(ops, batch):
     rng = np.random.default_rng(223)
-    n_head, n_kv, hd, past, batch = 8, 2, 128, 50, 40
+    n_head, n_kv, hd, past = 8, 2, 128, 50
     n_ctx = past + batch
     base = dev(filled(rng, n_kv, hd, n_ctx, past))
     q, k, v = (dev(rng.standard_normal((batch, h, hd)).astype(np.float32)) for h in (n_head, n_kv, n_kv))
@@ -331,11 +405,11 @@ def test_prefill_captured(ops):
         assert torch.equal(got, want) and torch.equal(a, b)
 
 
-@pytest.mark.parametrize("n_head,n_kv,hd", [(8, 2, 128), (12, 4, 64)])
-def test_unfused_prefill_reads_what_the_store_call_wrote(ops, n_head, n_kv, hd):
+@pytest.mark.parametrize("n_head,n_kv,hd,batch", [(8, 2, 128, 30), (12, 4, 64, 30), (8, 2, 128, 150)])
+def test_unfused_prefill_reads_what_the_store_call_wrote(ops, n_head, n_kv, hd, batch):
     """Rows stored by the unfused call, then the chunk with and without the rotation of q: the fused call's bytes and outputs."""
     rng = np.random.default_rng(224)
-    past, batch = 21, 30
+    past = 21
     n_ctx, scale, rope = past + batch, 1.0 / math.sqrt(hd), (1, hd, 1e6, None)
     base = filled(rng, n_kv, hd, n_ctx, past)
     q, k, v = rng.standard_normal((batch, n_head, hd)).astype(np.float32), rows(rng, batch, n_kv, hd), rows(rng, batch, n_kv, hd)
