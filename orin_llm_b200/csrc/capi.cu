@@ -605,26 +605,31 @@ int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void
 }
 
 // A short chunk is walked by the decode kernel, eight (token, head) pairs per CTA, straight from the 4-bit rows; a long one by the
-// prefill kernels, which take more pairs at a time but read fp16 copies, on one CTA per kv head and 128 pairs.  The limit is on
-// the eights of pairs of all kv heads; the smaller for heads of 128, whose prefill kernel is the tensor-core one.  Microseconds
-// per call, short way against long way: 32/8 heads of 128 behind 8192 rows, 8 tokens 22 against 63, 32 tokens (128 eights) 55
-// against 66, 64 tokens 93 against 67; behind 64 rows 10.4 against 11.8 and 11.1 against 12.3.  32/8 heads of 64 behind 8192 rows,
-// 8 tokens 16 against 112, 64 tokens (256 eights) 56 against 114.  The worst inside the limit is 28/4 heads, 32 tokens behind 512
-// rows: 15.4 against 14.5.
-static int chunk_blocks(int n_head, int n_kv, int head_dim, int batch) {
+// prefill kernels, which take more pairs at a time but read fp16 copies and are a launch or two more.  The limit is on the
+// eights of pairs of all kv heads: the first way's time goes with eights x rows, the second's hardly depends on the number of pairs
+// while that is small, so the limit falls with the rows; it is higher for heads of 64, whose prefill kernel is the warp-level one.
+// Microseconds per call, short way against long way, 32/8 heads of 128: 16 tokens (64 eights) behind 1024 rows 17.0 against
+// 18.7, 2048 18.4 against 20.2, 4096 23.7 against 21.6; 8 tokens behind 4096 rows 17.6 against 21.6, 8192 22.5 against 24.4; 4
+// tokens behind 32768 rows 33 against 61.  Heads of 64: 64 tokens (256 eights) behind 1024 rows 16.0 against 21.5, 2048 21.8 against 21.6;
+// 8 tokens behind 8192 rows 16.2 against 21.1, 32768 32 against 48.
+static int chunk_blocks(int n_head, int n_kv, int head_dim, int n_past, int batch) {
     const long long blocks = ((long long)batch * (n_head / n_kv) + 7) / 8;
-    return blocks * n_kv <= (head_dim == 128 ? 128 : 256) ? (int)blocks : 0;
+    const int limit = head_dim == 128 ? min(128, 24 + (96 << 10) / max(n_past, 1)) : min(256, 32 + (224 << 10) / max(n_past, 1));
+    return blocks * n_kv <= limit ? (int)blocks : 0;
 }
 constexpr size_t kChunkScratch = 4u << 20;      // partial results of a chunk's slices: at most 2 * 160 slices of 8 rows, and their groups
 
-// [fp16 queries][status word, 256 bytes][fp16 K rows][fp16 V rows]: the first two as in oattn_prefill.  A short chunk has its fp32
+constexpr size_t kSplitRows = (size_t)kSplitCtas * 128;       // a long chunk's (token, head) rows over all slices
+
+// [fp16 queries][status word, 256 bytes][fp16 K rows][fp16 V rows][slices' outputs][(maximum, sum)]: the first two as in oattn_prefill.  A short chunk has its fp32
 // queries and partial results behind the status word instead of the rows.
 size_t oattn_prefill_q4_workspace_bytes(int n_head, int n_kv, int head_dim, int max_batch, int max_rows) {
     const size_t head = oattn_prefill_workspace_bytes(n_head, n_kv, head_dim, max_batch);
     if (!head || max_rows < max_batch) return 0;
     const size_t copies = 2 * align256((size_t)n_kv * max_rows * head_dim * sizeof(__half));
     const size_t chunk = align256((size_t)max_batch * n_head * head_dim * sizeof(float)) + kChunkScratch;
-    return head + (copies > chunk ? copies : chunk);
+    const size_t long_way = copies + kSplitRows * (head_dim * sizeof(float) + sizeof(float2));
+    return head + (long_way > chunk ? long_way : chunk);
 }
 
 int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, uint16_t* out_f16, int n_head,
@@ -669,7 +674,7 @@ int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, voi
     rope_freq_table(a.rope, p.freq);
     cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e;
-    const int blocks = mmq || g_prefill_impl != 0 ? 0 : chunk_blocks(n_head, n_kv, head_dim, batch);
+    const int blocks = mmq || g_prefill_impl != 0 ? 0 : chunk_blocks(n_head, n_kv, head_dim, n_past, batch);
     p.q32 = nullptr; p.tickets = nullptr; p.n_tickets = 0;
     if (blocks) {
         DecodeQ4Args c;
@@ -696,6 +701,13 @@ int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, voi
             e = launch_decode_q4(c, head_dim, s, &g_launches);
             return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "prefill (short chunk) launch");
         }
+    }
+    const bool tc = head_dim == 128 && g_prefill_impl == 0;
+    if (!mmq && (tc || head_dim == 64)) {
+        a.n_split = max(1, (tc ? prefill_tc_splits : prefill_mma_splits)(n_head, n_kv, n_past, batch, dev->sm_count));
+        uint8_t* parts = wsb + head + 2 * align256((size_t)n_kv * rows * head_dim * sizeof(__half));
+        a.part_o = reinterpret_cast<float*>(parts);
+        a.part_ml = reinterpret_cast<float*>(parts + kSplitRows * head_dim * sizeof(float));
     }
     e = launch_prefill_q4_prologue(p, s, &g_launches);
     if (e != cudaSuccess) return cuda_fail(e, "prefill (4-bit cache) prologue launch");

@@ -103,6 +103,8 @@ struct TcArgs {
     int mmq_ds4;
     int* status;
     int n_head, n_kv, n_past, batch, G, TQ;   // TQ = floor(128 / G) tokens per tile
+    float2* part_ml;       // SPLIT: running maximum and sum of each row and slice; the unscaled output goes to part_o through tmO
+    int n_split;
     int out_tma;           // the output leaves through shared memory and bulk tensor stores (tmO is valid): 1 fp32, 2 fp16
 };
 
@@ -302,6 +304,8 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) {
 constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 constexpr uint32_t IDESC_PV = IDESC_S | (1u << 16);
 
+// SPLIT (see PrefillArgs): a CTA walks one of n_split slices of its tile's KV blocks and leaves the unscaled output.
+template <bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const TcArgs p) {
@@ -320,7 +324,11 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int t0 = tile * p.TQ;
     const int ntok = min(p.TQ, p.batch - t0);
     const int kv_end = p.n_past + t0 + ntok;              // rows any query of this tile may see
-    const int nb = (kv_end + BN - 1) / BN;
+    const int nb_all = (kv_end + BN - 1) / BN;
+    const int split = SPLIT ? blockIdx.z : 0;
+    const int jb = SPLIT ? (int)((long long)nb_all * split / p.n_split) : 0;       // this CTA's blocks are jb + (0 .. nb - 1)
+    const int nb = SPLIT ? (int)((long long)nb_all * (split + 1) / p.n_split) - jb : nb_all;
+    const int kv0 = jb * BN;
 
     if (tid == 0) {
         mbar_init(bar(Q_FULL), 1);
@@ -375,8 +383,8 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (j >= NKS) ok = mbar_wait(bar(S_FULL + s), ((j / NKS) - 1) & 1, s_abort);     // S_(j-NKS) done: stage free
                 if (!ok) return;
                 mbar_expect_tx(bar(K_FULL + s), TILE);
-                tma_load_3d(sbase + OFF_K + s * TILE, &tmK, 0, j * BN, kvh, bar(K_FULL + s));
-                tma_load_3d(sbase + OFF_K + s * TILE + SLAB, &tmK, 64, j * BN, kvh, bar(K_FULL + s));
+                tma_load_3d(sbase + OFF_K + s * TILE, &tmK, 0, kv0 + j * BN, kvh, bar(K_FULL + s));
+                tma_load_3d(sbase + OFF_K + s * TILE + SLAB, &tmK, 64, kv0 + j * BN, kvh, bar(K_FULL + s));
                 ++k_issued[s];
             };
             auto load_v = [&](int j) {
@@ -384,8 +392,8 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (j >= NVS) ok = mbar_wait(bar(PV_DONE + s), ((j / NVS) - 1) & 1, s_abort);    // P V of block j-2 done: stage free
                 if (!ok) return;
                 mbar_expect_tx(bar(V_FULL + s), TILE);
-                tma_load_3d(sbase + OFF_V + s * TILE, &tmV, 0, j * BN, kvh, bar(V_FULL + s));
-                tma_load_3d(sbase + OFF_V + s * TILE + SLAB, &tmV, 64, j * BN, kvh, bar(V_FULL + s));
+                tma_load_3d(sbase + OFF_V + s * TILE, &tmV, 0, kv0 + j * BN, kvh, bar(V_FULL + s));
+                tma_load_3d(sbase + OFF_V + s * TILE + SLAB, &tmV, 64, kv0 + j * BN, kvh, bar(V_FULL + s));
                 ++v_issued[s];
             };
             // consumption order of the MMA warp: K_0..K_2, then V_j, K_(j+3)
@@ -487,7 +495,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const int tok = row / p.G, hg = row - tok * p.G;
         const int tglob = t0 + tok;
         const bool valid = tok < ntok;
-        const int vis = p.n_past + tglob;                   // last visible cache row
+        const int vis = p.n_past + tglob - kv0;             // last visible cache row, from the CTA's first one
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
         const uint32_t to = TM_O + lane_addr;               // the accumulator row of this thread
         float* s_mref = reinterpret_cast<float*>(smem + OFF_MREF);
@@ -509,7 +517,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tmem_ld32(ts + 64, v + 64);
             tmem_ld32(ts + 96, v + 96);
             if (tid == 128 || tid == 256) TRACE(1 + team, 2, j);
-            if (j * BN + BN - 1 > p.n_past + t0) {          // block reaches past the tile's first query: mask
+            if (j * BN + BN - 1 > p.n_past + t0 - kv0) {          // block reaches past the tile's first query: mask
                 const int lim = vis - j * BN;               // columns <= lim are visible
 #pragma unroll
                 for (int i = 0; i < 128; ++i) if (i > lim) v[i] = -CUDART_INF_F;
@@ -611,16 +619,19 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const float M = fmaxf(m_l, other.x);
             const float w_me = (m_l == -CUDART_INF_F) ? 0.f : fast_exp2(m_l - M);
             const float w_ot = (other.x == -CUDART_INF_F) ? 0.f : fast_exp2(other.x - M);
-            const float inv = 1.f / (w_me * l + w_ot * other.y);
+            const float inv = SPLIT ? 1.f : 1.f / (w_me * l + w_ot * other.y);
+            const int ptok = SPLIT ? split * (gridDim.x * p.TQ) + tglob : tglob;      // row of the output, or of the slices' outputs
+            if (SPLIT && team == 0 && valid)
+                p.part_ml[(size_t)ptok * p.n_head + kvh * p.G + hg] = make_float2(M, w_me * l + w_ot * other.y);
             // this thread writes columns [64 team, 64 team + 64) of its row
-            float* dst = p.out + ((size_t)tglob * p.n_head + kvh * p.G + hg) * HD + 64 * team;
+            float* dst = p.out + ((size_t)ptok * p.n_head + kvh * p.G + hg) * HD + 64 * team;
 #pragma unroll 1
             for (int c = 0; c < 2; ++c) {
                 float a[32];
                 tmem_ld32(to + 64 * team + 32 * c, a);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) a[i] *= inv;
-                if (p.out_tma == 2) {
+                if (!SPLIT && p.out_tma == 2) {
                     // fp16: two slabs of 64 columns, one per team, the same way
                     uint8_t* rowp = smem + OFF_K + team * (BM * 128) + row * 128;
 #pragma unroll
@@ -641,7 +652,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     for (int i = 0; i < 8; ++i)
                         *reinterpret_cast<float4*>(dst + 32 * c + 4 * i) = make_float4(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]);
                 }
-                if (valid && p.out_mmq) {
+                if (!SPLIT && valid && p.out_mmq) {
                     // The 32 values are one quantisation group of the 128-value block of (head, token): what
                     // quantize_mmq_q8_1_k (src/kernels.cu:160-205) computes with a shuffle over eight lanes is a
                     // reduction over this thread's registers here.
@@ -673,12 +684,12 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             asm volatile("bar.sync 1, 256;\n" ::: "memory");
             if (tid == 32 * kFirstSoftmaxWarp && !*s_abort) {
                 // rows past the batch (a ragged last tile) lie outside the tensor map and are not written
-                if (p.out_tma == 2) {
+                if (!SPLIT && p.out_tma == 2) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) tma_store_3d(&tmO, 64 * c, kvh * p.G, t0, sbase + OFF_K + c * (BM * 128));
                 } else {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tma_store_3d(&tmO, 32 * c, kvh * p.G, t0, sbase + OFF_K + c * (BM * 128));
+                    for (int c = 0; c < 4; ++c) tma_store_3d(&tmO, 32 * c, kvh * p.G, (SPLIT ? split * (int)(gridDim.x * p.TQ) : 0) + t0, sbase + OFF_K + c * (BM * 128));
                 }
                 asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
                 asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");  // shared memory stays valid until it has been read
@@ -740,7 +751,19 @@ cudaError_t prefill_tc_set_attributes() {
         if (qres != cudaDriverEntryPointSuccess || !fn) return cudaErrorNotSupported;
         g_encode = reinterpret_cast<EncodeTiledFn>(fn);
     }
-    return cudaFuncSetAttribute(prefill_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    const cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(prefill_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+}
+
+// A CTA takes about 0.9 us a block; writing the slices' outputs and joining them 5 to 6 together, so eight blocks have to be saved.  64
+// tokens of 32/8 heads behind 8192 rows (16 tiles, 9 slices) 29 us against 67, prologue included, 256 tokens (64 tiles, 2
+// slices) 52 against 73; nine blocks in two slices 22 against 19.
+int prefill_tc_splits(int n_head, int n_kv, int n_past, int batch, int sm_count) {
+    const int TQ = 128 / (n_head / n_kv);
+    const long long ctas = (long long)n_kv * ((batch + TQ - 1) / TQ);
+    const int blocks = (n_past + min(batch, TQ) + BN - 1) / BN;          // of the shortest tile
+    const int n = (int)min(min((long long)min(sm_count, kSplitCtas) / ctas, (long long)blocks / kSplitMinBlocks), (long long)kMaxPrefillSplits);
+    return n > 1 && blocks - (blocks + n - 1) / n >= 8 ? n : 1;
 }
 
 cudaError_t launch_prefill_tc(const PrefillArgs& a, int sm_count, cudaStream_t stream, unsigned long long* launches) {
@@ -759,19 +782,25 @@ cudaError_t launch_prefill_tc(const PrefillArgs& a, int sm_count, cudaStream_t s
     const uint64_t orow = HD * sizeof(float);
     const bool out_tma = a.out && !((uintptr_t)a.out & 15) && make_out_map(&tmO, a.out, a.n_head, a.batch, orow, orow * a.n_head, G, TQ);
     // ... or the fp16 one, which has no other way out (the C entry checked its alignment)
-    if (a.out16 && !make_map(&tmO, a.out16, a.n_head, a.batch, rowb, rowb * a.n_head, G, TQ)) return cudaErrorInvalidValue;
+    const int tiles = (a.batch + TQ - 1) / TQ;
+    if (a.n_split > 1) {
+        if (!make_out_map(&tmO, a.part_o, a.n_head, (uint64_t)a.n_split * tiles * TQ, orow, orow * a.n_head, G, TQ)) return cudaErrorInvalidValue;
+    } else if (a.out16 && !make_map(&tmO, a.out16, a.n_head, a.batch, rowb, rowb * a.n_head, G, TQ)) return cudaErrorInvalidValue;
     TcArgs t;
-    t.out_tma = a.out16 ? 2 : (out_tma ? 1 : 0);
+    t.out_tma = a.n_split > 1 ? 1 : (a.out16 ? 2 : (out_tma ? 1 : 0));
+    t.part_ml = reinterpret_cast<float2*>(a.part_ml);
+    t.n_split = a.n_split;
     t.out = a.out;
     t.out16 = a.out16;
     t.out_mmq = a.out_mmq;
     t.mmq_ds4 = a.mmq_ds4;
     t.status = a.status;
     t.n_head = a.n_head; t.n_kv = a.n_kv; t.n_past = a.n_past; t.batch = a.batch; t.G = G; t.TQ = TQ;
-    dim3 grid((a.batch + TQ - 1) / TQ, a.n_kv);
-    const cudaError_t e = launch_dependent(prefill_tc_kernel, grid, kThreads, SMEM_BYTES, stream, 1, tmQ, tmK, tmV, tmO, t);
+    const dim3 grid(tiles, a.n_kv, a.n_split);
+    const cudaError_t e = a.n_split > 1 ? launch_dependent(prefill_tc_kernel<true>, grid, kThreads, SMEM_BYTES, stream, 1, tmQ, tmK, tmV, tmO, t)
+                                        : launch_dependent(prefill_tc_kernel<false>, grid, kThreads, SMEM_BYTES, stream, 1, tmQ, tmK, tmV, tmO, t);
     if (launches) *launches += 1;
-    return e;
+    return e != cudaSuccess || a.n_split == 1 ? e : launch_prefill_merge(a, tiles * TQ, stream, launches);
 }
 
 } // namespace oattn

@@ -416,8 +416,8 @@ def attn_decode_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, d
 def attn_prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse=FUSE_ALL, rope=None,
                     workspace=None, ext=None):
     """attn_prefill over one layer of a 4-bit cache, the chunk's rows quantised and appended first.  out: fp32 or fp16
-    [batch][n_head][head_dim] (the attention runs on fp16 operands either way).  The default workspace holds one layer's rows
-    in fp16, for all n_ctx of them; calls that may run at the same time need workspaces of their own."""
+    [batch][n_head][head_dim].  The default workspace holds one layer's rows in fp16, for all n_ctx of them; calls that may run
+    at the same time need workspaces of their own."""
     ws = workspace if workspace is not None else prefill_q4_workspace(n_head, n_kv, head_dim, batch, max(n_ctx, batch))
     ea, keep = _ext_address(ext) if ext else (None, None)
     capi.check(_q4().prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse, rope, ea, ws,

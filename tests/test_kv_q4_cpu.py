@@ -22,9 +22,11 @@ def test_sizes(ops):
     for n_kv, hd, n_ctx in ((0, 64, 1), (1, 96, 16), (1, 128, 0), (-1, 128, 5), (1, 128, (1 << 30) + 1)):
         assert L.oattn_kv_q4_bytes(n_kv, hd, n_ctx) == ops.kv_q4_bytes(n_kv, hd, n_ctx) == 0
     head = L.oattn_prefill_workspace_bytes(32, 8, 128, 512)
-    assert L.oattn_prefill_q4_workspace_bytes(32, 8, 128, 512, 8704) == head + 2 * 8 * 8704 * 128 * 2      # the rows in fp16
+    # the rows in fp16 and the slices' outputs, maxima and sums
+    assert L.oattn_prefill_q4_workspace_bytes(32, 8, 128, 512, 8704) == head + 2 * 8 * 8704 * 128 * 2 + 148 * 128 * (128 * 4 + 8)
     # ... or, where that is more, a short chunk's fp32 queries and partial results
-    assert L.oattn_prefill_q4_workspace_bytes(8, 2, 64, 4, 20) == L.oattn_prefill_workspace_bytes(8, 2, 64, 4) + 4 * 8 * 64 * 4 + (4 << 20)
+    assert (L.oattn_prefill_q4_workspace_bytes(8, 2, 64, 1200, 1200) ==
+            L.oattn_prefill_workspace_bytes(8, 2, 64, 1200) + max(1200 * 8 * 64 * 4 + (4 << 20), 2 * 2 * 1200 * 64 * 2 + 148 * 128 * (64 * 4 + 8)))
     assert L.oattn_prefill_q4_workspace_bytes(32, 8, 128, 512, 511) == 0          # fewer rows than the chunk alone has
     assert L.oattn_prefill_q4_workspace_bytes(32, 8, 96, 512, 8704) == 0
 
