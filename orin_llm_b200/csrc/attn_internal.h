@@ -141,10 +141,11 @@ struct PrefillArgs {
     uint8_t* out_mmq = nullptr;   // optional: the output as block_q8_1_mmq blocks [head][batch], 144 bytes each
     __half* out16 = nullptr;      // optional: the output as fp16 [batch][n_head][hd], instead of `out`
     int mmq_ds4 = 0;              // scales as fp16 (d, sum) pairs instead of fp32 d
-    // n_split > 1: every query tile's KV rows are cut into that many slices, one CTA each, and a further launch joins them (fp32 and
-    // fp16 outputs only).  Slice s of token t and head h has its unscaled output and its (maximum, sum) at row
+    // The tcgen05 kernel only.  n_split > 1: every query tile's KV rows are cut into that many slices, one CTA each, and a further
+    // launch joins them (fp32 and fp16 outputs only).  Slice s of token t and head h has its unscaled output and its (maximum, sum) at row
     // (s * tokens + t) * n_head + h, tokens = batch rounded up to whole tiles.
     int n_split = 1;
+    bool tc_hd64 = false;         // heads of 64 on the tcgen05 kernel, too
     float* part_o = nullptr;
     float* part_ml = nullptr;
 };
@@ -153,8 +154,6 @@ constexpr int kSplitMinBlocks = 4;            // 128-row blocks that a slice has
 // Slices for a call: as many as fill the SMs, fewer for a short context, 1 or less: not worth it.  Together they have at most
 // kSplitCtas * 128 rows.
 int prefill_tc_splits(int n_head, int n_kv, int n_past, int batch, int sm_count);
-int prefill_mma_splits(int n_head, int n_kv, int n_past, int batch, int sm_count);
-cudaError_t launch_prefill_merge(const PrefillArgs& a, int tokens, cudaStream_t stream, unsigned long long* launches);
 
 // Prologue shared by both prefill kernels: RoPE(q) -> q16, RoPE(k_new) + fp16 append of k_new, v_new.
 cudaError_t launch_prefill_prologue(const PrefillArgs& a, cudaStream_t stream, unsigned long long* launches);

@@ -607,11 +607,11 @@ int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void
 // A short chunk is walked by the decode kernel, eight (token, head) pairs per CTA, straight from the 4-bit rows; a long one by the
 // prefill kernels, which take more pairs at a time but read fp16 copies and are a launch or two more.  The limit is on the
 // eights of pairs of all kv heads: the first way's time goes with eights x rows, the second's hardly depends on the number of pairs
-// while that is small, so the limit falls with the rows; it is higher for heads of 64, whose prefill kernel is the warp-level one.
+// while that is small, so the limit falls with the rows; heads of 64 are half the work of the first way and little less of the second's.
 // Microseconds per call, short way against long way, 32/8 heads of 128: 16 tokens (64 eights) behind 1024 rows 17.0 against
 // 18.7, 2048 18.4 against 20.2, 4096 23.7 against 21.6; 8 tokens behind 4096 rows 17.6 against 21.6, 8192 22.5 against 24.4; 4
-// tokens behind 32768 rows 33 against 61.  Heads of 64: 64 tokens (256 eights) behind 1024 rows 16.0 against 21.5, 2048 21.8 against 21.6;
-// 8 tokens behind 8192 rows 16.2 against 21.1, 32768 32 against 48.
+// tokens behind 32768 rows 33 against 61.  Heads of 64: 64 tokens (256 eights) behind 512 rows 13.1 against 14.6, 1024 16.0
+// against 18.2; 16 tokens behind 4096 rows 17.2 against 18.0; 8 tokens behind 8192 rows 16.3 against 21.0, 32768 32 against 37.
 static int chunk_blocks(int n_head, int n_kv, int head_dim, int n_past, int batch) {
     const long long blocks = ((long long)batch * (n_head / n_kv) + 7) / 8;
     const int limit = head_dim == 128 ? min(128, 24 + (96 << 10) / max(n_past, 1)) : min(256, 32 + (224 << 10) / max(n_past, 1));
@@ -702,9 +702,9 @@ int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, voi
             return e == cudaSuccess ? OATTN_OK : cuda_fail(e, "prefill (short chunk) launch");
         }
     }
-    const bool tc = head_dim == 128 && g_prefill_impl == 0;
-    if (!mmq && (tc || head_dim == 64)) {
-        a.n_split = max(1, (tc ? prefill_tc_splits : prefill_mma_splits)(n_head, n_kv, n_past, batch, dev->sm_count));
+    a.tc_hd64 = true;
+    if (!mmq && g_prefill_impl == 0) {
+        a.n_split = prefill_tc_splits(n_head, n_kv, n_past, batch, dev->sm_count);
         uint8_t* parts = wsb + head + 2 * align256((size_t)n_kv * rows * head_dim * sizeof(__half));
         a.part_o = reinterpret_cast<float*>(parts);
         a.part_ml = reinterpret_cast<float*>(parts + kSplitRows * head_dim * sizeof(float));

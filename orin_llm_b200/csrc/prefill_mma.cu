@@ -30,8 +30,7 @@ struct PrefillSmem {
     static constexpr int TOTAL = Q_OFF + 64 * ROWB;
 };
 
-// SPLIT (see PrefillArgs): a CTA walks one of n_split slices of its rows and leaves the unscaled output.
-template <int HD, bool SPLIT>
+template <int HD>
 __global__ void __launch_bounds__(kThreads, 2) prefill_mma_kernel(const PrefillArgs p) {
     using L = PrefillSmem<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -45,17 +44,14 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_mma_kernel(const PrefillA
     const int t0 = tb * TB;
     const int ntok = min(TB, p.batch - t0);
     const int kv_end = p.n_past + t0 + ntok;     // rows any query of this CTA may see
-    const int nt_all = (kv_end + kTile - 1) / kTile;
-    const int split = SPLIT ? blockIdx.z : 0;
-    const int tile0 = SPLIT ? (int)((long long)nt_all * split / p.n_split) : 0;
-    const int nt = SPLIT ? (int)((long long)nt_all * (split + 1) / p.n_split) - tile0 : nt_all;
+    const int nt = (kv_end + kTile - 1) / kTile;
 
     const __half* Kg = reinterpret_cast<const __half*>(p.kc) + (size_t)kvh * p.n_ctx * HD;
     const __half* Vg = reinterpret_cast<const __half*>(p.vc) + (size_t)kvh * p.n_ctx * HD;
     const uint32_t smem_base = smem_u32(smem);
 
     auto load_tile = [&](int tile, int stage) {
-        const int row0 = (tile0 + tile) * kTile;
+        const int row0 = tile * kTile;
         const uint32_t sb = smem_base + stage * L::STAGE_BYTES;
         constexpr int PER_MAT = kTile * L::CHUNKS;
 #pragma unroll
@@ -116,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_mma_kernel(const PrefillA
             cp_async_commit();
         }
         const int stage = it % kStages;
-        const int row0 = (tile0 + it) * kTile;
+        const int row0 = it * kTile;
         const uint32_t sK = smem_base + stage * L::STAGE_BYTES;
         const uint32_t sV = sK + L::TILE_BYTES;
 
@@ -196,14 +192,6 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_mma_kernel(const PrefillA
         const int R = warp * 16 + r + 8 * hh;
         const int tok = R / G, hg = R % G;
         if (tok < ntok) {
-            if constexpr (SPLIT) {
-                const size_t row = ((size_t)split * (gridDim.x * TB) + t0 + tok) * p.n_head + kvh * G + hg;
-                if (t == 0) reinterpret_cast<float2*>(p.part_ml)[row] = make_float2(m_run[hh], l);
-#pragma unroll
-                for (int j = 0; j < HD / 8; ++j)
-                    *reinterpret_cast<float2*>(p.part_o + row * HD + 8 * j + 2 * t) = make_float2(o[j][2 * hh], o[j][2 * hh + 1]);
-                continue;
-            }
             const float inv = 1.f / l;
             if (p.out16) {
                 __half* dst16 = p.out16 + ((size_t)(t0 + tok) * p.n_head + kvh * G + hg) * HD;
@@ -220,83 +208,22 @@ __global__ void __launch_bounds__(kThreads, 2) prefill_mma_kernel(const PrefillA
     }
 }
 
-// Joins the slices of a split call: a row's HD/4 threads take 4 dims each.  Bound by reading the slices, from L2: 64 tokens of 32
-// heads in eight slices are 8 MB.
-template <int HD>
-__global__ void __launch_bounds__(256) prefill_merge_kernel(const PrefillArgs p, int tokens) {
-    pdl_trigger();
-    pdl_wait();
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long row = at / (HD / 4);                     // (token, head)
-    const int c4 = (int)(at % (HD / 4));
-    if (row >= (long long)p.batch * p.n_head) return;
-    const size_t step = (size_t)tokens * p.n_head;
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row;
-    const float4* o = reinterpret_cast<const float4*>(p.part_o) + row * (HD / 4) + c4;
-    float M = -CUDART_INF_F;
-#pragma unroll 4
-    for (int s = 0; s < p.n_split; ++s) M = fmaxf(M, ml[s * step].x);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float L = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < p.n_split; ++s) {
-        const float2 x = ml[s * step];
-        const float4 v = o[s * step * (HD / 4)];
-        const float w = x.x == -CUDART_INF_F ? 0.f : fast_exp2(x.x - M);       // a slice that the mask hides from this row
-        L += w * x.y;
-        acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
-    }
-    const float inv = 1.f / L;
-    acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
-    if (p.out16) reinterpret_cast<uint2*>(p.out16)[at] = make_uint2(pack_half2(acc.x, acc.y), pack_half2(acc.z, acc.w));
-    else         reinterpret_cast<float4*>(p.out)[at] = acc;
-}
-
-template <int HD>
-cudaError_t set_attributes() {
-    const cudaError_t e = cudaFuncSetAttribute(prefill_mma_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefillSmem<HD>::TOTAL);
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(prefill_mma_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefillSmem<HD>::TOTAL);
-}
-
 } // namespace
 
 cudaError_t prefill_mma_set_attributes() {
-    const cudaError_t e = set_attributes<128>();
-    return e != cudaSuccess ? e : set_attributes<64>();
-}
-
-cudaError_t launch_prefill_merge(const PrefillArgs& a, int tokens, cudaStream_t stream, unsigned long long* launches) {
-    const long long threads = (long long)a.batch * a.n_head * (a.head_dim / 4);
-    const dim3 grid((unsigned)((threads + 255) / 256));
-    const cudaError_t e = a.head_dim == 128 ? launch_dependent(prefill_merge_kernel<128>, grid, 256, 0, stream, 1, a, tokens)
-                                            : launch_dependent(prefill_merge_kernel<64>, grid, 256, 0, stream, 1, a, tokens);
-    if (launches) *launches += 1;
-    return e;
-}
-
-// Two CTAs per SM; a 64-row tile takes one about 0.9 us.  64 tokens of 32/8 heads behind 8192 rows (32 CTAs, 9 slices) 32 us
-// against 114, behind 1024 rows (2 slices) 21.5 against 23.
-int prefill_mma_splits(int n_head, int n_kv, int n_past, int batch, int sm_count) {
-    const int TB = 64 / (n_head / n_kv);
-    const long long ctas = (long long)n_kv * ((batch + TB - 1) / TB);
-    const int blocks = (n_past + min(batch, TB) + 127) / 128;            // of the shortest tile
-    return (int)min(min(2ll * min(sm_count, kSplitCtas) / ctas, (long long)blocks / kSplitMinBlocks), (long long)kMaxPrefillSplits);
+    cudaError_t e = cudaFuncSetAttribute(prefill_mma_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefillSmem<128>::TOTAL);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(prefill_mma_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefillSmem<64>::TOTAL);
 }
 
 cudaError_t launch_prefill_mma(const PrefillArgs& a, cudaStream_t stream, unsigned long long* launches) {
     const int G = a.n_head / a.n_kv;
     const int TB = 64 / G;
-    const dim3 grid((a.batch + TB - 1) / TB, a.n_kv, a.n_split);
-    if (a.n_split > 1) {
-        if (a.head_dim == 128) prefill_mma_kernel<128, true><<<grid, kThreads, PrefillSmem<128>::TOTAL, stream>>>(a);
-        else                   prefill_mma_kernel<64, true><<<grid, kThreads, PrefillSmem<64>::TOTAL, stream>>>(a);
-    } else {
-        if (a.head_dim == 128) prefill_mma_kernel<128, false><<<grid, kThreads, PrefillSmem<128>::TOTAL, stream>>>(a);
-        else                   prefill_mma_kernel<64, false><<<grid, kThreads, PrefillSmem<64>::TOTAL, stream>>>(a);
-    }
+    dim3 grid((a.batch + TB - 1) / TB, a.n_kv);
+    if (a.head_dim == 128) prefill_mma_kernel<128><<<grid, kThreads, PrefillSmem<128>::TOTAL, stream>>>(a);
+    else                   prefill_mma_kernel<64><<<grid, kThreads, PrefillSmem<64>::TOTAL, stream>>>(a);
     if (launches) *launches += 1;
-    const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess || a.n_split == 1 ? e : launch_prefill_merge(a, (int)grid.x * TB, stream, launches);
+    return cudaGetLastError();
 }
 
 } // namespace oattn

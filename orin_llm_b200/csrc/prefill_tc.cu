@@ -9,7 +9,9 @@
 // R -> token t0 + R/G, head kvh*G + R%G (G = n_head/n_kv), so a single pass over the kv head's K/V rows
 // serves all G query heads of floor(128/G) tokens (when G does not divide 128 the last few tile rows are
 // zero and unused).  The KV sequence is walked in blocks of
-// 128 rows.  384 threads = three warpgroups (warps 2 and 3 only hold the place that makes the softmax teams whole warpgroups,
+// 128 rows.  Heads of 128; heads of 64 (one slab per tile, half the MMA work, the same softmax) for callers that ask for them:
+// 512 tokens of 32/8 heads of 64 behind 8192 rows 77 us with the prologue, 157 on the warp-level kernel.
+// 384 threads = three warpgroups (warps 2 and 3 only hold the place that makes the softmax teams whole warpgroups,
 // so that registers can be moved to them); three roles:
 //   warp 0   (one lane)  TMA producer: Q tile once, then 128-row K blocks (three-stage ring) and V blocks
 //                        (two-stage ring) with cp.async.bulk.tensor, 128-byte swizzle, no multicast; rows
@@ -57,9 +59,9 @@ namespace {
 constexpr int kThreads = 384;                   // three warpgroups: {TMA, MMA, two idle warps}, softmax team 0, softmax team 1
 constexpr int kFirstSoftmaxWarp = 4;
 constexpr int kRegsService = 104, kRegsSoftmax = 200;   // per-thread register budgets after the set-up (setmaxnreg)
-constexpr int BM = 128, BN = 128, HD = 128;
+constexpr int BM = 128, BN = 128;
 constexpr int SLAB = 128 * 128;                 // bytes of one 128-row x 64-element fp16 slab
-constexpr int TILE = 2 * SLAB;                  // a 128 x 128 fp16 tile = two slabs
+constexpr int TILE = 2 * SLAB;                  // a 128 x 128 fp16 tile = two slabs (heads of 64 use the first one)
 constexpr int OFF_Q = 0;
 constexpr int NKS = 3, NVS = 2;                 // K and V ring depths
 constexpr int NSB = 3;                          // score buffers in TMEM
@@ -190,6 +192,21 @@ __device__ __forceinline__ void tc_group_ss(uint32_t d_tmem, const uint64_t (&a)
                    "l"(a[0]), "l"(a[1]), "l"(a[2]), "l"(a[3]), "l"(a[4]), "l"(a[5]), "l"(a[6]), "l"(a[7]),
                    "l"(b[0]), "l"(b[1]), "l"(b[2]), "l"(b[3]), "l"(b[4]), "l"(b[5]), "l"(b[6]), "l"(b[7]) : "memory");
 }
+// The same with four K16 steps, for heads of 64.
+__device__ __forceinline__ void tc_group_ss(uint32_t d_tmem, const uint64_t (&a)[4], const uint64_t (&b)[4], uint32_t idesc,
+                                            uint32_t bar_a) {
+    asm volatile("{\n.reg .pred e, pt, pf;\n"
+                 "elect.sync _|e, 0xffffffff;\n"
+                 "setp.eq.u32 pt, %2, 0;\n"
+                 "setp.ne.u32 pf, %2, 0;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %4, %8, %1, {%2, %2, %2, %2}, pf;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %5, %9, %1, {%2, %2, %2, %2}, pt;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %6, %10, %1, {%2, %2, %2, %2}, pt;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %7, %11, %1, {%2, %2, %2, %2}, pt;\n"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%3];\n}\n"
+                 ::"r"(d_tmem), "r"(idesc), "r"(0u), "r"(bar_a),
+                   "l"(a[0]), "l"(a[1]), "l"(a[2]), "l"(a[3]), "l"(b[0]), "l"(b[1]), "l"(b[2]), "l"(b[3]) : "memory");
+}
 // O (+)= P V: eight K16 steps with A from TMEM (128 lanes x 8 columns of packed fp16 pairs per step) and B[smem desc];
 // the first step accumulates only if `acc0`.  Then commit to bar_a.
 __device__ __forceinline__ void tc_group_ts(uint32_t d_tmem, uint32_t a_tmem, const uint64_t (&b)[8], uint32_t idesc, uint32_t acc0,
@@ -302,13 +319,15 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) {
 }
 // Instruction descriptor: fp32 accumulate, fp16 A and B, A K-major, N = 128, M = 128; bit 16 = B is MN-major.
 constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-constexpr uint32_t IDESC_PV = IDESC_S | (1u << 16);
+// ... and for P V, N = the head's width.
+template <int HD> constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 
 // SPLIT (see PrefillArgs): a CTA walks one of n_split slices of its tile's KV blocks and leaves the unscaled output.
-template <bool SPLIT>
+template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const TcArgs p) {
+    constexpr int NSL = HD / 64;                          // slabs of a tile
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t sbase = (raw + 1023u) & ~1023u;
@@ -375,25 +394,25 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (lane == 0) {
             bool ok = true;
             int k_issued[NKS] = {}, v_issued[NVS] = {};
-            mbar_expect_tx(bar(Q_FULL), 2 * 128 * p.G * p.TQ);       // two slabs of G*TQ rows of 128 bytes
+            mbar_expect_tx(bar(Q_FULL), NSL * 128 * p.G * p.TQ);     // slabs of G*TQ rows of 128 bytes
             tma_load_3d(sbase + OFF_Q, &tmQ, 0, kvh * p.G, t0, bar(Q_FULL));
-            tma_load_3d(sbase + OFF_Q + SLAB, &tmQ, 64, kvh * p.G, t0, bar(Q_FULL));
+            if (NSL == 2) tma_load_3d(sbase + OFF_Q + SLAB, &tmQ, 64, kvh * p.G, t0, bar(Q_FULL));
             auto load_k = [&](int j) {
                 const int s = j % NKS;
                 if (j >= NKS) ok = mbar_wait(bar(S_FULL + s), ((j / NKS) - 1) & 1, s_abort);     // S_(j-NKS) done: stage free
                 if (!ok) return;
-                mbar_expect_tx(bar(K_FULL + s), TILE);
+                mbar_expect_tx(bar(K_FULL + s), NSL * SLAB);
                 tma_load_3d(sbase + OFF_K + s * TILE, &tmK, 0, kv0 + j * BN, kvh, bar(K_FULL + s));
-                tma_load_3d(sbase + OFF_K + s * TILE + SLAB, &tmK, 64, kv0 + j * BN, kvh, bar(K_FULL + s));
+                if (NSL == 2) tma_load_3d(sbase + OFF_K + s * TILE + SLAB, &tmK, 64, kv0 + j * BN, kvh, bar(K_FULL + s));
                 ++k_issued[s];
             };
             auto load_v = [&](int j) {
                 const int s = j % NVS;
                 if (j >= NVS) ok = mbar_wait(bar(PV_DONE + s), ((j / NVS) - 1) & 1, s_abort);    // P V of block j-2 done: stage free
                 if (!ok) return;
-                mbar_expect_tx(bar(V_FULL + s), TILE);
+                mbar_expect_tx(bar(V_FULL + s), NSL * SLAB);
                 tma_load_3d(sbase + OFF_V + s * TILE, &tmV, 0, kv0 + j * BN, kvh, bar(V_FULL + s));
-                tma_load_3d(sbase + OFF_V + s * TILE + SLAB, &tmV, 64, kv0 + j * BN, kvh, bar(V_FULL + s));
+                if (NSL == 2) tma_load_3d(sbase + OFF_V + s * TILE + SLAB, &tmV, 64, kv0 + j * BN, kvh, bar(V_FULL + s));
                 ++v_issued[s];
             };
             // consumption order of the MMA warp: K_0..K_2, then V_j, K_(j+3)
@@ -417,21 +436,24 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         mbar_wait_warp(bar(Q_FULL), 0, s_abort);
         // Descriptors are built once: per k-step for Q, per ring stage and k-step for K and V (the offsets are added to the
         // 14-bit address field, in 16-byte units; it cannot carry out of the field).
-        uint64_t dQ[8], dK0[8], dV0[8];
+        constexpr int KS = HD / 16;                          // k-steps of Q K^T
+        uint64_t dQ[KS], dK0[KS], dV0[8];
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
             const uint32_t off = (uint32_t)((kk >> 2) * SLAB + (kk & 3) * 32);
-            dQ[kk] = desc_kmajor(sbase + OFF_Q + off);
-            dK0[kk] = desc_kmajor(sbase + OFF_K + off);
+            if (kk < KS) {
+                dQ[kk] = desc_kmajor(sbase + OFF_Q + off);
+                dK0[kk] = desc_kmajor(sbase + OFF_K + off);
+            }
             dV0[kk] = desc_mnmajor(sbase + OFF_V + kk * 2048);       // V: 16 rows of 128 B per k-step
         }
         // S_j = Q K_j^T into score buffer s = j % NSB, K from ring stage s.  The commit publishes the scores and frees the
         // K stage.
         auto issue_s = [&](int j, int s) {
             if (lane == 0) TRACE(0, 0, j);
-            uint64_t dKs[8];
+            uint64_t dKs[KS];
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk) dKs[kk] = dK0[kk] + (uint64_t)((s * TILE) >> 4);
+            for (int kk = 0; kk < KS; ++kk) dKs[kk] = dK0[kk] + (uint64_t)((s * TILE) >> 4);
             tc_group_ss(TM_S + s * BN, dQ, dKs, IDESC_S, bar(S_FULL + s));
         };
         tc_fence_after();
@@ -461,7 +483,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) dVs[kk] = dV0[kk] + (uint64_t)((sv * TILE) >> 4);
             // commit: accumulator complete up to block j; V stage sv free
-            tc_group_ts(TM_O, TM_S + b * BN, dVs, IDESC_PV, j > 0 ? 1u : 0u, bar(PV_DONE + sv));
+            tc_group_ts(TM_O, TM_S + b * BN, dVs, IDESC_PV<HD>, j > 0 ? 1u : 0u, bar(PV_DONE + sv));
             if (lane == 0) TRACE(0, 3, j);
             // what the next block's P V needs, looked at before the S group below is issued
             const int bn = (b + 1 == NSB) ? 0 : b + 1;
@@ -557,7 +579,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 const float alpha = need ? fast_exp2(m_prev - m_new) : 1.f;
                 float o[32];
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < HD / 32; ++c) {
                     tmem_ld32(to + 32 * c, o);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] *= alpha;
@@ -623,27 +645,28 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const int ptok = SPLIT ? split * (gridDim.x * p.TQ) + tglob : tglob;      // row of the output, or of the slices' outputs
             if (SPLIT && team == 0 && valid)
                 p.part_ml[(size_t)ptok * p.n_head + kvh * p.G + hg] = make_float2(M, w_me * l + w_ot * other.y);
-            // this thread writes columns [64 team, 64 team + 64) of its row
-            float* dst = p.out + ((size_t)ptok * p.n_head + kvh * p.G + hg) * HD + 64 * team;
+            // this thread writes half of its row's columns, the second team the second half
+            float* dst = p.out + ((size_t)ptok * p.n_head + kvh * p.G + hg) * HD + HD / 2 * team;
 #pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < NSL; ++c) {
                 float a[32];
-                tmem_ld32(to + 64 * team + 32 * c, a);
+                tmem_ld32(to + HD / 2 * team + 32 * c, a);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) a[i] *= inv;
                 if (!SPLIT && p.out_tma == 2) {
-                    // fp16: two slabs of 64 columns, one per team, the same way
-                    uint8_t* rowp = smem + OFF_K + team * (BM * 128) + row * 128;
+                    // fp16: slabs of 64 columns, the same way; one per team, or half of the one
+                    uint8_t* rowp = smem + OFF_K + (NSL == 2 ? team : 0) * (BM * 128) + row * 128;
+                    const int c16 = NSL == 2 ? 4 * c : 4 * team;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<uint4*>(rowp + (((4 * c + i) ^ (row & 7)) << 4)) =
+                        *reinterpret_cast<uint4*>(rowp + (((c16 + i) ^ (row & 7)) << 4)) =
                             make_uint4(pack_half2(a[8 * i], a[8 * i + 1]), pack_half2(a[8 * i + 2], a[8 * i + 3]),
                                        pack_half2(a[8 * i + 4], a[8 * i + 5]), pack_half2(a[8 * i + 6], a[8 * i + 7]));
                 } else if (p.out_tma) {
                     // Straight from here a warp's store would touch 32 rows, 512 bytes apart, with 16 bytes each.  The
                     // tile goes through shared memory instead (the K ring is idle now): four slabs of 32 columns, a row's
                     // 128 bytes of a slab swizzled like a tensor-map tile, and leaves as four bulk tensor stores.
-                    uint8_t* rowp = smem + OFF_K + (2 * team + c) * (BM * 128) + row * 128;
+                    uint8_t* rowp = smem + OFF_K + (NSL * team + c) * (BM * 128) + row * 128;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         *reinterpret_cast<float4*>(rowp + ((i ^ (row & 7)) << 4)) = make_float4(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]);
@@ -652,7 +675,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     for (int i = 0; i < 8; ++i)
                         *reinterpret_cast<float4*>(dst + 32 * c + 4 * i) = make_float4(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]);
                 }
-                if (!SPLIT && valid && p.out_mmq) {
+                if (HD == 128 && !SPLIT && valid && p.out_mmq) {
                     // The 32 values are one quantisation group of the 128-value block of (head, token): what
                     // quantize_mmq_q8_1_k (src/kernels.cu:160-205) computes with a shuffle over eight lanes is a
                     // reduction over this thread's registers here.
@@ -686,10 +709,10 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 // rows past the batch (a ragged last tile) lie outside the tensor map and are not written
                 if (!SPLIT && p.out_tma == 2) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) tma_store_3d(&tmO, 64 * c, kvh * p.G, t0, sbase + OFF_K + c * (BM * 128));
+                    for (int c = 0; c < NSL; ++c) tma_store_3d(&tmO, 64 * c, kvh * p.G, t0, sbase + OFF_K + c * (BM * 128));
                 } else {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tma_store_3d(&tmO, 32 * c, kvh * p.G, (SPLIT ? split * (int)(gridDim.x * p.TQ) : 0) + t0, sbase + OFF_K + c * (BM * 128));
+                    for (int c = 0; c < HD / 32; ++c) tma_store_3d(&tmO, 32 * c, kvh * p.G, (SPLIT ? split * (int)(gridDim.x * p.TQ) : 0) + t0, sbase + OFF_K + c * (BM * 128));
                 }
                 asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
                 asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");  // shared memory stays valid until it has been read
@@ -705,16 +728,48 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (tid == 0 && *s_abort && p.status) atomicExch(p.status, 1);
 }
 
+// Joins the slices of a split call: a row's HD/4 threads take 4 dims each.  Bound by reading the slices, from L2: 64 tokens of 32
+// heads in eight slices are 8 MB.
+template <int HD>
+__global__ void __launch_bounds__(256) prefill_merge_kernel(const PrefillArgs p, int tokens) {
+    pdl_trigger();
+    pdl_wait();
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long row = at / (HD / 4);                     // (token, head)
+    const int c4 = (int)(at % (HD / 4));
+    if (row >= (long long)p.batch * p.n_head) return;
+    const size_t step = (size_t)tokens * p.n_head;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row;
+    const float4* o = reinterpret_cast<const float4*>(p.part_o) + row * (HD / 4) + c4;
+    float M = -CUDART_INF_F;
+#pragma unroll 4
+    for (int s = 0; s < p.n_split; ++s) M = fmaxf(M, ml[s * step].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < p.n_split; ++s) {
+        const float2 x = ml[s * step];
+        const float4 v = o[s * step * (HD / 4)];
+        const float w = x.x == -CUDART_INF_F ? 0.f : fast_exp2(x.x - M);       // a slice that the mask hides from this row
+        L += w * x.y;
+        acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+    }
+    const float inv = 1.f / L;
+    acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+    if (p.out16) reinterpret_cast<uint2*>(p.out16)[at] = make_uint2(pack_half2(acc.x, acc.y), pack_half2(acc.z, acc.w));
+    else         reinterpret_cast<float4*>(p.out)[at] = acc;
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn g_encode = nullptr;
 
-// fp16 tensor [d2][d1][128] with the given strides (bytes); box = 64 x b1 x b2, 128-byte swizzle, zero fill.
-// fp32 tensor [d2][d1][128] (the output): box = 32 x b1 x b2 (one 128-byte swizzle span of columns), for stores.
-bool make_out_map(CUtensorMap* m, const void* base, uint64_t d1, uint64_t d2, uint64_t stride1, uint64_t stride2, uint32_t b1,
+// fp16 tensor [d2][d1][hd] with the given strides (bytes); box = 64 x b1 x b2, 128-byte swizzle, zero fill.
+// fp32 tensor [d2][d1][hd] (the output): box = 32 x b1 x b2 (one 128-byte swizzle span of columns), for stores.
+bool make_out_map(CUtensorMap* m, const void* base, int hd, uint64_t d1, uint64_t d2, uint64_t stride1, uint64_t stride2, uint32_t b1,
                   uint32_t b2) {
-    cuuint64_t dims[3] = {(cuuint64_t)HD, d1, d2};
+    cuuint64_t dims[3] = {(cuuint64_t)hd, d1, d2};
     cuuint64_t strides[2] = {stride1, stride2};
     cuuint32_t box[3] = {32, b1, b2};
     cuuint32_t estr[3] = {1, 1, 1};
@@ -723,15 +778,40 @@ bool make_out_map(CUtensorMap* m, const void* base, uint64_t d1, uint64_t d2, ui
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool make_map(CUtensorMap* m, const void* base, uint64_t d1, uint64_t d2, uint64_t stride1, uint64_t stride2, uint32_t b1,
+bool make_map(CUtensorMap* m, const void* base, int hd, uint64_t d1, uint64_t d2, uint64_t stride1, uint64_t stride2, uint32_t b1,
               uint32_t b2) {
-    cuuint64_t dims[3] = {(cuuint64_t)HD, d1, d2};
+    cuuint64_t dims[3] = {(cuuint64_t)hd, d1, d2};
     cuuint64_t strides[2] = {stride1, stride2};
     cuuint32_t box[3] = {64, b1, b2};
     cuuint32_t estr[3] = {1, 1, 1};
     return g_encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD, bool SPLIT>
+cudaError_t set_attributes() {
+    // the register budgets are shares of what the kernel is compiled with
+    cudaFuncAttributes fa;
+    cudaError_t e = cudaFuncGetAttributes(&fa, prefill_tc_kernel<HD, SPLIT>);
+    if (e != cudaSuccess) return e;
+    if (fa.numRegs * kThreads < kRegsService * 128 + kRegsSoftmax * (kThreads - 128)) return cudaErrorInvalidConfiguration;
+    return cudaFuncSetAttribute(prefill_tc_kernel<HD, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+}
+// a.n_split > 1, `tokens`: see PrefillArgs
+cudaError_t launch_merge(const PrefillArgs& a, int tokens, cudaStream_t stream, unsigned long long* launches) {
+    const long long threads = (long long)a.batch * a.n_head * (a.head_dim / 4);
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    const cudaError_t e = a.head_dim == 128 ? launch_dependent(prefill_merge_kernel<128>, grid, 256, 0, stream, 1, a, tokens)
+                                            : launch_dependent(prefill_merge_kernel<64>, grid, 256, 0, stream, 1, a, tokens);
+    if (launches) *launches += 1;
+    return e;
+}
+template <int HD>
+cudaError_t launch_kernel(dim3 grid, bool split, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                          const CUtensorMap& o, const TcArgs& t) {
+    return split ? launch_dependent(prefill_tc_kernel<HD, true>, grid, kThreads, SMEM_BYTES, stream, 1, q, k, v, o, t)
+                 : launch_dependent(prefill_tc_kernel<HD, false>, grid, kThreads, SMEM_BYTES, stream, 1, q, k, v, o, t);
 }
 
 } // namespace
@@ -751,13 +831,15 @@ cudaError_t prefill_tc_set_attributes() {
         if (qres != cudaDriverEntryPointSuccess || !fn) return cudaErrorNotSupported;
         g_encode = reinterpret_cast<EncodeTiledFn>(fn);
     }
-    const cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(prefill_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    cudaError_t e;
+    if ((e = set_attributes<128, false>()) != cudaSuccess || (e = set_attributes<128, true>()) != cudaSuccess) return e;
+    if ((e = set_attributes<64, false>()) != cudaSuccess) return e;
+    return set_attributes<64, true>();
 }
 
 // A CTA takes about 0.9 us a block; writing the slices' outputs and joining them 5 to 6 together, so eight blocks have to be saved.  64
-// tokens of 32/8 heads behind 8192 rows (16 tiles, 9 slices) 29 us against 67, prologue included, 256 tokens (64 tiles, 2
-// slices) 52 against 73; nine blocks in two slices 22 against 19.
+// tokens of 32/8 heads behind 8192 rows (16 tiles, 9 slices) 29 us against 67, prologue included, 128 tokens (32 tiles, 4
+// slices) 37 against 69; nine blocks in two slices 22 against 19.
 int prefill_tc_splits(int n_head, int n_kv, int n_past, int batch, int sm_count) {
     const int TQ = 128 / (n_head / n_kv);
     const long long ctas = (long long)n_kv * ((batch + TQ - 1) / TQ);
@@ -769,23 +851,24 @@ int prefill_tc_splits(int n_head, int n_kv, int n_past, int batch, int sm_count)
 cudaError_t launch_prefill_tc(const PrefillArgs& a, int sm_count, cudaStream_t stream, unsigned long long* launches) {
     (void)sm_count;
     const int G = a.n_head / a.n_kv;
-    if (a.head_dim != HD || G > 128 || !g_encode) return cudaErrorNotSupported;
+    const int HD = a.head_dim;
+    if ((HD != 128 && !(HD == 64 && a.tc_hd64)) || G > 128 || !g_encode) return cudaErrorNotSupported;
     const int TQ = 128 / G;
     const uint64_t rows = (uint64_t)a.n_past + a.batch;          // rows past the chunk are never read (zero fill)
     CUtensorMap tmQ, tmK, tmV;
     const uint64_t rowb = HD * sizeof(__half);
-    if (!make_map(&tmQ, a.q16, a.n_head, a.batch, rowb, rowb * a.n_head, G, TQ)) return cudaErrorInvalidValue;
-    if (!make_map(&tmK, a.kc, rows, a.n_kv, rowb, rowb * a.n_ctx, BN, 1)) return cudaErrorInvalidValue;
-    if (!make_map(&tmV, a.vc, rows, a.n_kv, rowb, rowb * a.n_ctx, BN, 1)) return cudaErrorInvalidValue;
+    if (!make_map(&tmQ, a.q16, HD, a.n_head, a.batch, rowb, rowb * a.n_head, G, TQ)) return cudaErrorInvalidValue;
+    if (!make_map(&tmK, a.kc, HD, rows, a.n_kv, rowb, rowb * a.n_ctx, BN, 1)) return cudaErrorInvalidValue;
+    if (!make_map(&tmV, a.vc, HD, rows, a.n_kv, rowb, rowb * a.n_ctx, BN, 1)) return cudaErrorInvalidValue;
     // the fp32 output as a tensor map for bulk stores (16-byte aligned base; else the kernel stores directly)
     CUtensorMap tmO = tmQ;
     const uint64_t orow = HD * sizeof(float);
-    const bool out_tma = a.out && !((uintptr_t)a.out & 15) && make_out_map(&tmO, a.out, a.n_head, a.batch, orow, orow * a.n_head, G, TQ);
+    const bool out_tma = a.out && !((uintptr_t)a.out & 15) && make_out_map(&tmO, a.out, HD, a.n_head, a.batch, orow, orow * a.n_head, G, TQ);
     // ... or the fp16 one, which has no other way out (the C entry checked its alignment)
     const int tiles = (a.batch + TQ - 1) / TQ;
     if (a.n_split > 1) {
-        if (!make_out_map(&tmO, a.part_o, a.n_head, (uint64_t)a.n_split * tiles * TQ, orow, orow * a.n_head, G, TQ)) return cudaErrorInvalidValue;
-    } else if (a.out16 && !make_map(&tmO, a.out16, a.n_head, a.batch, rowb, rowb * a.n_head, G, TQ)) return cudaErrorInvalidValue;
+        if (!make_out_map(&tmO, a.part_o, HD, a.n_head, (uint64_t)a.n_split * tiles * TQ, orow, orow * a.n_head, G, TQ)) return cudaErrorInvalidValue;
+    } else if (a.out16 && !make_map(&tmO, a.out16, HD, a.n_head, a.batch, rowb, rowb * a.n_head, G, TQ)) return cudaErrorInvalidValue;
     TcArgs t;
     t.out_tma = a.n_split > 1 ? 1 : (a.out16 ? 2 : (out_tma ? 1 : 0));
     t.part_ml = reinterpret_cast<float2*>(a.part_ml);
@@ -797,10 +880,10 @@ cudaError_t launch_prefill_tc(const PrefillArgs& a, int sm_count, cudaStream_t s
     t.status = a.status;
     t.n_head = a.n_head; t.n_kv = a.n_kv; t.n_past = a.n_past; t.batch = a.batch; t.G = G; t.TQ = TQ;
     const dim3 grid(tiles, a.n_kv, a.n_split);
-    const cudaError_t e = a.n_split > 1 ? launch_dependent(prefill_tc_kernel<true>, grid, kThreads, SMEM_BYTES, stream, 1, tmQ, tmK, tmV, tmO, t)
-                                        : launch_dependent(prefill_tc_kernel<false>, grid, kThreads, SMEM_BYTES, stream, 1, tmQ, tmK, tmV, tmO, t);
+    const cudaError_t e = HD == 128 ? launch_kernel<128>(grid, a.n_split > 1, stream, tmQ, tmK, tmV, tmO, t)
+                                    : launch_kernel<64>(grid, a.n_split > 1, stream, tmQ, tmK, tmV, tmO, t);
     if (launches) *launches += 1;
-    return e != cudaSuccess || a.n_split == 1 ? e : launch_prefill_merge(a, tiles * TQ, stream, launches);
+    return e != cudaSuccess || a.n_split == 1 ? e : launch_merge(a, tiles * TQ, stream, launches);
 }
 
 } // namespace oattn
