@@ -343,14 +343,15 @@ int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void
                     int head_dim, int n_ctx, const int* d_pos, float scale, int fuse, const oattn_rope_params* rope,
                     const oattn_ext* ext, void* workspace, size_t workspace_bytes, void* stream);
 
-/* oattn_prefill_ex on the 4-bit cache (ext may be NULL): the chunk's rows are quantised into the cache, and every query sees the
- * rows as the cache holds them, its own chunk's among them.  The output is fp32 (`out`) or fp16 (`out_f16`, [batch][n_head]
- * [head_dim]): pass one of them; with ext->out_mmq both may be NULL.  A short chunk (up to 1024 (token, head) pairs for
- * head_dim 128, 2048 for 64; fewer behind more than 900 rows, 300 to 500 behind 8192) is attended from the 4-bit rows themselves,
- * with the accuracy of oattn_decode_q4, in two launches; a longer one, or one with ext->out_mmq, on fp16 copies of the rows,
- * which the first of two or three launches makes in the workspace.  The workspace is sized for `max_rows` = the largest n_past + batch and
- * serves all layers; it need not be cleared, and calls that may run at the same time need one each.  oattn_prefill_status reads
- * its status word (same n_head, head_dim, batch). */
+/* oattn_prefill_ex on the 4-bit cache (ext may be NULL): the chunk's rows are quantised into the cache, and every query sees
+ * the rows as the cache holds them, its own chunk's among them.  The output is fp32 (`out`) or fp16 (`out_f16`,
+ * [batch][n_head][head_dim]): pass one of them; with ext->out_mmq both may be NULL.  A short chunk (up to 1024 (token, head)
+ * pairs for head_dim 128, 2048 for 64; fewer behind more than 900 rows, 300 to 500 behind 8192) is attended from the 4-bit
+ * rows themselves, with the accuracy of oattn_decode_q4, in two launches; a longer one, or one with ext->out_mmq, on fp16
+ * copies of the rows, which the first of two or three launches makes in the workspace.  A NaN in a row or a query shows in
+ * the outputs that see it (on the second way in those of earlier tokens of the chunk, too, as in oattn_prefill_ex).  The
+ * workspace is sized for `max_rows` = the largest n_past + batch and serves all layers; it need not be cleared, and calls
+ * that may run at the same time need one each.  oattn_prefill_status reads its status word (same n_head, head_dim, batch). */
 size_t oattn_prefill_q4_workspace_bytes(int n_head, int n_kv, int head_dim, int max_batch, int max_rows);
 int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, void* cache, float* out, uint16_t* out_f16, int n_head,
                      int n_kv, int head_dim, int n_ctx, int n_past, int batch, float scale, int fuse,

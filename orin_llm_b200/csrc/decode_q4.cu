@@ -455,6 +455,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         uint32_t vs[NT][2][NG];
 #pragma unroll
         for (int j = 0; j < NT; ++j) load_scales<NG>(blk + (j >> 1) * F::BLOCK + F::VS_OFF + (8 * (j & 1) + 2 * t) * F::SROWB, vs[j]);
+        if (CHUNK && nrow_all < 16 * NB) {                   // a later token's row may hold anything: 0 * NaN would show
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    if (8 * j + 2 * t >= nrow) vs[j][0][g] = 0u;
+                    if (8 * j + 2 * t + 1 >= nrow) vs[j][1][g] = 0u;
+                }
+        }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             uint32_t a[NB][4];

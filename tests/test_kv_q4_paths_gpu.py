@@ -149,6 +149,25 @@ def test_short_chunk_behind_a_long_context(ops, n_head, n_kv, hd, past, batch, h
     assert ops.prefill_status(n_head, n_kv, hd, batch, ops.prefill_q4_workspace(n_head, n_kv, hd, batch, n_ctx)) == 0
 
 
+@pytest.mark.parametrize("n_head,n_kv,hd,past", [(4, 4, 128, 700), (12, 2, 128, 45), (6, 3, 64, 640), (8, 8, 64, 0)])
+def test_short_chunk_hides_a_later_tokens_nan(ops, n_head, n_kv, hd, past):
+    """The last token's key and value are not finite: the tokens before it give the bits they give without it."""
+    rng = np.random.default_rng(206)
+    batch = 7
+    n_ctx = past + batch
+    cache = filled(rng, n_kv, hd, n_ctx, past)
+    q, k, v = rng.standard_normal((batch, n_head, hd)).astype(np.float32), rows(rng, batch, n_kv, hd), rows(rng, batch, n_kv, hd)
+    outs = []
+    for bad in (False, True):
+        if bad:
+            k[-1, :, 5] = v[-1, :, 9] = np.nan
+        out = torch.empty(batch, n_head, hd, device="cuda")
+        ops.attn_prefill_q4(dev(q), dev(k), dev(v), dev(cache), out, n_head, n_kv, hd, n_ctx, past, batch, 0.1, ops.FUSE_KV_APPEND)
+        outs.append(out.cpu().numpy())
+    assert np.isfinite(outs[0]).all() and np.array_equal(outs[0][:-1], outs[1][:-1])
+    assert np.isnan(outs[1][-1]).all()
+
+
 def test_short_chunk_over_many_slices_and_in_a_graph(ops):
     """20000 rows, so that a chunk's slices merge in two levels; the same bits from a graph, and from both kernels to their bounds."""
     n_head, n_kv, hd, past, batch = 8, 2, 128, 20000, 6
