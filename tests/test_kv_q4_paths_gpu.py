@@ -397,10 +397,10 @@ def test_two_streams_with_workspaces_of_their_own(ops):
         ops.set_stream(None)
 
 
-@pytest.mark.parametrize("batch", [40, 160])
-def test_prefill_captured(ops, batch):
+@pytest.mark.parametrize("hd,past,batch", [(128, 50, 40), (128, 50, 160), (128, 1500, 160), (64, 1600, 270)])
+def test_prefill_captured(ops, hd, past, batch):
     rng = np.random.default_rng(223)
-    n_head, n_kv, hd, past = 8, 2, 128, 50
+    n_head, n_kv = 8, 2
     n_ctx = past + batch
     base = dev(filled(rng, n_kv, hd, n_ctx, past))
     q, k, v = (dev(rng.standard_normal((batch, h, hd)).astype(np.float32)) for h in (n_head, n_kv, n_kv))
