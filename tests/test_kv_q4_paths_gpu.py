@@ -168,6 +168,32 @@ def test_short_chunk_hides_a_later_tokens_nan(ops, n_head, n_kv, hd, past):
     assert np.isnan(outs[1][-1]).all()
 
 
+@pytest.mark.parametrize("amp_q,amp_k,amp_v", [(1e-4, 300.0, 1e-3), (300.0, 1e-3, 20000.0), (1.0, 1.0, 50.0), (1e-20, 1.0, 1e-5)])
+@pytest.mark.parametrize("hd,past,batch", [(128, 327, 6), (64, 327, 6), (128, 1700, 300), (64, 1700, 600)])
+def test_chunk_at_any_scale(ops, hd, past, batch, amp_q, amp_k, amp_v):
+    """The values of the decode test of this name, for a chunk that takes the 4-bit rows and one whose fp16 copies are read in slices."""
+    short = batch < 100
+    rng = np.random.default_rng(207)
+    n_head, n_kv = 4, 1
+    n_ctx = past + batch
+    cache = np.zeros((n_kv, (n_ctx + 15) // 16, 18 * hd), np.uint8)
+    k, v = amp_k * rows(rng, n_ctx, n_kv, hd), amp_v * rng.standard_normal((n_ctx, n_kv, hd))
+    v[: n_ctx // 2] *= 0.01
+    v = np.clip(v, -60000, 60000)
+    ref.write_rows(cache, hd, range(n_ctx), k.astype(np.float32), v.astype(np.float32))
+    q = (amp_q * rng.standard_normal((batch, n_head, hd))).astype(np.float32)
+    scale = 0.3 / (amp_q * amp_k * hd)
+    out = torch.empty(batch, n_head, hd, device="cuda")
+    ops.attn_prefill_q4(dev(q), None, None, dev(cache), out, n_head, n_kv, hd, n_ctx, past, batch, scale, ops.FUSE_NONE)
+    K, V = ref.read_rows(cache, hd, n_ctx)
+    want, most = ref.attend(q, K, V, past, np.float32(scale))
+    err = np.abs(out.cpu().numpy() - want).max()
+    # the scaled queries of the second way are fp16 and may be subnormal there: off by up to 2^-25 each, in a power of two
+    small = 2 * math.log(2) * 2.0 ** -25 * np.abs(K).sum(-1).max() * np.abs(V).max()
+    bound = decode_bound(most, scale, V) if short else prefill_bound(most, scale, V, False) + small
+    assert err <= bound, (err, bound)
+
+
 def test_short_chunk_over_many_slices_and_in_a_graph(ops):
     """20000 rows, so that a chunk's slices merge in two levels; the same bits from a graph, and from both kernels to their bounds."""
     n_head, n_kv, hd, past, batch = 8, 2, 128, 20000, 6
