@@ -423,11 +423,15 @@ __global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kerne
     load_rows(warp);
     // cos and sin in double: a key's code is a decision at a border, so the rotated key is rounded to fp32 once
     __shared__ double s_cos[HD / 2], s_sin[HD / 2];
+    __shared__ float2 s_cs[HD / 2];                       // rounded, for the queries
     if (rope_q || rope_k) {
         for (int i = tid; i < a.rope.n_rot / 2; i += kPrologueThreads) {
             float f = p.freq[i];
             if (a.rope.freq_factors) f = __fdiv_rn(f, a.rope.freq_factors[i]);
-            sincos((double)__fmul_rn((float)pos, f), &s_sin[i], &s_cos[i]);
+            double sn, cs;
+            sincos((double)__fmul_rn((float)pos, f), &sn, &cs);
+            s_sin[i] = sn; s_cos[i] = cs;
+            s_cs[i] = make_float2((float)cs, (float)sn);
         }
     }
     __syncthreads();
@@ -465,7 +469,25 @@ __global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kerne
 #pragma unroll
                 for (int e = 0; e < F::EPL; ++e) x[e] = x[e] * rn * nw[F::EPL * lane + e];
             }
-            if (r.kind == 0 ? rope_q : (r.kind == 1 && rope_k)) {
+            if (r.kind == 0 && rope_q && a.rope.n_rot == HD) {
+                // a pair's two elements are in this lane or 16 lanes away
+                if (a.rope.rope_type != 1) {
+#pragma unroll
+                    for (int e = 0; e < F::EPL; e += 2) {
+                        const float2 cs = s_cs[(F::EPL * lane + e) / 2];
+                        const float v0 = x[e], v1 = x[e + 1];
+                        x[e] = v0 * cs.x - v1 * cs.y;
+                        x[e + 1] = v0 * cs.y + v1 * cs.x;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < F::EPL; ++e) {
+                        const float2 cs = s_cs[F::EPL * (lane & 15) + e];
+                        const float y = __shfl_xor_sync(0xffffffffu, x[e], 16);
+                        x[e] = fmaf(lane < 16 ? -y : y, cs.y, x[e] * cs.x);
+                    }
+                }
+            } else if (r.kind == 0 ? rope_q : (r.kind == 1 && rope_k)) {
                 // the row passes through shared memory: a pair's two elements may lie in any two lanes
 #pragma unroll
                 for (int e = 0; e < F::EPL; ++e) row[F::EPL * lane + e] = x[e];
@@ -474,7 +496,7 @@ __global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kerne
                     int i0, i1;
                     rope_pair_index(a.rope.rope_type, pp, a.rope.n_rot, i0, i1);
                     if (r.kind == 0) {
-                        const float v0 = row[i0], v1 = row[i1], c = (float)s_cos[pp], s = (float)s_sin[pp];
+                        const float v0 = row[i0], v1 = row[i1], c = s_cs[pp].x, s = s_cs[pp].y;
                         row[i0] = v0 * c - v1 * s;
                         row[i1] = v0 * s + v1 * c;
                     } else {
