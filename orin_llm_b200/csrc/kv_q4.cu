@@ -441,10 +441,7 @@ __global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kerne
         for (int i = tid; i < p.n_tickets; i += kPrologueThreads) p.tickets[i] = 0;
     }
     for (int j0 = warp; j0 < jobs; j0 += W * RB) {
-        if (j0 != warp) {
-            __syncwarp();                                 // every lane has read the rows that the next ones replace
-            load_rows(j0);
-        }
+        if (j0 != warp) load_rows(j0);
         cp_async_wait<0>();
         __syncwarp();
 #pragma unroll 1
