@@ -245,6 +245,7 @@ def test_decode_shows_a_nan_and_an_empty_cache_gives_zero(ops):
                                                        (32, 8, 64, 0, 3), (16, 1, 128, 5, 16), (5, 5, 64, 28, 8), (8, 8, 128, 60, 41),
                                                        # more (token, head) pairs than are taken from the 4-bit rows: the fp16 copies
                                                        (12, 2, 128, 20, 190), (8, 8, 128, 131, 140), (9, 3, 128, 130, 131), (4, 1, 64, 35, 530),
+                                                       (32, 8, 64, 0, 70), (16, 16, 64, 0, 200), (12, 12, 128, 0, 100),
                                                        # ... cut into slices of at least 512 rows: 3, 5, 4, 5; 3, 3, 4
                                                        (8, 2, 128, 1500, 140), (5, 1, 128, 2500, 210), (9, 3, 128, 2000, 160), (32, 2, 128, 2560, 70),
                                                        (8, 8, 64, 1600, 260), (16, 1, 64, 1500, 129), (12, 4, 64, 2047, 190)])
