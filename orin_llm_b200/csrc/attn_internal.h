@@ -148,12 +148,16 @@ struct PrefillArgs {
     bool tc_hd64 = false;         // heads of 64 on the tcgen05 kernel, too
     float* part_o = nullptr;
     float* part_ml = nullptr;
+    float* acc = nullptr;         // workspace for sums that leave TMEM on the way; nullptr (heads of 128 without slices): none do
 };
 constexpr int kMaxPrefillSplits = 16, kSplitCtas = 148;
 constexpr int kSplitMinBlocks = 4;            // 128-row blocks that a slice has at least
 // Slices for a call: as many as fill the SMs, fewer for a short context, 1 or less: not worth it.  Together they have at most
 // kSplitCtas * 128 rows.
 int prefill_tc_splits(int n_head, int n_kv, int n_past, int batch, int sm_count);
+// The P V sum of a tile leaves TMEM in front of every block whose number divides by kPrefillAccBlocks, unless fewer than kPrefillAccRest
+// blocks are left (see acc_leaves in prefill_tc.cu).
+constexpr int kPrefillAccBlocks = 48, kPrefillAccRest = 16;
 
 // Prologue shared by both prefill kernels: RoPE(q) -> q16, RoPE(k_new) + fp16 append of k_new, v_new.
 cudaError_t launch_prefill_prologue(const PrefillArgs& a, cudaStream_t stream, unsigned long long* launches);

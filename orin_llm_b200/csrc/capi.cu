@@ -620,15 +620,24 @@ static int chunk_blocks(int n_head, int n_kv, int head_dim, int n_past, int batc
 constexpr size_t kChunkScratch = 4u << 20;      // partial results of a chunk's slices: at most 2 * 160 slices of 8 rows, and their groups
 
 constexpr size_t kSplitRows = (size_t)kSplitCtas * 128;       // a long chunk's (token, head) rows over all slices
+// Bytes of the sums that leave TMEM, for tiles of 128 rows; 0 where `blocks` 128-row blocks at most are walked in one go.
+static size_t prefill_acc_bytes(size_t tiles, int head_dim, long long blocks) {
+    return blocks < kPrefillAccBlocks + kPrefillAccRest ? 0 : tiles * 128 * head_dim * sizeof(float);
+}
 
-// [fp16 queries][status word, 256 bytes][fp16 K rows][fp16 V rows][slices' outputs][(maximum, sum)]: the first two as in oattn_prefill.  A short chunk has its fp32
-// queries and partial results behind the status word instead of the rows.
+// [fp16 queries][status word, 256 bytes][fp16 K rows][fp16 V rows], then either [slices' outputs][(maximum, sum)][their sums that leave
+// TMEM] or those of the whole tiles alone: the first two as in oattn_prefill.  A short chunk has its fp32 queries and partial results
+// behind the status word instead of the rows.
 size_t oattn_prefill_q4_workspace_bytes(int n_head, int n_kv, int head_dim, int max_batch, int max_rows) {
     const size_t head = oattn_prefill_workspace_bytes(n_head, n_kv, head_dim, max_batch);
     if (!head || max_rows < max_batch) return 0;
     const size_t copies = 2 * align256((size_t)n_kv * max_rows * head_dim * sizeof(__half));
     const size_t chunk = align256((size_t)max_batch * n_head * head_dim * sizeof(float)) + kChunkScratch;
-    const size_t long_way = copies + kSplitRows * (head_dim * sizeof(float) + sizeof(float2));
+    const long long blocks = ((long long)max_rows + 127) / 128;
+    const int tokens = 128 / (n_head / n_kv);                 // of a tile
+    const size_t sliced = kSplitRows * (head_dim * sizeof(float) + sizeof(float2)) + prefill_acc_bytes(kSplitCtas, head_dim, (blocks + 1) / 2);
+    const size_t whole = prefill_acc_bytes((size_t)n_kv * ((max_batch + tokens - 1) / tokens), head_dim, blocks);
+    const size_t long_way = copies + (sliced > whole ? sliced : whole);
     return head + (long_way > chunk ? long_way : chunk);
 }
 
@@ -703,11 +712,12 @@ int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, voi
         }
     }
     a.tc_hd64 = true;
-    if (!mmq && g_prefill_impl == 0) {
-        a.n_split = prefill_tc_splits(n_head, n_kv, n_past, batch, dev->sm_count);
+    if (g_prefill_impl == 0) {
+        if (!mmq) a.n_split = prefill_tc_splits(n_head, n_kv, n_past, batch, dev->sm_count);
         uint8_t* parts = wsb + head + 2 * align256((size_t)n_kv * rows * head_dim * sizeof(__half));
         a.part_o = reinterpret_cast<float*>(parts);
         a.part_ml = reinterpret_cast<float*>(parts + kSplitRows * head_dim * sizeof(float));
+        a.acc = a.n_split > 1 ? a.part_ml + 2 * kSplitRows : a.part_o;
     }
     e = launch_prefill_q4_prologue(p, s, &g_launches);
     if (e != cudaSuccess) return cuda_fail(e, "prefill (4-bit cache) prologue launch");

@@ -70,7 +70,8 @@ constexpr int OFF_V = OFF_K + NKS * TILE;
 constexpr int OFF_BAR = OFF_V + NVS * TILE;
 constexpr int OFF_MREF = OFF_BAR + 256;         // float [2][128]: reference max published per block parity
 constexpr int OFF_MX = OFF_MREF + 1024;         // float2 [2 teams][128 rows]: (m, l) exchanged at the end
-constexpr int SMEM_BYTES = OFF_MX + 2048 + 1024;   // + slack for 1024-byte alignment
+constexpr int OFF_MACC = OFF_MX + 2048;         // float [128]: reference max of the sums that left TMEM (ACC)
+constexpr int SMEM_BYTES = OFF_MACC + 512 + 1024;   // + slack for 1024-byte alignment
 static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 constexpr long long kWaitCycles = 2000000000LL;    // ~1 s
 constexpr long long kDrainCycles = 200000000LL;    // ~0.1 s
@@ -107,6 +108,7 @@ struct TcArgs {
     int n_head, n_kv, n_past, batch, G, TQ;   // TQ = floor(128 / G) tokens per tile
     float2* part_ml;       // SPLIT: running maximum and sum of each row and slice; the unscaled output goes to part_o through tmO
     int n_split;
+    float4* acc;           // ACC: sums that left TMEM, [CTA][HD/4][128 rows]
     int out_tma;           // the output leaves through shared memory and bulk tensor stores (tmO is valid): 1 fp32, 2 fp16
 };
 
@@ -322,8 +324,35 @@ constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_
 // ... and for P V, N = the head's width.
 template <int HD> constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 
+// ACC: whether the accumulator's sum leaves TMEM in front of block j of nb, so that P_j V_j starts a new one.  The tensor core cuts
+// off what an addition has below the last place of its fp32 sum, always towards zero: in one sum the output is 6.3e-9 of itself short
+// for every row, 5.1e-5 behind 8192 rows, 8.3e-4 behind 131072, 3.3e-3 behind 524288 (measured: 512 tokens of 32/8 heads).  With at
+// most 63 blocks in a sum it is 5.1e-5 at most, 4e-5 behind any number of them: no more than what the fp16 operands cost (1.4e-5 to
+// 1.5e-4).  The sums are added in global memory (L2), in fp32 and rounded to nearest, by the row's own thread.  A sum that leaves
+// costs a CTA about 2.5 us, a block 0.95: after 32 blocks instead of 48 it was 7 % of a long walk for 2.5e-5.
+__host__ __device__ constexpr bool acc_leaves(int j, int nb) { return j > 0 && j % kPrefillAccBlocks == 0 && nb - j >= kPrefillAccRest; }
+static_assert(kPrefillAccBlocks % 2 == 0, "the first softmax team takes the sums");
+
+// acc = the accumulator row at `to`, and keep times what is there unless that is nothing yet.  Out of line, for the registers of the
+// loop that calls it.
+template <int HD>
+__device__ __noinline__ void acc_add(uint32_t to, float4* acc, float keep, bool first) {
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c, acc += 8 * BM) {
+        float4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = first ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(acc + i * BM);
+        float o[32];
+        tmem_ld32(to + 32 * c, o);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            acc[i * BM] = make_float4(fmaf(keep, x[i].x, o[4 * i]), fmaf(keep, x[i].y, o[4 * i + 1]),
+                                      fmaf(keep, x[i].z, o[4 * i + 2]), fmaf(keep, x[i].w, o[4 * i + 3]));
+    }
+}
+
 // SPLIT (see PrefillArgs): a CTA walks one of n_split slices of its tile's KV blocks and leaves the unscaled output.
-template <int HD, bool SPLIT>
+template <int HD, bool SPLIT, bool ACC>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const TcArgs p) {
@@ -483,7 +512,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) dVs[kk] = dV0[kk] + (uint64_t)((sv * TILE) >> 4);
             // commit: accumulator complete up to block j; V stage sv free
-            tc_group_ts(TM_O, TM_S + b * BN, dVs, IDESC_PV<HD>, j > 0 ? 1u : 0u, bar(PV_DONE + sv));
+            tc_group_ts(TM_O, TM_S + b * BN, dVs, IDESC_PV<HD>, j > 0 && !(ACC && acc_leaves(j, nb)) ? 1u : 0u, bar(PV_DONE + sv));
             if (lane == 0) TRACE(0, 3, j);
             // what the next block's P V needs, looked at before the S group below is issued
             const int bn = (b + 1 == NSB) ? 0 : b + 1;
@@ -522,9 +551,15 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t to = TM_O + lane_addr;               // the accumulator row of this thread
         float* s_mref = reinterpret_cast<float*>(smem + OFF_MREF);
         float m_l = -CUDART_INF_F, l = 0.f;                 // this thread's partial row sum and the reference max it is relative to
+        float* s_macc = reinterpret_cast<float*>(smem + OFF_MACC);
+        auto acc_row = [&]() { return p.acc + (((size_t)split * gridDim.y + kvh) * gridDim.x + tile) * (HD / 4 * BM) + row; };
         bool ok = true;
 
-        for (int j = team; j < nb && ok; j += 2) {
+        int j = team;
+        // the blocks of one sum at a time
+        for (int sum = 0;; ++sum) {
+        const int end = ACC && acc_leaves((sum + 1) * kPrefillAccBlocks, nb) ? (sum + 1) * kPrefillAccBlocks : nb;
+        for (; j < end && ok; j += 2) {
             const int b = j % NSB;
             const uint32_t ts = TM_S + lane_addr + b * BN;  // score buffer of this block, this thread's lane
             if (tid == 128 || tid == 256) TRACE(1 + team, 0, j);
@@ -623,10 +658,29 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (lane == 0) mbar_arrive(bar(P_FULL + b));         // one arrival per warp (the barrier counts 4)
             if (tid == 128 || tid == 256) TRACE(1 + team, 5, j);
         }
+        if (!ACC || end == nb || !ok) break;
+        if (team == 0) {
+            // The first team has block j = end in front of it, whose P V waits for this team's P.  O is complete up to block j-1 once
+            // these barriers say so: as in the rescale above, the scores prove that every P V up to j-3 has completed, without which
+            // a barrier could be two phases away from the one waited for.
+            ok = mbar_wait(bar(S_FULL + j % NSB), (j / NSB) & 1, s_abort);
+            if (ok) ok = mbar_wait(bar(PV_DONE + (j & 1)), ((j - 2) >> 1) & 1, s_abort);
+            if (ok) ok = mbar_wait(bar(PV_DONE + ((j - 1) & 1)), ((j - 1) >> 1) & 1, s_abort);
+            if (ok) ok = mbar_wait(bar(MREF + ((j - 1) & 1)), ((j - 1) >> 1) & 1, s_abort);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const float m_now = s_mref[((j - 1) & 1) * BM + row], m_old = sum ? s_macc[row] : -CUDART_INF_F;
+            s_macc[row] = m_now;
+            acc_add<HD>(to, acc_row(), m_old == -CUDART_INF_F ? 0.f : fast_exp2(m_old - m_now), sum == 0);
+        }
+        }
         // ---- add the two teams' row sums and write the output -----------------------------------------
         float2* s_x = reinterpret_cast<float2*>(smem + OFF_MX);
+        const bool have_acc = ACC && nb >= kPrefillAccBlocks + kPrefillAccRest;
         if (ok) {
             s_x[team * 128 + row] = make_float2(m_l, l);
+            if (have_acc && team == 0) __threadfence();     // the sums that left TMEM, for the second team
             mbar_arrive(bar(XCH));
             ok = mbar_wait(bar(XCH), 0, s_abort);
         }
@@ -645,12 +699,25 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const int ptok = SPLIT ? split * (gridDim.x * p.TQ) + tglob : tglob;      // row of the output, or of the slices' outputs
             if (SPLIT && team == 0 && valid)
                 p.part_ml[(size_t)ptok * p.n_head + kvh * p.G + hg] = make_float2(M, w_me * l + w_ot * other.y);
+            const float m_acc = have_acc ? s_macc[row] : -CUDART_INF_F;
+            const float w_acc = m_acc == -CUDART_INF_F ? 0.f : fast_exp2(m_acc - M);
             // this thread writes half of its row's columns, the second team the second half
             float* dst = p.out + ((size_t)ptok * p.n_head + kvh * p.G + hg) * HD + HD / 2 * team;
 #pragma unroll 1
             for (int c = 0; c < NSL; ++c) {
                 float a[32];
                 tmem_ld32(to + HD / 2 * team + 32 * c, a);
+                if (have_acc) {
+                    const float4* acc = acc_row() + (HD / 8 * team + 8 * c) * BM;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 x = __ldcg(acc + i * BM);
+                        a[4 * i] = fmaf(w_acc, x.x, a[4 * i]);
+                        a[4 * i + 1] = fmaf(w_acc, x.y, a[4 * i + 1]);
+                        a[4 * i + 2] = fmaf(w_acc, x.z, a[4 * i + 2]);
+                        a[4 * i + 3] = fmaf(w_acc, x.w, a[4 * i + 3]);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 32; ++i) a[i] *= inv;
                 if (!SPLIT && p.out_tma == 2) {
@@ -789,14 +856,21 @@ bool make_map(CUtensorMap* m, const void* base, int hd, uint64_t d1, uint64_t d2
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD, bool SPLIT>
+template <int HD, bool SPLIT, bool ACC>
 cudaError_t set_attributes() {
     // the register budgets are shares of what the kernel is compiled with
     cudaFuncAttributes fa;
-    cudaError_t e = cudaFuncGetAttributes(&fa, prefill_tc_kernel<HD, SPLIT>);
+    cudaError_t e = cudaFuncGetAttributes(&fa, prefill_tc_kernel<HD, SPLIT, ACC>);
     if (e != cudaSuccess) return e;
     if (fa.numRegs * kThreads < kRegsService * 128 + kRegsSoftmax * (kThreads - 128)) return cudaErrorInvalidConfiguration;
-    return cudaFuncSetAttribute(prefill_tc_kernel<HD, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    return cudaFuncSetAttribute(prefill_tc_kernel<HD, SPLIT, ACC>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+}
+template <int HD>
+cudaError_t set_attributes_hd() {
+    cudaError_t e;
+    if ((e = set_attributes<HD, false, false>()) != cudaSuccess || (e = set_attributes<HD, false, true>()) != cudaSuccess) return e;
+    if ((e = set_attributes<HD, true, false>()) != cudaSuccess) return e;
+    return set_attributes<HD, true, true>();
 }
 // a.n_split > 1, `tokens`: see PrefillArgs
 cudaError_t launch_merge(const PrefillArgs& a, int tokens, cudaStream_t stream, unsigned long long* launches) {
@@ -810,8 +884,9 @@ cudaError_t launch_merge(const PrefillArgs& a, int tokens, cudaStream_t stream, 
 template <int HD>
 cudaError_t launch_kernel(dim3 grid, bool split, cudaStream_t stream, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                           const CUtensorMap& o, const TcArgs& t) {
-    return split ? launch_dependent(prefill_tc_kernel<HD, true>, grid, kThreads, SMEM_BYTES, stream, 1, q, k, v, o, t)
-                 : launch_dependent(prefill_tc_kernel<HD, false>, grid, kThreads, SMEM_BYTES, stream, 1, q, k, v, o, t);
+    auto go = [&](auto kernel) { return launch_dependent(kernel, grid, kThreads, SMEM_BYTES, stream, 1, q, k, v, o, t); };
+    if (split) return t.acc ? go(prefill_tc_kernel<HD, true, true>) : go(prefill_tc_kernel<HD, true, false>);
+    return t.acc ? go(prefill_tc_kernel<HD, false, true>) : go(prefill_tc_kernel<HD, false, false>);
 }
 
 } // namespace
@@ -832,9 +907,8 @@ cudaError_t prefill_tc_set_attributes() {
         g_encode = reinterpret_cast<EncodeTiledFn>(fn);
     }
     cudaError_t e;
-    if ((e = set_attributes<128, false>()) != cudaSuccess || (e = set_attributes<128, true>()) != cudaSuccess) return e;
-    if ((e = set_attributes<64, false>()) != cudaSuccess) return e;
-    return set_attributes<64, true>();
+    if ((e = set_attributes_hd<128>()) != cudaSuccess) return e;
+    return set_attributes_hd<64>();
 }
 
 // A CTA takes about 0.9 us a block; writing the slices' outputs and joining them 5 to 6 together, so eight blocks have to be saved.  64
@@ -873,6 +947,9 @@ cudaError_t launch_prefill_tc(const PrefillArgs& a, int sm_count, cudaStream_t s
     t.out_tma = a.n_split > 1 ? 1 : (a.out16 ? 2 : (out_tma ? 1 : 0));
     t.part_ml = reinterpret_cast<float2*>(a.part_ml);
     t.n_split = a.n_split;
+    // (the longest walk of a CTA: the last tile's blocks, or its share of them)
+    const long long walk = (a.n_past + a.batch + BN - 1) / BN;
+    t.acc = (walk + a.n_split - 1) / a.n_split >= kPrefillAccBlocks + kPrefillAccRest ? reinterpret_cast<float4*>(a.acc) : nullptr;
     t.out = a.out;
     t.out16 = a.out16;
     t.out_mmq = a.out_mmq;
