@@ -388,13 +388,16 @@ def decode_q4_workspace(n_head, n_kv, head_dim):
 
 def prefill_q4_workspace(n_head, n_kv, head_dim, batch, rows):
     """Scratch for attn_prefill_q4 calls with n_past + batch <= rows; it serves every layer.  A block that became too small is
-    kept: work on a stream torch does not know of, or a captured graph, may still be using it."""
+    kept: work on a stream torch does not know of, or a captured graph, may still be using it.  So that few are, a block has
+    room for chunks of 512 tokens from the start and twice the length or the rows where either was not enough."""
     key = (n_head, n_kv, head_dim, torch._C._cuda_getDevice())
     have = _state["prefill_q4_ws"].setdefault(key, [])           # [(batch, rows, block)], the newest last
     if have and batch <= have[-1][0] and rows <= have[-1][1]:
         return have[-1][2]
     if have:
-        batch, rows = max(batch, have[-1][0]), max(rows, 2 * have[-1][1] if rows > have[-1][1] else have[-1][1])
+        rows = max(rows, 2 * have[-1][1] if rows > have[-1][1] else have[-1][1])
+        batch = max(batch, min(2 * have[-1][0], rows) if batch > have[-1][0] else have[-1][0])
+    batch = max(batch, min(512, rows))
     nbytes = capi.lib().oattn_prefill_q4_workspace_bytes(n_head, n_kv, head_dim, batch, rows)
     if nbytes == 0:
         raise capi.AttnError(capi.ERR_UNSUPPORTED, "prefill shape not supported")

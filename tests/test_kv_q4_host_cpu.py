@@ -1,0 +1,51 @@
+"""CPU tests of the host side of the 4-bit cache: what the default workspace of the prefill call grows to."""
+import pytest
+import torch
+
+from orin_llm_b200 import build, capi
+
+
+@pytest.fixture
+def ops(monkeypatch):
+    """The module with no workspace yet, and with storage-less blocks in place of the GPU's."""
+    build.build()
+    from orin_llm_b200 import ops as _ops
+    real = torch.empty
+    monkeypatch.setitem(_ops._state, "prefill_q4_ws", {})
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: real(*a, **{**k, "device": "meta"}))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
+    return _ops
+
+
+def kept(ops):
+    return [b for have in ops._state["prefill_q4_ws"].values() for _, _, b in have]
+
+
+@pytest.mark.parametrize("n_ctx,lengths,most", [(32768, range(45, 513), 1), (32768, range(1, 4097), 4), (300, range(1, 301), 1), (40, [1, 40], 1)])
+def test_longer_and_longer_prompts_keep_few_workspaces(ops, n_ctx, lengths, most):
+    L = capi.lib()
+    for n in lengths:
+        ws = ops.prefill_q4_workspace(32, 8, 128, n, n_ctx)
+        assert ws.numel() >= L.oattn_prefill_q4_workspace_bytes(32, 8, 128, n, n_ctx)
+    assert len(kept(ops)) <= most
+
+
+def test_longer_and_longer_contexts_keep_few_workspaces(ops):
+    L = capi.lib()
+    for rows in range(100, 20000, 37):
+        ws = ops.prefill_q4_workspace(12, 2, 64, min(rows, 700), rows)
+        assert ws.numel() >= L.oattn_prefill_q4_workspace_bytes(12, 2, 64, min(rows, 700), rows)
+    # 100 rows doubled until they are 20000
+    assert len(kept(ops)) <= 9
+    # all of them together are less than what the last two would be, and a small context's block holds no more than its own rows
+    sizes = [b.numel() for b in kept(ops)]
+    assert sum(sizes) <= 2.5 * sizes[-1] + 9 * L.oattn_prefill_q4_workspace_bytes(12, 2, 64, 700, 700)
+    assert sizes[0] == L.oattn_prefill_q4_workspace_bytes(12, 2, 64, 100, 100)
+
+
+def test_a_chunk_longer_than_its_rows_has_no_workspace(ops):
+    with pytest.raises(capi.AttnError):
+        ops.prefill_q4_workspace(8, 2, 128, 600, 100)
+    ops.prefill_q4_workspace(8, 2, 128, 100, 300)
+    with pytest.raises(capi.AttnError):
+        ops.prefill_q4_workspace(8, 2, 128, 1000, 300)
