@@ -11,8 +11,9 @@
 // is an fp16 subnormal, exactly code * 2^-20, and the powers of two go into q and the final scale.  The left operands q and
 // P d are fp32; a decode step has at most eight heads per CTA, so the other eight rows of the tile hold what the rounding of the
 // first eight to fp16 left over (x = hi + lo, 22 bits together): the result keeps fp32 accuracy and the instruction count is
-// the same.  q is scaled by a power of two per head, P d by a fixed one that a warp lowers, starting over, when its sums overflowed,
-// so that neither half leaves the fp16 range.
+// the same.  q is scaled by a power of two per head, P d by one that goes by the largest step d so far and is lowered when a larger
+// one comes, as a running maximum is, with the sums so far: so neither half leaves the fp16 range, and what the rounding of
+// P d loses is at most 2^-22 of it or 2^-38 of the largest step.
 //
 // What bounds it: the warp-level matrix instruction takes its scheduler 8.1 cycles and lets nothing else issue beside it (measured:
 // with 8 fp32 multiply-adds per product 16.0 cycles, with 4 logic operations 13.2), so a 16-position block costs a scheduler its
@@ -381,7 +382,34 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
     // low halves in lanes t >= 2), dim 16 j + 2 r (o[2j]) and the next (o[2j+1])
     F2 o[HD / 8], om[NG];
     F2 m_run, l_run;                                         // per head (the same twice, and the two keys' shares, where a lane has one)
-    float pscale = 8192.f;                                   // P d is carried times this
+    // P d is carried times `pscale`; d_lim = 2^16 / pscale, the first step that would leave fp16 (P is at most 1).  The same in all lanes,
+    // but for a chunk's last blocks, where a row goes by the positions it sees.
+    float pscale = 137438953472.f, d_lim = 4.76837158203125e-7f;       // 2^37: the smallest step, 2^-24, comes to 2^13
+    auto lower = [&](float d_max) {                          // brings d_max to [2^13, 2^14): steps up to four times as large fit after it
+        if (!(d_max >= d_lim)) return;
+        const uint32_t e = __float_as_uint(d_max) >> 23, next = (267 - e) << 23;      // exponent fields
+        const float by = __uint_as_float(next - __float_as_uint(pscale) + (127u << 23));
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) o[j] = o[j] * F2(by, by);
+        pscale = __uint_as_float(next);
+        d_lim = __uint_as_float((e + 3) << 23);
+    };
+    auto finite = [](float d) { return d <= 65504.f ? d : 0.f; };
+    // ... before P d of the NB blocks at `blk`, all of whose rows count: a lane looks at one row, or at the same as another lane
+    auto fit = [&](int nb, const uint8_t* blk) {
+        const uint8_t* at = blk + (nb == 2 ? lane >> 4 : 0) * F::BLOCK + F::VS_OFF + (lane & 15) * F::SROWB;
+        float d0, d1 = 0.f;
+        if constexpr (NG == 2) {
+            const uint2 w = *reinterpret_cast<const uint2*>(at);
+            d0 = half_lo(w.x);
+            d1 = half_lo(w.y);
+        } else {
+            d0 = half_lo(*reinterpret_cast<const uint32_t*>(at));
+        }
+        if (!__any_sync(0xffffffffu, fmaxf(d0, d1) >= d_lim)) return;
+        // (a step that is not finite shows in the output at any scale; positive numbers are in the order of their bits)
+        lower(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(finite(d0), finite(d1))))));
+    };
 
     // One turn over NB blocks that lie next to each other in the ring.
     auto turn = [&](auto nb_c, const uint8_t* blk, int nrow, int nrow_all) {
@@ -463,6 +491,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
                     if (8 * j + 2 * t >= nrow) vs[j][0][g] = 0u;
                     if (8 * j + 2 * t + 1 >= nrow) vs[j][1][g] = 0u;
                 }
+            float d_max = 0.f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) d_max = fmaxf(d_max, fmaxf(finite(half_lo(vs[j][0][g])), finite(half_lo(vs[j][1][g]))));
+            d_max = fmaxf(d_max, __shfl_xor_sync(0xffffffffu, d_max, 1));
+            lower(fmaxf(d_max, __shfl_xor_sync(0xffffffffu, d_max, 2)));
+        } else {
+            fit(NB, blk);
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -582,6 +619,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         }
         l_run = fma2(l_run, alpha, sum);
 
+        fit(NB, blk);
         uint32_t vs[NT][NG];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -627,23 +665,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         }
     };
 
-    // P d is carried times 2^13, which overflows fp16 where a step is 8 or more (values of V spread over more than 120).
-    // Infinities cannot leave the sums again, so one look at the end finds them; the warp then looks its steps up and
-    // starts over with a power of two that holds for them, unless it is the data that are not finite.
-    for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) o[j] = F2(0.f, 0.f);
 #pragma unroll
     for (int g = 0; g < NG; ++g) om[g] = F2(0.f, 0.f);
     m_run = F2(-CUDART_INF_F, -CUDART_INF_F);
     l_run = F2(0.f, 0.f);
-    if (pass) {
-#pragma unroll
-        for (int k = 0; k < kTurns; ++k) {
-            if (k < turns) load_turn(k);
-            cp_async_commit();
-        }
-    }
     for (int it = 0; it < turns; ++it) {
         cp_async_wait<kTurns - 1>();
         __syncwarp();
@@ -691,28 +718,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) decode_q4_kernel(const __grid
         cp_async_commit();
     }
     cp_async_wait<0>();
-    F2 any = o[0];
-#pragma unroll
-    for (int j = 1; j < HD / 8; ++j) any = any + o[j];
-    // (an infinity or a NaN in any of them leaves no finite sum)
-    if (!__any_sync(0xffffffffu, !(fabsf(any.x()) + fabsf(any.y()) <= 3.402823466e38f))) break;
-    float d_max = 0.f;
-    for (int it = 0; it < turns; ++it) {
-        const int b0 = first(it), nb = plan.step == 2 && b0 + 1 < blk1 ? 2 : 1;
-        for (int i = lane; i < nb * 16 * NG; i += 32) {
-            const int row = b0 * 16 + i / NG;
-            uint32_t w = 0u;
-            if (owner && row == new_pos) w = s_new[64 + 2 + i % NG];
-            else if (row < npos) w = *reinterpret_cast<const uint32_t*>(cache + (size_t)(row >> 4) * F::BLOCK + F::VS_OFF + (row & 15) * F::SROWB + 4 * (i % NG));
-            const float d = half_lo(w);
-            if (d <= 65504.f) d_max = fmaxf(d_max, d);
-        }
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) d_max = fmaxf(d_max, __shfl_xor_sync(0xffffffffu, d_max, off));
-    if (!(d_max * pscale > 65000.f)) break;                  // nothing overflowed: the data are not finite
-    pscale = __uint_as_float((uint32_t)(127 + 14 - ((int)(__float_as_uint(d_max) >> 23) - 127)) << 23);     // d_max * pscale in [2^14, 2^15)
-    }
 
     // ---- merge the warps: O of a warp scaled by e^(m_w - M), sums in warp order ----------------------------------
     __syncthreads();

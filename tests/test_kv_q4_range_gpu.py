@@ -1,14 +1,19 @@
-"""GPU tests of the 4-bit cache over its range: long sums, steps far apart, values beyond fp16, long rolls.  Tolerances not derived
-here: test_kv_q4_gpu.py."""
+"""GPU tests of the 4-bit cache over its range: long sums, steps that are small or far apart.  Tolerances not derived here:
+test_kv_q4_gpu.py."""
 import math
 
 import numpy as np
 import pytest
 import torch
 
-from test_kv_q4_gpu import long_cache, prefill_bound
+import q4_reference as ref
+from test_kv_q4_gpu import decode_bound, dev, filled, long_cache, prefill_bound, rows
 
 pytestmark = pytest.mark.gpu
+
+
+def dpos(p):
+    return torch.tensor([p], dtype=torch.int32, device="cuda")
 
 
 # ------------------------------------------------------------------------------------------------- sums over long contexts
@@ -67,3 +72,137 @@ def test_a_long_chunk_repeats_itself(ops, n_head, n_kv, hd, past, batch):
         assert float((outs[0][:, h] - want).abs().max()) <= bound
         # ... which is for the worst case: roundings of random sign leave a tenth of it in the mean
         assert float((outs[0][:, h] - want).norm() / want.norm()) <= 1e-3
+
+
+# ------------------------------------------------------------------------------------------------- steps
+def repeated_row(rng, n_kv, hd, n, step, at, amp=1.0):
+    """A cache of n rows that are all alike -- K zero, V of about 15 steps -- but for row `at`, whose K is amp times a random row and
+    whose V is zero.  The cache (on the GPU; every kv head the same), K and V of row `at`, V of the others."""
+    block = np.zeros((1, 1, 18 * hd), np.uint8)
+    zero = np.zeros((16, 1, hd), np.float32)
+    v = (step * rng.integers(0, 16, (1, 1, hd))).astype(np.float32)
+    v[..., ::64], v[..., 1::64] = 0, 15 * step
+    ref.write_rows(block, hd, range(16), zero, np.repeat(v, 16, 0))
+    cache = dev(block).expand(n_kv, (n + 15) // 16, 18 * hd).contiguous()
+    k = (amp * rng.standard_normal((1, 1, hd))).astype(np.float32)
+    ref.write_rows(block, hd, [at % 16], k, zero[:1])
+    cache[:, at // 16] = dev(block[:, 0])
+    K, V = ref.read_rows(block, hd, 16)
+    return cache, K[0, at % 16], V[0, (at + 1) % 16]
+
+
+def repeated_row_attention(q, k, v, n, scale):
+    """q [n_head][hd] over that cache: n - 1 rows of score 0 and value v, one of score q . k and value 0.  And the bound's `most`."""
+    s = (q.astype(np.float64) @ k) * np.float32(scale)
+    rest = (n - 1) * np.exp(-s)
+    return (rest / (1 + rest))[:, None] * v, float((np.abs(q.astype(np.float64)) @ np.abs(k)).max())
+
+
+# Many kv heads leave one CTA to each, whose eight warps walk 885 rows apiece.
+@pytest.mark.parametrize("step", [1e-2, 1e-4, 1e-5, 2.0 ** -24])
+@pytest.mark.parametrize("group,hd", [(1, 64), (3, 128), (4, 64), (8, 64), (8, 128)])
+def test_decode_counts_small_values_behind_a_dominant_row(ops, group, hd, step):
+    """One row has nearly all of the weight, the others a sum of weights of the size of the bound ten times over: what they add to the
+    output is not lost, however small the steps of their values."""
+    rng = np.random.default_rng(300)
+    n_kv, n, at = 160, 8 * 885, 1234
+    n_head, scale = n_kv * group, 1.0 / math.sqrt(hd)
+    cache, k, v = repeated_row(rng, n_kv, hd, n, step, at)
+    # the dominant row's score is 13 to 17
+    q = np.stack([k * (13 + 4 * i / group) / (scale * (k @ k)) for i in range(group)]).astype(np.float32)
+    out = torch.empty(n_head, hd, device="cuda")
+    ops.attn_decode_q4(dev(np.tile(q, (n_kv, 1))), None, None, cache, out, n_head, n_kv, hd, n, dpos(n - 1), scale, ops.FUSE_NONE)
+    want, most = repeated_row_attention(q, k, v, n, scale)
+    err = np.abs(out.view(n_kv, group, hd).cpu().numpy() - want).max()
+    assert err <= decode_bound(most, scale, v), (err, decode_bound(most, scale, v))
+
+
+@pytest.mark.parametrize("step", [1e-2, 1e-5])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_short_chunk_counts_small_values_behind_a_dominant_row(ops, hd, step):
+    rng = np.random.default_rng(301)
+    n_kv, group, batch = 24, 4, 2
+    n, at, scale = 12 * 8 * 885, 1234, 1.0 / math.sqrt(hd)
+    n_head = n_kv * group
+    cache, k, v = repeated_row(rng, n_kv, hd, n, step, at)
+    q = np.stack([k * (13 + 4 * i / group) / (scale * (k @ k)) for i in range(group)]).astype(np.float32)
+    out = torch.empty(batch, n_head, hd, device="cuda")
+    ops.attn_prefill_q4(dev(np.tile(q, (batch, n_kv, 1))), None, None, cache, out, n_head, n_kv, hd, n, n - batch, batch, scale, ops.FUSE_NONE)
+    for b in range(batch):
+        want, most = repeated_row_attention(q, k, v, n - batch + b + 1, scale)
+        err = np.abs(out[b].view(n_kv, group, hd).cpu().numpy() - want).max()
+        assert err <= decode_bound(most, scale, v), (err, decode_bound(most, scale, v))
+
+
+AMPLITUDES = {"growing": lambda n: np.logspace(-6, 4, n), "falling": lambda n: np.logspace(4, -6, n),
+              "one large": lambda n: np.where(np.arange(n) == n // 3, 1e4, 1e-3), "none, then small": lambda n: np.where(np.arange(n) < n // 2, 0, 1e-5)}
+
+
+@pytest.mark.parametrize("order", sorted(AMPLITUDES))
+@pytest.mark.parametrize("n_head,n_kv,hd", [(2, 2, 128), (3, 1, 64), (8, 2, 128), (4, 1, 64), (8, 1, 64), (14, 2, 128), (16, 1, 128)])
+def test_decode_with_steps_far_apart(ops, n_head, n_kv, hd, order):
+    """Steps that grow, fall or jump along the context: those of ten orders of magnitude are summed in one scale after another."""
+    rng = np.random.default_rng(302)
+    n, scale = 1500, 0.3 / math.sqrt(hd)
+    k, v = rows(rng, n, n_kv, hd), rng.standard_normal((n, n_kv, hd)).clip(-6, 6)
+    v = (v * AMPLITUDES[order](n)[:, None, None]).astype(np.float32)
+    cache = np.zeros((n_kv, (n + 15) // 16, 18 * hd), np.uint8)
+    ref.write_rows(cache, hd, range(n), k, v)
+    K, V = ref.read_rows(cache, hd, n)
+    q = rng.standard_normal((1, n_head, hd)).astype(np.float32)
+    out = torch.empty(n_head, hd, device="cuda")
+    for length in (n, 500, 40):
+        ops.attn_decode_q4(dev(q[0]), None, None, dev(cache), out, n_head, n_kv, hd, n, dpos(length - 1), scale, ops.FUSE_NONE)
+        want, most = ref.attend(q, K[:, :length], V[:, :length], length - 1, scale)
+        err = np.abs(out.cpu().numpy() - want[0]).max()
+        assert err <= decode_bound(most, scale, V[:, :length]), (length, err, decode_bound(most, scale, V[:, :length]))
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd", [(2, 2, 64), (8, 2, 128), (4, 1, 64), (7, 1, 64), (14, 2, 128), (16, 1, 128)])
+@pytest.mark.parametrize("amp_old,amp_new", [(1e-3, 9000.0), (0.01, 400.0), (9000.0, 1e-3), (1.0, 1.0)])
+def test_decode_with_a_step_of_its_own_for_the_appended_row(ops, n_head, n_kv, hd, amp_old, amp_new):
+    rng = np.random.default_rng(303)
+    scale = 1.0 / math.sqrt(hd)
+    for length in (1, 17, 300, 1030):
+        cache = np.zeros((n_kv, (length + 20) // 16 + 1, 18 * hd), np.uint8)
+        n_ctx = 16 * cache.shape[1]
+        k, v = rows(rng, length, n_kv, hd), rng.standard_normal((length, n_kv, hd)).clip(-6, 6)
+        v[:-1] *= amp_old
+        v[-1] *= amp_new
+        v = v.astype(np.float32)
+        if length > 1:
+            ref.write_rows(cache, hd, range(length - 1), k[:-1], v[:-1])
+        q = rng.standard_normal((1, n_head, hd)).astype(np.float32)
+        d_cache, out = dev(cache), torch.empty(n_head, hd, device="cuda")
+        ops.attn_decode_q4(dev(q[0]), dev(k[-1]), dev(v[-1]), d_cache, out, n_head, n_kv, hd, n_ctx, dpos(length - 1), scale, ops.FUSE_KV_APPEND)
+        ref.write_rows(cache, hd, [length - 1], k[-1:], v[-1:])
+        assert np.array_equal(d_cache.cpu().numpy(), cache)
+        K, V = ref.read_rows(cache, hd, length)
+        want, most = ref.attend(q, K, V, length - 1, scale)
+        err = np.abs(out.cpu().numpy() - want[0]).max()
+        assert err <= decode_bound(most, scale, V), (length, err, decode_bound(most, scale, V))
+
+
+@pytest.mark.parametrize("bad", [1e6, np.nan])
+@pytest.mark.parametrize("n_head,n_kv,chunk", [(4, 1, 0), (8, 1, 0), (8, 1, 3)])
+def test_a_step_that_is_not_finite_stays_in_its_group(ops, n_head, n_kv, chunk, bad):
+    """A range beyond 15 fp16 steps, or a NaN, in the first 64 values of a row: the other 64 of the output are what they would be."""
+    rng = np.random.default_rng(304)
+    hd, n, scale = 128, 333, 0.0884
+    cache = filled(rng, n_kv, hd, n, n)
+    v = rows(rng, 1, n_kv, hd)
+    v[0, :, 3] = bad
+    ref.write_rows(cache, hd, [200], rows(rng, 1, n_kv, hd), v)
+    m = max(chunk, 1)
+    q = rng.standard_normal((m, n_head, hd)).astype(np.float32)
+    out = torch.empty(m, n_head, hd, device="cuda")
+    if chunk:
+        ops.attn_prefill_q4(dev(q), None, None, dev(cache), out, n_head, n_kv, hd, n, n - m, m, scale, ops.FUSE_NONE)
+    else:
+        ops.attn_decode_q4(dev(q[0]), None, None, dev(cache), out[0], n_head, n_kv, hd, n, dpos(n - 1), scale, ops.FUSE_NONE)
+    K, V = ref.read_rows(cache, hd, n)
+    assert not np.isfinite(V[:, 200, :64]).any() and np.isfinite(np.delete(V, 200, 1)).all()
+    want, most = ref.attend(q, K, np.nan_to_num(V), n - m, scale)
+    got = out.cpu().numpy()
+    assert not np.isfinite(got[..., :64]).any()
+    assert np.abs(got[..., 64:] - want[..., 64:]).max() <= decode_bound(most, scale, V[..., 64:])
