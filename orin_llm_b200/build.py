@@ -5,6 +5,7 @@
 nvcc cross-compiles without a GPU.  The CUDA runtime is linked statically so that the library
 does not depend on which libcudart the host process has loaded.
 """
+import contextlib
 import os
 import shutil
 import subprocess
@@ -53,30 +54,40 @@ BINDING_SRC = os.path.join(HERE, "host", "torch_binding.cpp")
 
 
 def build_binding(force=False):
-    """The torch binding of the 4-bit cache's calls (host/torch_binding.cpp), linked against the C-ABI library."""
+    """The torch binding of the 4-bit cache's calls (host/torch_binding.cpp), linked against the C-ABI library.  Returns at once
+    where the one that is there is newer than its source and header and was made for this torch and this Python."""
     import sysconfig
 
     import torch
-    build(force=False)
     stamp = "%s %s" % (torch.__version__, sys.version.split()[0])       # it is bound to both
     stamp_file = BINDING_LIB + ".for"
     deps = [BINDING_SRC, os.path.join(HERE, "..", "include", "orin_attn_b200.h")]
     if (not force and os.path.exists(BINDING_LIB) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp
             and all(os.path.getmtime(d) <= os.path.getmtime(BINDING_LIB) for d in deps)):
         return BINDING_LIB
+    build(force=False)
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
-    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-o", BINDING_LIB, BINDING_SRC,
+    made = "%s.%d" % (BINDING_LIB, os.getpid())             # put in place whole: another process may load or build it now
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-o", made, BINDING_SRC,
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
            "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
            "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
            "-L" + LIBDIR, "-lorin_attn_b200", "-Wl,-rpath,$ORIGIN"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError("_q4_binding.so is missing or was built for another torch, Python or source (here: torch and Python %s), and "
+                           "g++ does not run to build it: %s" % (stamp, e)) from e
     if r.returncode != 0:
         raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
-    with open(stamp_file, "w") as f:
+    with contextlib.suppress(FileNotFoundError):
+        os.remove(stamp_file)                               # (without one the file in between counts as stale)
+    os.replace(made, BINDING_LIB)
+    with open("%s.%d" % (stamp_file, os.getpid()), "w") as f:
         f.write(stamp)
+    os.replace(f.name, stamp_file)
     return BINDING_LIB
 
 

@@ -7,7 +7,6 @@ torch is used only for device memory and streams.  There is no CPU implementatio
 """
 import ctypes
 import math
-import os
 
 import torch
 
@@ -322,15 +321,15 @@ _binding = None
 
 
 def _q4():
-    """The module that checks the tensors and makes the C calls (host/torch_binding.cpp); built with the library, or on first use."""
+    """The module that checks the tensors and makes the C calls (host/torch_binding.cpp); built with the library, or on first use, and
+    again where it was made for another torch, Python or source."""
     global _binding
     if _binding is None:
         import importlib.util
 
         from . import build
         capi.lib()
-        path = build.BINDING_LIB if os.path.exists(build.BINDING_LIB) else build.build_binding()
-        spec = importlib.util.spec_from_file_location("_q4_binding", path)
+        spec = importlib.util.spec_from_file_location("_q4_binding", build.build_binding())
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         _binding = module

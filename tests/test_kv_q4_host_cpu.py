@@ -49,3 +49,59 @@ def test_a_chunk_longer_than_its_rows_has_no_workspace(ops):
     ops.prefill_q4_workspace(8, 2, 128, 100, 300)
     with pytest.raises(capi.AttnError):
         ops.prefill_q4_workspace(8, 2, 128, 1000, 300)
+
+
+# ------------------------------------------------------------------------------------------------- the compiled binding
+class Compiled(Exception):
+    pass
+
+
+@pytest.fixture
+def binding(monkeypatch, tmp_path):
+    """The built binding's files at a place of their own, a compiler that only says that it was called, and nothing loaded yet."""
+    import os
+    import shutil
+    from orin_llm_b200 import ops as _ops
+    build.build()
+    path = str(tmp_path / "_q4_binding.so")
+    for end in ("", ".for"):
+        shutil.copy2(build.build_binding() + end, path + end)
+
+    def run(cmd, *a, **k):
+        raise Compiled(os.path.basename(cmd[0]))
+    monkeypatch.setattr(build, "BINDING_LIB", path)
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(_ops, "_binding", None)
+    return _ops, path
+
+
+def test_a_current_binding_is_not_built_again(binding):
+    _, path = binding
+    assert build.build_binding() == path
+
+
+@pytest.mark.parametrize("stale", ["torch", "older", "no stamp"])
+def test_a_stale_binding_is_not_loaded(binding, stale):
+    """Made for another torch or Python, or before its source or header changed: built again, not mapped."""
+    import os
+    ops, path = binding
+    if stale == "torch":
+        open(path + ".for", "w").write("1.0.0 3.0.0")
+    elif stale == "older":
+        t = os.path.getmtime(build.BINDING_SRC) - 60
+        os.utime(path, (t, t))
+    else:
+        os.remove(path + ".for")
+    with pytest.raises(Compiled, match="g\\+\\+"):
+        ops._q4()
+
+
+def test_a_binding_that_cannot_be_built_says_so(binding, monkeypatch):
+    ops, path = binding
+    open(path + ".for", "w").write("1.0.0 3.0.0")
+
+    def run(cmd, *a, **k):
+        raise FileNotFoundError(cmd[0])
+    monkeypatch.setattr(build.subprocess, "run", run)
+    with pytest.raises(RuntimeError, match="_q4_binding.so was built for"):
+        ops._q4()
