@@ -103,5 +103,5 @@ def test_a_binding_that_cannot_be_built_says_so(binding, monkeypatch):
     def run(cmd, *a, **k):
         raise FileNotFoundError(cmd[0])
     monkeypatch.setattr(build.subprocess, "run", run)
-    with pytest.raises(RuntimeError, match="_q4_binding.so was built for"):
+    with pytest.raises(RuntimeError, match="_q4_binding.so is missing or was built for"):
         ops._q4()
