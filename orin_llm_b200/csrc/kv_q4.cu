@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kStoreThreads, 5) kv_store_q4_kernel(uint8_t* 
 // One warp turns rows [row0, row1) of a block into fp16; dk, dv: where row 0 of the block would go.  K: a lane takes the four
 // (two) code words of place t of a row, 16 bytes, and writes 16-byte pieces, four lanes 64 bytes.  V: a word holds a pair of
 // dims of four rows, so the block passes through shared memory (`s_v`, kVStride bytes a row: the lanes' 4-byte stores
-// then fall into 32 different banks).  32768 positions of 8 heads: 28.7 us for 172 MB, 0.92 of the measured copy bandwidth; a warp
+// then fall into 32 different banks).  FIT: for products, where a group with a value beyond fp16 is NaN (see q4_fit).  32768 positions of 8 heads: 28.7 us for 172 MB, 0.92 of the measured copy bandwidth; a warp
 // per row with byte loads took 61.5 us.
 template <int HD>
 constexpr int kVStride = HD * 2 + 16;
@@ -148,7 +148,11 @@ __device__ __forceinline__ uint4 q4_eight(uint32_t w, float d, float m) {
     return make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
 }
 
-template <int HD>
+// The step of a group whose values become operands in fp16.  One that holds a larger value counts as NaN: as an infinity it would
+// give a score of minus infinity where the query is negative, and the row would vanish from a softmax that it belongs to.
+__device__ __forceinline__ float q4_fit(float d, float m) { return fmaf(15.f, d, m) >= 65520.f ? CUDART_NAN_F : d; }
+
+template <int HD, bool FIT>
 __device__ __forceinline__ void q4_load_block(const uint8_t* blk, __half* dk, __half* dv, int row0, int row1, uint8_t* s_v, int lane) {
     using F = Q4<HD>;
     constexpr int NW = HD / 32, NG = F::NG;
@@ -181,6 +185,7 @@ __device__ __forceinline__ void q4_load_block(const uint8_t* blk, __half* dk, __
     auto dm = [](uint32_t w, float& d, float& m) {
         d = __half2float(__ushort_as_half((uint16_t)w));
         m = __half2float(__ushort_as_half((uint16_t)(w >> 16)));
+        if (FIT) d = q4_fit(d, m);
     };
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -234,7 +239,7 @@ __global__ void __launch_bounds__(32 * kLoadWarps) kv_load_q4_kernel(const uint8
     const uint8_t* blk = cache + ((size_t)head * q4_blocks(n_ctx) + b) * Q4<HD>::BLOCK;
     // row 0 of the block; may lie in front of the destination, whose rows outside [row0, row1) are not touched
     const long long at = ((long long)head * dst_ctx + dst_base + 16 * b - row_base) * HD;
-    q4_load_block<HD>(blk, reinterpret_cast<__half*>(kc) + at, reinterpret_cast<__half*>(vc) + at, max(row_base - 16 * b, 0),
+    q4_load_block<HD, false>(blk, reinterpret_cast<__half*>(kc) + at, reinterpret_cast<__half*>(vc) + at, max(row_base - 16 * b, 0),
                       min(row_base + rows - 16 * b, 16), s_v[warp], lane);
 }
 
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kerne
         if (job >= (long long)a.n_kv * nb) return;
         const int head = (int)(job / nb), b = (int)(job % nb);
         const size_t dst = ((size_t)head * rows + 16 * b) * HD;
-        q4_load_block<HD>(p.cache + ((size_t)head * nblk + b) * F::BLOCK, p.k16 + dst, p.v16 + dst, 0, min(expand - 16 * b, 16), s_v[warp], lane);
+        q4_load_block<HD, true>(p.cache + ((size_t)head * nblk + b) * F::BLOCK, p.k16 + dst, p.v16 + dst, 0, min(expand - 16 * b, 16), s_v[warp], lane);
         return;
     }
     const int b = idx, pos = a.n_past + b;
@@ -526,7 +531,7 @@ __global__ void __launch_bounds__(kPrologueThreads, 4) prefill_q4_prologue_kerne
             else             q4_store_row<HD, false>(blk, pos & 15, codes, s, lane);
             if (p.q32) continue;
             __half* dst = (r.kind == 1 ? p.k16 : p.v16) + ((size_t)r.head * rows + pos) * HD + F::EPL * lane;
-            const float d = __half2float(s.d), m = __half2float(s.m);
+            const float m = __half2float(s.m), d = q4_fit(__half2float(s.d), m);
 #pragma unroll
             for (int e = 0; e < F::EPL; e += 2)
                 *reinterpret_cast<uint32_t*>(dst + e) = pack_half2(q4_value((codes >> (4 * e)) & 15u, d, m), q4_value((codes >> (4 * e + 4)) & 15u, d, m));

@@ -1,4 +1,5 @@
-"""GPU tests of the 4-bit cache over its range: long sums, steps that are small or far apart.  Tolerances not derived here:
+"""GPU tests of the 4-bit cache over its range: long sums, steps that are small or far apart, values beyond fp16.
+Tolerances not derived here:
 test_kv_q4_gpu.py."""
 import math
 
@@ -206,3 +207,48 @@ def test_a_step_that_is_not_finite_stays_in_its_group(ops, n_head, n_kv, chunk, 
     got = out.cpu().numpy()
     assert not np.isfinite(got[..., :64]).any()
     assert np.abs(got[..., 64:] - want[..., 64:]).max() <= decode_bound(most, scale, V[..., 64:])
+
+
+# ------------------------------------------------------------------------------------------------- values beyond fp16
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("batch", [1, 5, 600])
+@pytest.mark.parametrize("which,where", [("k", 7), ("v", 7), ("k", 40), ("v", 40)])
+def test_a_value_beyond_fp16(ops, which, where, batch, hd):
+    """The format holds 1e5 behind a minimum and a step that fit fp16.  Decode and a short chunk work on the codes; a long chunk works on
+    fp16 copies, where such a row is NaN and shows, and is never another finite number.  Row 7 lies in front of the chunk, row 40 is
+    its first."""
+    rng = np.random.default_rng(305)
+    n_head, n_kv, past, scale = 4, 2, 40, 1.0 / math.sqrt(hd)
+    n = past + batch
+    q, k, v = rng.standard_normal((batch, n_head, hd)).astype(np.float32), rows(rng, n, n_kv, hd), rows(rng, n, n_kv, hd)
+    q[..., :64] *= 1e-5 if which == "k" else 1
+    (k if which == "k" else v)[where, 1, 3] = 1e5
+    q[..., 3] = -np.abs(q[..., 3])
+    cache = np.zeros((n_kv, (n + 15) // 16, 18 * hd), np.uint8)
+    ref.write_rows(cache, hd, range(past), k[:past], v[:past])
+    d_cache, out = dev(cache), torch.empty(batch, n_head, hd, device="cuda")
+    if batch == 1:
+        ops.attn_decode_q4(dev(q[0]), dev(k[past]), dev(v[past]), d_cache, out[0], n_head, n_kv, hd, n, dpos(past), scale, ops.FUSE_KV_APPEND)
+    else:
+        ops.attn_prefill_q4(dev(q), dev(k[past:]), dev(v[past:]), d_cache, out, n_head, n_kv, hd, n, past, batch, scale, ops.FUSE_KV_APPEND)
+    ref.write_rows(cache, hd, range(past, n), k[past:], v[past:])
+    assert np.array_equal(d_cache.cpu().numpy(), cache)
+    K, V = ref.read_rows(cache, hd, n)
+    assert (K if which == "k" else V)[1, where].max() > 65520
+    want, most = ref.attend(q, K, V, past, scale)
+    got = out.cpu().numpy()
+    if batch < 100:
+        assert np.abs(got - want).max() <= decode_bound(most, scale, V)
+        return
+    # the first kv head's heads have nothing to do with it, nor has the second half of V
+    assert np.abs(got[:, :2] - want[:, :2]).max() <= prefill_bound(most, scale, V[0], False)
+    if which == "k":
+        assert np.isnan(got[:, 2:]).all()
+    else:
+        assert np.isnan(got[:, 2:, :64]).all()
+        if hd == 128:
+            assert np.abs(got[:, 2:, 64:] - want[:, 2:, 64:]).max() <= prefill_bound(most, scale, V[1, :, 64:], False)
+    # read back, the value is the nearest fp16 number
+    kh, vh = (torch.empty(n_kv, n, hd, dtype=torch.float16, device="cuda") for _ in range(2))
+    ops.kv_load_q4(d_cache, kh, vh, n_kv, hd, n, 0, n)
+    assert float((kh if which == "k" else vh)[1, where, 3]) == math.inf
