@@ -1,6 +1,5 @@
-"""GPU tests of the 4-bit cache over its range: long sums, steps that are small or far apart, values beyond fp16.
-Tolerances not derived here:
-test_kv_q4_gpu.py."""
+"""GPU tests of the 4-bit cache over its range: long sums, steps that are small or far apart, values beyond fp16, long rolls.
+Tolerances that are not derived here: test_kv_q4_gpu.py."""
 import math
 
 import numpy as np
@@ -252,3 +251,32 @@ def test_a_value_beyond_fp16(ops, which, where, batch, hd):
     kh, vh = (torch.empty(n_kv, n, hd, dtype=torch.float16, device="cuda") for _ in range(2))
     ops.kv_load_q4(d_cache, kh, vh, n_kv, hd, n, 0, n)
     assert float((kh if which == "k" else vh)[1, where, 3]) == math.inf
+
+
+# ------------------------------------------------------------------------------------------------- rolls of many steps
+def row_bytes(cache, hd, which):
+    """Codes (a byte per pair of dims) and scales of every row of a cache on the GPU, uint8 [heads][rows][bytes]."""
+    even = np.arange(0, hd, 2)
+    at = np.stack([(ref.v_byte if which else ref.k_byte)(hd, s, even) for s in range(16)])
+    scale = 16 * hd + which * hd + np.arange(hd).reshape(16, -1)
+    at = torch.from_numpy(np.concatenate((at, scale), 1)).cuda()
+    return cache[..., at.reshape(-1)].view(cache.shape[0], -1, at.shape[1])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_layer,n_kv,n_ctx,n_keep,shift", [(1, 2, 2049, 0, 1), (2, 2, 4000, 7, 13), (1, 3, 5000, 20, 16), (1, 2, 12345, 1000, 5555),
+                                                             (2, 1, 30011, 3, 511), (1, 1, 8192, 5, 4094), (1, 2, 6000, 100, 5900), (1, 1, 2600, 515, 512)])
+def test_a_roll_of_many_steps(ops, hd, n_layer, n_kv, n_ctx, n_keep, shift):
+    """Contexts of more steps than are in flight at once, so that a window is filled while another leaves and used again: every byte."""
+    gen = torch.Generator(device="cuda").manual_seed(306)
+    cache = ops.KVCacheQ4(n_layer, n_kv, n_ctx, hd)
+    cache.buf.copy_(torch.randint(0, 256, cache.buf.shape, dtype=torch.uint8, device="cuda", generator=gen))
+    before = cache.buf.view(n_layer * n_kv, -1, 18 * hd).clone()
+    for _ in range(2):                                     # the second one rolls what the first one left
+        cache.shift(n_keep, shift)
+        after = cache.buf.view_as(before)
+        for which in (0, 1):
+            want, got = row_bytes(before, hd, which), row_bytes(after, hd, which)
+            moved = torch.cat((want[:, :n_keep], want[:, n_keep + shift: n_ctx], torch.zeros_like(want[:, :shift]), want[:, n_ctx:]), 1)
+            assert torch.equal(got, moved)
+        before = after.clone()
