@@ -189,7 +189,7 @@ struct DecodeQ4Args {
     // (token, head) pairs, heads_per_cta = 8 of them per CTA, q is rotated already and the chunk's rows are in the cache.
     int n_past = 0, batch = 0;
     __half* out16 = nullptr;            // fp16 output of a chunk, instead of `out`
-    int emit_partial = 0;
+    static constexpr int emit_partial = 0;       // always the normalised output (emit_final)
     int8_t* out_qs = nullptr;
     float* out_scales = nullptr;
 };
