@@ -63,9 +63,10 @@ def build_binding(force=False):
     stamp_file = BINDING_LIB + ".for"
     deps = [BINDING_SRC, os.path.join(HERE, "..", "include", "orin_attn_b200.h")]
     if (not force and os.path.exists(BINDING_LIB) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp
-            and all(os.path.getmtime(d) <= os.path.getmtime(BINDING_LIB) for d in deps)):
+            and all(os.path.getmtime(d) <= os.path.getmtime(BINDING_LIB) for d in deps if os.path.exists(d))):
         return BINDING_LIB
-    build(force=False)
+    if not os.path.exists(LIB):                             # (one that is there may be loaded already, and stays as it is)
+        build()
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     made = "%s.%d" % (BINDING_LIB, os.getpid())             # put in place whole: another process may load or build it now

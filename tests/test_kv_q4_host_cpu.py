@@ -105,3 +105,20 @@ def test_a_binding_that_cannot_be_built_says_so(binding, monkeypatch):
     monkeypatch.setattr(build.subprocess, "run", run)
     with pytest.raises(RuntimeError, match="_q4_binding.so is missing or was built for"):
         ops._q4()
+
+
+def test_the_library_is_not_built_again_under_its_binding(binding, monkeypatch):
+    """It may be loaded already: the binding would be linked to a second one, which was never initialised."""
+    ops, path = binding
+    open(path + ".for", "w").write("1.0.0 3.0.0")
+    monkeypatch.setattr(build, "needs_build", lambda: True)
+    with pytest.raises(Compiled, match="g\\+\\+"):
+        ops._q4()
+
+
+def test_a_binding_without_its_source_is_current(binding, monkeypatch):
+    """An installed package has no header and may have no source."""
+    _, path = binding
+    monkeypatch.setattr(build, "BINDING_SRC", path + ".cpp")
+    monkeypatch.setattr(build, "HERE", path + ".package")
+    assert build.build_binding() == path
