@@ -42,7 +42,7 @@ const at::Tensor& tensor(const char* name, PyObject* o) {
 }
 
 const char* name_of(at::ScalarType t) {
-    return t == at::kFloat ? "float32" : t == at::kHalf ? "float16" : t == at::kByte ? "uint8" : t == at::kInt ? "int32" : c10::toString(t);
+    return t == at::kFloat ? "float32" : t == at::kHalf ? "float16" : t == at::kByte ? "uint8" : t == at::kInt ? "int32" : t == at::kChar ? "int8" : c10::toString(t);
 }
 
 // Address of a contiguous tensor of that type with at least `numel` elements on CUDA device `dev`.
@@ -89,11 +89,41 @@ const oattn_rope_params* rope_of(PyObject* o, oattn_rope_params& r, int dev) {
     return &r;
 }
 
-const oattn_ext* ext_of(PyObject* o) {
+// Device of the cache, whatever it is: what comes with it is checked against that before it is itself (cache_of).
+int device_of(PyObject* o) { return (int)tensor("cache", o).get_device(); }
+
+// The extras of the attention calls, a dict of the C struct's members, for `batch` tokens.
+const oattn_ext* ext_of(PyObject* o, oattn_ext& e, int n_head, int n_kv, int hd, int batch, int dev) {
     if (o == Py_None) return nullptr;
-    void* p = PyLong_AsVoidPtr(o);
-    if (!p && PyErr_Occurred()) throw Refused();
-    return static_cast<const oattn_ext*>(p);
+    if (!PyDict_Check(o)) refuse(PyExc_TypeError, "ext: a dict is needed, got %s", Py_TYPE(o)->tp_name);
+    if (PyDict_GET_SIZE(o) == 0) return nullptr;
+    e = oattn_ext();
+    Py_ssize_t known = 0;
+    auto get = [&](const char* name) {
+        PyObject* v = PyDict_GetItemString(o, name);         // borrowed
+        if (v) ++known;
+        return v && v != Py_None ? v : nullptr;
+    };
+    auto member = [&](const char* name, at::ScalarType type, long long numel) {
+        PyObject* v = get(name);
+        return v ? address(name, v, type, numel, dev) : nullptr;
+    };
+    const long long nq = (long long)n_head * hd, nk = (long long)n_kv * hd;
+    e.bias_q = static_cast<const float*>(member("bias_q", at::kFloat, nq));
+    e.bias_k = static_cast<const float*>(member("bias_k", at::kFloat, nk));
+    e.bias_v = static_cast<const float*>(member("bias_v", at::kFloat, nk));
+    e.norm_q = static_cast<const float*>(member("norm_q", at::kFloat, hd));
+    e.norm_k = static_cast<const float*>(member("norm_k", at::kFloat, hd));
+    e.out_qs = static_cast<int8_t*>(member("out_qs", at::kChar, nq));
+    e.out_scales = static_cast<float*>(member("out_scales", at::kFloat, nq / 32));
+    e.out_mmq = member("out_mmq", at::kByte, (long long)batch * n_head * 144);       // one block of 128 values per token and head
+    if (PyObject* v = get("norm_eps")) e.norm_eps = to_float(v);
+    if (PyObject* v = get("out_mmq_ds4")) {
+        e.out_mmq_ds4 = PyObject_IsTrue(v);
+        if (e.out_mmq_ds4 < 0) throw Refused();
+    }
+    if (known != PyDict_GET_SIZE(o)) refuse(PyExc_ValueError, "unknown extension keys in %R", o);
+    return &e;
 }
 
 template <typename F>
@@ -145,11 +175,13 @@ PyObject* kv_shift_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// (q, k_new, v_new, cache, out | None, n_head, n_kv, head_dim, n_ctx, d_pos, scale, fuse, rope | None, ext address | None, workspace,
+// (q, k_new, v_new, cache, out | None, n_head, n_kv, head_dim, n_ctx, d_pos, scale, fuse, rope | None, ext | None, workspace,
 //  stream | None)
 PyObject* decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 16, [&] {
         const int n_head = to_int(a[5]), n_kv = to_int(a[6]), hd = to_int(a[7]), n_ctx = to_int(a[8]), fuse = to_int(a[11]);
+        oattn_ext x;
+        const oattn_ext* ext = ext_of(a[13], x, n_head, n_kv, hd, 1, device_of(a[3]));
         const Cache c = cache_of(a[3], 1, n_kv, hd, n_ctx);
         const float* q = static_cast<const float*>(address("q", a[0], at::kFloat, (long long)n_head * hd, c.dev));
         const float *k = nullptr, *v = nullptr;
@@ -157,7 +189,6 @@ PyObject* decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
             k = static_cast<const float*>(address("k_new", a[1], at::kFloat, (long long)n_kv * hd, c.dev));
             v = static_cast<const float*>(address("v_new", a[2], at::kFloat, (long long)n_kv * hd, c.dev));
         }
-        const oattn_ext* ext = ext_of(a[13]);
         float* out = nullptr;
         if (a[4] != Py_None || !ext || !ext->out_qs) out = static_cast<float*>(address("out", a[4], at::kFloat, (long long)n_head * hd, c.dev));
         const int* d_pos = static_cast<const int*>(address("d_pos", a[9], at::kInt, 1, c.dev));
@@ -169,11 +200,13 @@ PyObject* decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// (q, k_new, v_new, cache, out | None, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse, rope | None, ext address | None,
+// (q, k_new, v_new, cache, out | None, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse, rope | None, ext | None,
 //  workspace, stream | None); out: fp32 or fp16
 PyObject* prefill_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 17, [&] {
         const int n_head = to_int(a[5]), n_kv = to_int(a[6]), hd = to_int(a[7]), n_ctx = to_int(a[8]), batch = to_int(a[10]), fuse = to_int(a[12]);
+        oattn_ext x;
+        const oattn_ext* ext = ext_of(a[14], x, n_head, n_kv, hd, batch, device_of(a[3]));
         const Cache c = cache_of(a[3], 1, n_kv, hd, n_ctx);
         const long long nq = (long long)batch * n_head * hd, nk = (long long)batch * n_kv * hd;
         const float* q = static_cast<const float*>(address("q", a[0], at::kFloat, nq, c.dev));
@@ -182,7 +215,6 @@ PyObject* prefill_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
             k = static_cast<const float*>(address("k_new", a[1], at::kFloat, nk, c.dev));
             v = static_cast<const float*>(address("v_new", a[2], at::kFloat, nk, c.dev));
         }
-        const oattn_ext* ext = ext_of(a[14]);
         float* out = nullptr;
         uint16_t* out16 = nullptr;
         if (a[4] != Py_None || !ext || !ext->out_mmq) {

@@ -336,11 +336,6 @@ def _q4():
     return _binding
 
 
-def _ext_address(ext):
-    ref, keep = _ext_params(ext)
-    return (None if ref is None else ctypes.addressof(keep)), keep
-
-
 def kv_q4_bytes(n_kv, head_dim, n_ctx):
     """Bytes of one layer of a 4-bit cache (oattn_kv_q4_bytes); 0 for a shape that has none."""
     if n_kv <= 0 or n_ctx <= 0 or n_ctx > 1 << 30 or head_dim not in (64, 128):
@@ -409,10 +404,8 @@ def attn_decode_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, d
     """attn_decode over one layer of a 4-bit cache, the new row quantised and appended in the same launch.  Calls that may run
     at the same time, graph replays among them, need workspaces of their own (of decode_q4_workspace's size)."""
     ws = workspace if workspace is not None else decode_q4_workspace(n_head, n_kv, head_dim)
-    ea, keep = _ext_address(ext) if ext else (None, None)
-    capi.check(_q4().decode_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, d_pos, scale, fuse, rope, ea, ws,
+    capi.check(_q4().decode_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, d_pos, scale, fuse, rope, ext, ws,
                                _state["stream"]))
-    del keep
 
 
 def attn_prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse=FUSE_ALL, rope=None,
@@ -421,10 +414,8 @@ def attn_prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, 
     [batch][n_head][head_dim].  The default workspace holds one layer's rows in fp16, for all n_ctx of them; calls that may run
     at the same time need workspaces of their own."""
     ws = workspace if workspace is not None else prefill_q4_workspace(n_head, n_kv, head_dim, batch, max(n_ctx, batch))
-    ea, keep = _ext_address(ext) if ext else (None, None)
-    capi.check(_q4().prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse, rope, ea, ws,
+    capi.check(_q4().prefill_q4(q, k_new, v_new, cache, out, n_head, n_kv, head_dim, n_ctx, n_past, batch, scale, fuse, rope, ext, ws,
                                 _state["stream"]))
-    del keep
 
 
 class KVCacheQ4:

@@ -122,3 +122,52 @@ def test_a_binding_without_its_source_is_current(binding, monkeypatch):
     monkeypatch.setattr(build, "BINDING_SRC", path + ".cpp")
     monkeypatch.setattr(build, "HERE", path + ".package")
     assert build.build_binding() == path
+
+
+# ------------------------------------------------------------------------------------------------- tensors around the attention
+N_HEAD, N_KV, HD, BATCH = 6, 2, 128, 3
+EXTRAS = {"bias_q": (torch.float32, N_HEAD * HD), "bias_k": (torch.float32, N_KV * HD), "bias_v": (torch.float32, N_KV * HD),
+          "norm_q": (torch.float32, HD), "norm_k": (torch.float32, HD), "out_qs": (torch.int8, N_HEAD * HD),
+          "out_scales": (torch.float32, N_HEAD * HD // 32), "out_mmq": (torch.uint8, BATCH * N_HEAD * 144)}
+
+
+def call_with(extra, prefill):
+    from orin_llm_b200 import ops as _ops
+    build.build()
+    cache, x = torch.zeros(N_KV, 1, 18 * HD, dtype=torch.uint8), torch.zeros(BATCH, N_HEAD, HD)
+    ws = torch.zeros(1, dtype=torch.uint8)
+    if prefill:
+        _ops.attn_prefill_q4(x, x, x, cache, x, N_HEAD, N_KV, HD, 16, 0, BATCH, 0.1, _ops.FUSE_KV_APPEND, None, ws, extra)
+    else:
+        _ops.attn_decode_q4(x, x, x, cache, x, N_HEAD, N_KV, HD, 16, torch.zeros(1, dtype=torch.int32), 0.1, _ops.FUSE_KV_APPEND, None, ws, extra)
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("name", sorted(EXTRAS))
+def test_extras_of_the_wrong_kind_are_refused(name, prefill):
+    """Before anything is launched, and by name.  (What is in order gets as far as the cache, which is not on a GPU here.)"""
+    dtype, numel = EXTRAS[name]
+    with pytest.raises(ValueError, match="current CUDA device"):
+        call_with({name: torch.zeros(numel, dtype=dtype)}, prefill)
+    if name != "out_mmq" or prefill:                       # (a decode call takes the blocks of one token, which the C entry refuses)
+        with pytest.raises(ValueError, match="%s: .*at least" % name):
+            call_with({name: torch.zeros(numel - 1, dtype=dtype)}, prefill)
+    with pytest.raises(ValueError, match=name + ": "):
+        call_with({name: torch.zeros(numel, dtype=torch.float16)}, prefill)
+    with pytest.raises(ValueError, match="%s: .*not contiguous" % name):
+        call_with({name: torch.zeros(2, numel, dtype=dtype).t()}, prefill)
+    with pytest.raises(TypeError, match=name + ": a tensor"):
+        call_with({name: 12345}, prefill)
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+def test_extras_that_are_no_extras(prefill):
+    for extra in ({}, {"norm_eps": 1e-6}, {"bias_q": None, "out_mmq_ds4": True}):
+        with pytest.raises(ValueError, match="current CUDA device"):
+            call_with(extra, prefill)
+    with pytest.raises(ValueError, match="unknown extension"):
+        call_with({"nonsense": 1}, prefill)
+    with pytest.raises(TypeError, match="dict"):
+        call_with([1], prefill)
+    with pytest.raises(TypeError):
+        call_with({"norm_eps": "small"}, prefill)

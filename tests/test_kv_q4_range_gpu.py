@@ -280,3 +280,60 @@ def test_a_roll_of_many_steps(ops, hd, n_layer, n_kv, n_ctx, n_keep, shift):
             moved = torch.cat((want[:, :n_keep], want[:, n_keep + shift: n_ctx], torch.zeros_like(want[:, :shift]), want[:, n_ctx:]), 1)
             assert torch.equal(got, moved)
         before = after.clone()
+
+
+# ------------------------------------------------------------------------------------------------- what stands around the attention
+def test_block_output_of_a_long_context(ops):
+    """The blocks next to the fp32 output and instead of it, behind more rows than go into one sum."""
+    n_head, n_kv, hd, past, batch = 8, 2, 128, 9000, 149
+    n = past + batch
+    raw, _, V = long_cache(ops, n_kv, hd, n)
+    q = torch.randn(batch, n_head, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(307))
+    f32, blk = torch.empty(batch, n_head, hd, device="cuda"), [torch.zeros(n_head * batch * 144, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    for out, b in ((f32, blk[0]), (None, blk[1])):
+        ops.attn_prefill_q4(q, None, None, raw, out, n_head, n_kv, hd, n, past, batch, 0.0884, ops.FUSE_NONE, ext=dict(out_mmq=b))
+    assert torch.equal(blk[0], blk[1])
+    b = blk[0].view(n_head, batch, 144)
+    d = b[..., :16].contiguous().view(torch.float32)
+    val = (b[..., 16:].contiguous().view(torch.int8).view(n_head, batch, 4, 32).float() * d[..., None]).reshape(n_head, batch, hd).transpose(0, 1)
+    assert ((val - f32).abs() <= 0.5001 * d.transpose(0, 1).repeat_interleave(32, -1) + 1e-7).all()
+    # Without the blocks the rows are cut into slices, whose weights are relative to maxima of their own: both calls round each weight to
+    # fp16, by 2^-11 of it at most, so the two means of the values lie within twice that of the largest value, and the sums' share.
+    other = torch.empty_like(f32)
+    ops.attn_prefill_q4(q, None, None, raw, other, n_head, n_kv, hd, n, past, batch, 0.0884, ops.FUSE_NONE)
+    assert float((other - f32).abs().max()) <= (2 * 2.0 ** -11 + 2 * 63 * 8 * 2.0 ** -23) * float(V.abs().max())
+
+
+@pytest.mark.parametrize("batch", [1, 4, 200])
+def test_a_bias_at_any_address(ops, batch):
+    """Biases are read one number at a time: those of a packed parameter block may begin anywhere."""
+    rng = np.random.default_rng(308)
+    n_head, n_kv, hd, past = 12, 4, 64, 30
+    n, scale, rope = past + batch, 0.125, (1, hd, 1e4, None)
+    base, q = dev(filled(rng, n_kv, hd, n, past)), dev(rng.standard_normal((batch, n_head, hd)).astype(np.float32))
+    k, v = (dev(rows(rng, batch, n_kv, hd)) for _ in range(2))
+    sizes = [n_head * hd, n_kv * hd, n_kv * hd]
+    packed = dev(rng.standard_normal(sum(sizes) + 3).astype(np.float32))
+    res = []
+    for shift in (0, 1, 3):
+        where = packed.new_empty(packed.numel() + 3)
+        where[shift: shift + packed.numel()] = packed
+        bias = dict(zip(("bias_q", "bias_k", "bias_v"), where[shift:].split(sizes + [where.numel() - shift - sum(sizes)])))
+        cache, out = base.clone(), torch.empty(batch, n_head, hd, device="cuda")
+        if batch == 1:
+            ops.attn_decode_q4(q[0], k[0], v[0], cache, out[0], n_head, n_kv, hd, n, dpos(past), scale, ops.FUSE_ALL, rope, ext=bias)
+        else:
+            ops.attn_prefill_q4(q, k, v, cache, out, n_head, n_kv, hd, n, past, batch, scale, ops.FUSE_ALL, rope, ext=bias)
+        res.append((cache, out))
+    assert all(torch.equal(x, y) for r in res for x, y in zip(r, res[0]))
+
+
+def test_extras_on_another_device_are_refused(ops):
+    c, x = ops.KVCacheQ4(1, 2, 64, 128).layer(0), torch.zeros(1, 2, 128, device="cuda")
+    good = dict(bias_q=torch.zeros(256, device="cuda"))
+    ops.attn_decode_q4(x, x, x, c, x.clone(), 2, 2, 128, 64, dpos(0), 0.1, ops.FUSE_KV_APPEND, ext=good)
+    for bad in (dict(bias_q=torch.zeros(256)), dict(norm_k=torch.zeros(128)), dict(bias_q=torch.zeros(128, device="cuda"))):
+        with pytest.raises(ValueError, match=list(bad)[0] + ": "):
+            ops.attn_decode_q4(x, x, x, c, x.clone(), 2, 2, 128, 64, dpos(0), 0.1, ops.FUSE_KV_APPEND, ext=bad)
+        with pytest.raises(ValueError, match=list(bad)[0] + ": "):
+            ops.attn_prefill_q4(x, x, x, c, x.clone(), 2, 2, 128, 64, 0, 1, 0.1, ops.FUSE_KV_APPEND, ext=bad)
