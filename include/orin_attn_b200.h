@@ -310,7 +310,8 @@ int oattn_prefill_status(const void* workspace, int n_head, int head_dim, int ba
  * A byte belongs to one row: writing a row leaves the bytes of every other row as they are.  Rows that were never
  * written may hold anything; no call lets them into a result.
  *
- * `cache` must be 16-byte aligned; k, v, q, k_new, v_new and out likewise.  head_dim 64 or 128. */
+ * `cache` must be 16-byte aligned; k, v, q, k_new, v_new and out likewise (biases and norms may lie anywhere).  head_dim 64 or
+ * 128. */
 size_t oattn_kv_q4_bytes(int n_kv, int head_dim, int n_ctx);
 
 /* oattn_kv_store into the 4-bit cache: rows k, v [batch][heads][head_dim] fp32 at positions pos_base + b, or with d_pos

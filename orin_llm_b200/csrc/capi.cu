@@ -576,7 +576,6 @@ int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void
     const bool q8_only = ext && ext->out_qs;
     if (!q || (!out && !q8_only) || !d_pos || !(scale > 0.0f)) return OATTN_ERR_ARG;
     if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new) & 15) return OATTN_ERR_ARG;
-    if (ext && (((uintptr_t)ext->bias_q | (uintptr_t)ext->bias_k | (uintptr_t)ext->bias_v) & 15)) return OATTN_ERR_ARG;
     if (fuse & ~OATTN_FUSE_ALL) return OATTN_ERR_ARG;
     if ((fuse & OATTN_FUSE_ROPE_K) && !(fuse & OATTN_FUSE_KV_APPEND)) return OATTN_ERR_ARG;
     if ((fuse & OATTN_FUSE_KV_APPEND) && (!k_new || !v_new)) return OATTN_ERR_ARG;
@@ -654,7 +653,6 @@ int oattn_prefill_q4(const float* q, const float* k_new, const float* v_new, voi
     if (mmq && (head_dim != 128 || g_prefill_impl != 0 || ((uintptr_t)ext->out_mmq & 15))) return OATTN_ERR_UNSUPPORTED;
     if (batch <= 0 || n_past < 0 || n_past > n_ctx - batch) return OATTN_ERR_ARG;
     if (((uintptr_t)out | (uintptr_t)out_f16 | (uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new) & 15) return OATTN_ERR_ARG;
-    if (ext && (((uintptr_t)ext->bias_q | (uintptr_t)ext->bias_k | (uintptr_t)ext->bias_v) & 15)) return OATTN_ERR_ARG;
     if (fuse & ~OATTN_FUSE_ALL) return OATTN_ERR_ARG;
     if ((fuse & OATTN_FUSE_ROPE_K) && !(fuse & OATTN_FUSE_KV_APPEND)) return OATTN_ERR_ARG;
     if ((fuse & OATTN_FUSE_KV_APPEND) && (!k_new || !v_new)) return OATTN_ERR_ARG;
