@@ -349,7 +349,9 @@ int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void
  * [batch][n_head][head_dim]): pass one of them; with ext->out_mmq both may be NULL.  A short chunk (up to 1024 (token, head)
  * pairs for head_dim 128, 2048 for 64; fewer behind more than 900 rows, 300 to 500 behind 8192) is attended from the 4-bit
  * rows themselves, with the accuracy of oattn_decode_q4, in two launches; a longer one, or one with ext->out_mmq, on fp16
- * copies of the rows, which the first of two or three launches makes in the workspace: a row's group with a value beyond fp16
+ * copies of the rows, which the first of two or three launches makes in the workspace, and with fp16 queries and softmax weights,
+ * as oattn_prefill_ex: errors of fp16 size whatever the output's type, 0.3e-4 to 2e-4 of the output, at any context length (who
+ * needs less passes the chunk in short pieces).  On this way a row's group with a value beyond fp16
  * (m + 15 d of 65520 or more) is NaN there, while decode and a short chunk take it as it is.  A NaN in a row or a query shows in
  * the outputs that see it (on the second way in those of earlier tokens of the chunk, too, as in oattn_prefill_ex).  The
  * workspace is sized for `max_rows` = the largest n_past + batch and serves all layers; it need not be cleared, and calls

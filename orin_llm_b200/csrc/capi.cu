@@ -611,6 +611,9 @@ int oattn_decode_q4(const float* q, const float* k_new, const float* v_new, void
 // 18.7, 2048 18.4 against 20.2, 4096 23.7 against 21.6; 8 tokens behind 4096 rows 17.6 against 21.6, 8192 22.5 against 24.4; 4
 // tokens behind 32768 rows 33 against 61.  Heads of 64: 64 tokens (256 eights) behind 512 rows 13.1 against 14.6, 1024 16.0
 // against 18.2; 16 tokens behind 4096 rows 17.2 against 18.0; 8 tokens behind 8192 rows 16.3 against 21.0, 32768 32 against 37.
+// Over 405 shapes (groups of 1 to 8 heads, 1 to 16 kv heads, 16 to 256 eights, 0 to 32768 rows) the rule's way is within 1.2 of the
+// better one, within 1.1 in 396, but for one: 16 tokens of 16/16 heads of 128 behind 32768 rows take 112 us the long way, 53 the
+// short one (the copies of many kv heads, which the rule does not look at).
 static int chunk_blocks(int n_head, int n_kv, int head_dim, int n_past, int batch) {
     const long long blocks = ((long long)batch * (n_head / n_kv) + 7) / 8;
     const int limit = head_dim == 128 ? min(128, 24 + (96 << 10) / max(n_past, 1)) : min(256, 32 + (224 << 10) / max(n_past, 1));

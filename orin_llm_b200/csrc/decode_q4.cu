@@ -16,11 +16,12 @@
 // P d loses is at most 2^-22 of it or 2^-38 of the largest step.
 //
 // What bounds it: the warp-level matrix instruction takes its scheduler 8.1 cycles and lets nothing else issue beside it (measured:
-// with 8 fp32 multiply-adds per product 16.0 cycles, with 4 logic operations 13.2), so a 16-position block costs a scheduler its
-// 32 products plus about 220 other instructions, 640 cycles; at the measured copy bandwidth the bytes would arrive in 400.  One
-// million rows of 16/2 heads: 85 us, 3.55 TB/s of cache, 0.54 of the copy bandwidth (the fp16 cache: 158 us).  Eight warps per
-// SM instead of sixteen run as fast (91 us), so latency is not the limit.  The 8-bit float form of the instruction is emulated
-// (21 cycles); the 8-bit integer form takes the same 8.1 for twice the depth, but q needs three digits, so nothing is won.
+// with 8 fp32 multiply-adds per product 16.0 cycles, with 4 logic operations 13.2).  A 16-position block is 32 products, 259 cycles,
+// and about 340 other instructions (counted by ncu), 600 cycles of a scheduler; every further block takes one 0.33 us, which is about
+// that at the clocks seen, and at the measured copy bandwidth its bytes would arrive in 0.21.  One million rows of 16/2 heads: 86 to
+// 87 us, 3.5 TB/s of cache, 0.53 of the copy bandwidth (the fp16 cache: 158 us).  8, 12 and 16 warps per SM took 90.8, 87.5 and 88.9
+// us at the time, so latency is not the limit.  The 8-bit float form of the instruction is emulated (21 cycles); the 8-bit integer
+// form takes the same 8.1 for twice the depth, but q needs three digits, so nothing is won.
 // At a few thousand rows a call is a chain of dependent round trips: 5.3 us from launch to output in one CTA, 2.3 more for a merge.
 #include <type_traits>
 

@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kStoreThreads, 5) kv_store_q4_kernel(uint8_t* 
 // One warp turns rows [row0, row1) of a block into fp16; dk, dv: where row 0 of the block would go.  K: a lane takes the four
 // (two) code words of place t of a row, 16 bytes, and writes 16-byte pieces, four lanes 64 bytes.  V: a word holds a pair of
 // dims of four rows, so the block passes through shared memory (`s_v`, kVStride bytes a row: the lanes' 4-byte stores
-// then fall into 32 different banks).  FIT: for products, where a group with a value beyond fp16 is NaN (see q4_fit).  32768 positions of 8 heads: 28.7 us for 172 MB, 0.92 of the measured copy bandwidth; a warp
+// then fall into 32 different banks).  FIT: for products, where a group with a value beyond fp16 is NaN (see q4_fit).  32768 positions of 8 heads: 28.8 us for 172 MB, 0.91 of the measured copy bandwidth; a warp
 // per row with byte loads took 61.5 us.
 template <int HD>
 constexpr int kVStride = HD * 2 + 16;
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kShiftThreads) kv_shift_q4_kernel(uint8_t* cac
 // reads.  The other CTAs turn the cache rows in front of the chunk into fp16, once for all query tiles: expanding them inside
 // the attention kernel would repeat that for each of its tiles (16 for 512 tokens of a 4-head group), on the warps that bound it.
 // 512 tokens of 32/8 heads behind 8192 rows: 19 us on a cold cache, 13 for the tokens alone (instruction issue, 0.6 of the slots:
-// a warp takes a row at a time) and 9.6 for the rows alone (43 MB); the attention behind it takes 70.  Queries rotated in registers instead
+// a warp takes a row at a time) and 9.6 for the rows alone (43 MB); the attention behind it takes 72.  Queries rotated in registers instead
 // of through shared memory: 1.1 us less, included.
 // For a short chunk (see DecodeQ4Args) the queries stay fp32 and nothing is copied: the decode kernel reads the 4-bit rows.
 constexpr int kPrologueThreads = 256;

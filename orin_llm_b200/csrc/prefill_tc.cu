@@ -10,7 +10,8 @@
 // serves all G query heads of floor(128/G) tokens (when G does not divide 128 the last few tile rows are
 // zero and unused).  The KV sequence is walked in blocks of
 // 128 rows.  Heads of 128; heads of 64 (one slab per tile, half the MMA work, the same softmax) for callers that ask for them:
-// 512 tokens of 32/8 heads of 64 behind 8192 rows 77 us with the prologue, 157 on the warp-level kernel.
+// 512 tokens of 32/8 heads of 64 behind 8192 rows 77 us with the prologue, 157 on the warp-level kernel; exp2 and the hand-over of
+// maxima bound it as they do for heads of 128, with the tensor pipe 31 % busy instead of 58.
 // 384 threads = three warpgroups (warps 2 and 3 only hold the place that makes the softmax teams whole warpgroups,
 // so that registers can be moved to them); three roles:
 //   warp 0   (one lane)  TMA producer: Q tile once, then 128-row K blocks (three-stage ring) and V blocks
@@ -33,6 +34,12 @@
 //                        exp2; fp16 P stored back to TMEM (tcgen05.st).  Each thread keeps its own partial
 //                        row sum; the two are added at the end and O/l goes to global memory.
 // TMEM: 3 x 128 score columns + 128 accumulator columns = 512.
+//
+// Operands are fp16 because the tensor core has no wider form at this rate (tf32 has the same 11 bits; a second product for the low
+// halves of Q alone is half as much matrix work again): Q once it is rotated and scaled, K and V as the cache or the copies of its
+// rows hold them, P as it is stored to TMEM.  Sums, maxima and the row sum (of P before it is rounded) are fp32.  Relative to the
+// output, over 4-bit rows made fp16: Q 3.0e-5 to 9.3e-5, K 1.3e-5 to 9.6e-5, V 0.8e-5 to 9.1e-5, P 0.9e-5 to 6.4e-5, the four together
+// 3.4e-5 behind 8192 rows and up to 1.7e-4 in a few hundred; an fp16 output adds 2e-4.
 //
 // What bounds the loop (measured with clock stamps and with a stand-alone issue-rate kernel): an M128 N128 K16 MMA
 // takes the tensor pipe 64 cycles, 1024 per KV block, whether its A operand comes from shared memory or from TMEM and
@@ -327,8 +334,7 @@ template <int HD> constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint3
 // ACC: whether the accumulator's sum leaves TMEM in front of block j of nb, so that P_j V_j starts a new one.  The tensor core cuts
 // off what an addition has below the last place of its fp32 sum, always towards zero: in one sum the output is 6.3e-9 of itself short
 // for every row, 5.1e-5 behind 8192 rows, 8.3e-4 behind 131072, 3.3e-3 behind 524288 (measured: 512 tokens of 32/8 heads).  With at
-// most 63 blocks in a sum it is 5.1e-5 at most, 4e-5 behind any number of them: no more than what the fp16 operands cost (1.4e-5 to
-// 1.5e-4).  The sums are added in global memory (L2), in fp32 and rounded to nearest, by the row's own thread.  A sum that leaves
+// most 63 blocks in a sum it is 5.1e-5 at most, 4e-5 behind any number of them: no more than what the fp16 operands cost.  The sums are added in global memory (L2), in fp32 and rounded to nearest, by the row's own thread.  A sum that leaves
 // costs a CTA about 2.5 us, a block 0.95: after 32 blocks instead of 48 it was 7 % of a long walk for 2.5e-5.
 __host__ __device__ constexpr bool acc_leaves(int j, int nb) { return j > 0 && j % kPrefillAccBlocks == 0 && nb - j >= kPrefillAccRest; }
 static_assert(kPrefillAccBlocks % 2 == 0, "the first softmax team takes the sums");
