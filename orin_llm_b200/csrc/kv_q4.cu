@@ -29,8 +29,8 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) { float r; a
 // or four (HD 64) share a row, four lanes a 64-dim group, a lane 16 dims: the 8 of word t, i and the 8 of word t, i + 1, so that
 // it owns two neighbouring code words of K, and the minimum and maximum of a group cost two shuffles.  The block is put
 // together in shared memory and leaves in 16-byte pieces; of a block at either end of the range only the stored rows' bytes do.
-// Bound by the fp32 rows it reads, 1024 bytes per position and head against 144 written: 16384 positions of 8 heads take 34 us
-// on a cold cache (4.5 TB/s, 0.69 of the measured copy bandwidth), with the issue slots 68 % busy and 4.5 cycles per issue
+// Bound by the fp32 rows it reads, 1024 bytes per position and head against 144 written: 16384 positions of 8 heads take 33.4 us
+// on a cold cache (4.6 TB/s, 0.70 of the measured copy bandwidth), with the issue slots 62 % busy and 5.4 cycles per issue
 // spent on loads -- neither alone is the limit.  A warp per row, four or two values a lane, needs five shuffles twice per
 // row and a double division per row instead of per four: 49 us against 21 for 8192 positions.  The heads of a block are
 // neighbours in the grid because they are neighbours in the rows.

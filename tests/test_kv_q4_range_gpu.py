@@ -74,6 +74,33 @@ def test_a_long_chunk_repeats_itself(ops, n_head, n_kv, hd, past, batch):
         assert float((outs[0][:, h] - want).norm() / want.norm()) <= 1e-3
 
 
+@pytest.mark.parametrize("n_head,n_kv,hd,past,batch,half", [(32, 8, 128, 9000, 512, False), (16, 1, 64, 70000, 140, True)])
+def test_a_long_chunk_captured(ops, n_head, n_kv, hd, past, batch, half):
+    """A call whose sums pass through the workspace, replayed over a workspace that held something else in between: the same bits."""
+    n, scale = past + batch, 1.0 / math.sqrt(hd)
+    raw, _, _ = long_cache(ops, n_kv, hd, n)
+    gen = torch.Generator(device="cuda").manual_seed(402)
+    q = 2 * torch.randn(batch, n_head, hd, device="cuda", generator=gen)
+    kn, vn = (torch.randn(batch, n_kv, hd, device="cuda", generator=gen) for _ in range(2))
+    ws = torch.empty(ops.prefill_q4_workspace(n_head, n_kv, hd, batch, n).numel(), dtype=torch.uint8, device="cuda")
+    want, got = (torch.zeros(batch, n_head, hd, dtype=torch.float16 if half else torch.float32, device="cuda") for _ in range(2))
+
+    def call(out):
+        ops.attn_prefill_q4(q, kn, vn, raw, out, n_head, n_kv, hd, n, past, batch, scale, ops.FUSE_ALL, (1, hd, 1e6, None), ws)
+
+    call(want)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(got)
+    for fill in (0, 255):                                  # (255: NaN wherever it is read as a number)
+        got.zero_()
+        ws.fill_(fill)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and bool(torch.isfinite(got).all())
+
+
 # ------------------------------------------------------------------------------------------------- steps
 def repeated_row(rng, n_kv, hd, n, step, at, amp=1.0):
     """A cache of n rows that are all alike -- K zero, V of about 15 steps -- but for row `at`, whose K is amp times a random row and
